@@ -1,0 +1,461 @@
+// The paged key / value cache: head norms, rotation and the write in one
+// launch, reading rows back, and moving accepted drafted tokens.
+#include "nkt_attn_device.h"
+
+namespace nkt {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWindow = 64;  // tokens of one value window: one per lane of a wave
+
+// Tokens per 16-byte piece of the value layout.
+template <bool I8>
+constexpr int kUnit = I8 ? 16 : 8;
+
+// Maximum over groups of N lanes of |x| as ordered bits: a NaN is above
+// every number, so it is not lost.
+template <int N>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#pragma unroll
+  for (int off = N / 2; off >= 1; off >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)v, off);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int off = N / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off);
+  return v;
+}
+
+// The scale of a row with this maximum; NaN for a row with a NaN or an
+// infinity, whose codes then do not matter.
+__device__ __forceinline__ float scale_from_max(uint32_t max_bits) {
+  const float s = __uint_as_float(max_bits) / 127.0f;
+  return max_bits >= 0x7f800000u ? __builtin_nanf("") : s == 0.0f ? 1.0f : s;
+}
+// round-half-even(x / scale)
+__device__ __forceinline__ uint32_t code_of(float x, float scale) {
+  const float r = __builtin_rintf(x / scale);
+  return (uint32_t)(int)fminf(fmaxf(r, -127.0f), 127.0f) & 0xffu;
+}
+
+__device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f32(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Pieces and single tokens of a 64-token window: lane l holds token l's slot
+// (-1: none).  Returns the tokens at which a run of U consecutive slots fills
+// one 16-byte piece of the value layout (bit l); *single: the other stored ones.
+template <int U>
+__device__ __forceinline__ uint64_t whole_pieces(int64_t slot, int lane, uint64_t* single) {
+  const int64_t before = ((int64_t)__shfl_up((int)(slot >> 32), 1) << 32) | (uint32_t)__shfl_up((int)slot, 1);
+  const bool stored = slot >= 0;
+  const uint64_t valid = __ballot(stored);
+  const uint64_t follows = __ballot(lane > 0 && stored && slot == before + 1);
+  constexpr uint64_t kRun = (1ull << (U - 1)) - 1;
+  const uint64_t next = lane < 63 ? follows >> (lane + 1) : 0;
+  const bool whole = stored && lane + U <= 64 && (slot & (U - 1)) == 0 && (next & kRun) == kRun;
+  const uint64_t pieces = __ballot(whole);
+  uint64_t covered = 0;
+#pragma unroll
+  for (int j = 0; j < U; ++j) covered |= pieces << j;
+  *single = valid & ~covered;
+  return pieces;
+}
+
+__device__ __forceinline__ int next_bit(uint64_t& bits) {
+  const int i = __builtin_ctzll(bits);
+  bits &= bits - 1;
+  return i;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return ((int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
+// ---------------------------------------------------------------------------
+// Write.  The first rope_blocks workgroups take the query and key rows (one
+// row of D values per D / 8 lanes, four from each half of the head, so that a
+// rotation's two values sit in one lane); the others take windows of 64 tokens
+// of one head's values, which they turn in LDS so that runs of consecutive
+// slots go out as whole 16-byte pieces of the value layout.
+// ---------------------------------------------------------------------------
+template <int D, bool I8>
+__global__ __launch_bounds__(kThreads) void write_kernel(CacheView c, WriteArgs a, int rope_blocks) {
+  constexpr int LR = D / 8;
+  constexpr int kRows = kThreads / LR;
+  const int tid = threadIdx.x;
+  const int l = tid % LR, g = tid / LR;
+  const int HK = c.kv_heads;
+  __shared__ int64_t s_slot[kWindow];
+  __shared__ __align__(16) uint8_t s_rows[kWindow * D * (I8 ? 1 : 2)];
+
+  if ((int)blockIdx.x < rope_blocks) {
+    const int H = a.heads + HK;
+    const int row = (int)blockIdx.x * kRows + g;
+    const bool live = row < a.tokens * H;
+    const int t = live ? row / H : 0;
+    const int h = live ? row - t * H : 0;
+    const bool is_k = h >= a.heads;
+    const uint16_t* src = is_k ? a.k + t * a.k_stride + (h - a.heads) * D : a.q + t * a.q_stride + h * D;
+    const u32x2 w1 = *(const u32x2*)(src + 4 * l);
+    const u32x2 w2 = *(const u32x2*)(src + D / 2 + 4 * l);
+    float x1[4] = {lo_f32(w1[0]), hi_f32(w1[0]), lo_f32(w1[1]), hi_f32(w1[1])};
+    float x2[4] = {lo_f32(w2[0]), hi_f32(w2[0]), lo_f32(w2[1]), hi_f32(w2[1])};
+    const uint16_t* nw = is_k ? a.k_norm : a.q_norm;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
+    ss = group_sum<LR>(ss);
+    if (nw) {
+      const float inv = 1.0f / __builtin_sqrtf(ss * (1.0f / D) + a.eps);
+      const u32x2 n1 = *(const u32x2*)(nw + 4 * l);
+      const u32x2 n2 = *(const u32x2*)(nw + D / 2 + 4 * l);
+      const float m1[4] = {lo_f32(n1[0]), hi_f32(n1[0]), lo_f32(n1[1]), hi_f32(n1[1])};
+      const float m2[4] = {lo_f32(n2[0]), hi_f32(n2[0]), lo_f32(n2[1]), hi_f32(n2[1])};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x1[i] *= inv * m1[i], x2[i] *= inv * m2[i];
+    }
+    const int64_t pos = a.positions[t];
+    const bool pos_ok = pos >= 0 && pos < a.rope_rows;
+    if (live && !pos_ok && l == 0) report(c.status, kBadPosition);
+    const float* rp = a.rope + (pos_ok ? pos : 0) * D;
+    const f32x4 cs = *(const f32x4*)(rp + 4 * l);
+    const f32x4 sn = *(const f32x4*)(rp + D / 2 + 4 * l);
+    float y1[4], y2[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y1[i] = pos_ok ? x1[i] * cs[i] - x2[i] * sn[i] : 0.f;
+      y2[i] = pos_ok ? x2[i] * cs[i] + x1[i] * sn[i] : 0.f;
+    }
+    // the maximum by all lanes (a wave may hold query rows beside key rows)
+    uint32_t top = 0;
+    if (I8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t b1 = __float_as_uint(y1[i]) & 0x7fffffffu, b2 = __float_as_uint(y2[i]) & 0x7fffffffu;
+        top = b1 > top ? b1 : top;
+        top = b2 > top ? b2 : top;
+      }
+      top = group_max<LR>(top);
+    }
+    if (!live) return;
+    if (!is_k) {
+      uint16_t* dst = a.q_out + ((int64_t)t * a.heads + h) * D;
+      *(u32x2*)(dst + 4 * l) = u32x2{pack_bf16x2(y1[0], y1[1]), pack_bf16x2(y1[2], y1[3])};
+      *(u32x2*)(dst + D / 2 + 4 * l) = u32x2{pack_bf16x2(y2[0], y2[1]), pack_bf16x2(y2[2], y2[3])};
+      return;
+    }
+    const int64_t slot = pos_ok ? checked_slot(c, a.slots[t]) : -1;
+    if (slot < 0) return;
+    const int off = (int)slot & ((1 << c.page_shift) - 1);
+    const int64_t at = block_of(c, slot >> c.page_shift, h - a.heads) + off * D;
+    if (!I8) {
+      uint16_t* dst = (uint16_t*)c.k + at;
+      *(u32x2*)(dst + 4 * l) = u32x2{pack_bf16x2(y1[0], y1[1]), pack_bf16x2(y1[2], y1[3])};
+      *(u32x2*)(dst + D / 2 + 4 * l) = u32x2{pack_bf16x2(y2[0], y2[1]), pack_bf16x2(y2[2], y2[3])};
+    } else {
+      const float s = scale_from_max(top);
+      uint32_t p1 = 0, p2 = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p1 |= code_of(y1[i], s) << (8 * i), p2 |= code_of(y2[i], s) << (8 * i);
+      *(uint32_t*)(c.k + at + 4 * l) = p1;
+      *(uint32_t*)(c.k + at + D / 2 + 4 * l) = p2;
+      if (l == 0) c.k_scales[scale_of(c, slot, h - a.heads)] = s;
+    }
+    return;
+  }
+
+  const int item = (int)blockIdx.x - rope_blocks;
+  const int h = item % HK;
+  const int t0 = item / HK * kWindow;
+  if (tid < kWindow) {
+    int64_t slot = -1;
+    if (t0 + tid < a.tokens) {
+      const int64_t pos = a.positions[t0 + tid];
+      if (pos >= 0 && pos < a.rope_rows) slot = checked_slot(c, a.slots[t0 + tid]);
+    }
+    s_slot[tid] = slot;
+  }
+  __syncthreads();
+  for (int r = g; r < kWindow && t0 + r < a.tokens; r += kRows) {
+    const uint16_t* src = a.v + (t0 + r) * a.v_stride + h * D + 8 * l;
+    const u32x2 w1 = *(const u32x2*)src;
+    const u32x2 w2 = *(const u32x2*)(src + 4);
+    if (!I8) {
+      *(u32x4*)(s_rows + (r * D + 8 * l) * 2) = u32x4{w1[0], w1[1], w2[0], w2[1]};
+    } else {
+      const float x[8] = {lo_f32(w1[0]), hi_f32(w1[0]), lo_f32(w1[1]), hi_f32(w1[1]),
+                          lo_f32(w2[0]), hi_f32(w2[0]), lo_f32(w2[1]), hi_f32(w2[1])};
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
+        top = b > top ? b : top;
+      }
+      top = group_max<LR>(top);
+      const float s = scale_from_max(top);
+      uint32_t p[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i >> 2] |= code_of(x[i], s) << (8 * (i & 3));
+      *(u32x2*)(s_rows + r * D + 8 * l) = u32x2{p[0], p[1]};
+      const int64_t slot = s_slot[r];
+      if (l == 0 && slot >= 0) c.v_scales[scale_of(c, slot, h)] = s;
+    }
+  }
+  __syncthreads();
+  constexpr int U = kUnit<I8>;
+  const int lane = tid & 63, wave = tid >> 6;
+  uint64_t single;
+  uint64_t pieces = whole_pieces<U>(s_slot[lane], lane, &single);
+  const int mask = (1 << c.page_shift) - 1;
+  for (int n = 0; pieces; ++n) {
+    const int t = next_bit(pieces);
+    if ((n & 3) != wave) continue;
+    const int64_t slot = uniform64(s_slot[t]);
+    uint8_t* dst = c.v + (block_of(c, slot >> c.page_shift, h) + ((int)slot & mask) * D) * (I8 ? 1 : 2);
+    for (int d = lane; d < D; d += 64) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!I8) {
+          const uint16_t* s = (const uint16_t*)s_rows + (t + 2 * i) * D + d;
+          w[i] = s[0] | (uint32_t)s[D] << 16;
+        } else {
+          const uint8_t* s = s_rows + (t + 4 * i) * D + d;
+          w[i] = s[0] | (uint32_t)s[D] << 8 | (uint32_t)s[2 * D] << 16 | (uint32_t)s[3 * D] << 24;
+        }
+      }
+      *(u32x4*)(dst + d * 16) = w;
+    }
+  }
+  for (int n = 0; single; ++n) {
+    const int t = next_bit(single);
+    if ((n & 3) != wave) continue;
+    const int64_t slot = uniform64(s_slot[t]);
+    const int off = (int)slot & mask;
+    const int64_t at = block_of(c, slot >> c.page_shift, h) + (off & ~(U - 1)) * D + (off & (U - 1));
+    for (int d = lane; d < D; d += 64) {
+      if (!I8)
+        ((uint16_t*)c.v)[at + d * U] = ((const uint16_t*)s_rows)[t * D + d];
+      else
+        c.v[at + d * U] = s_rows[t * D + d];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Read: one workgroup per window of 64 slots of one head.  Keys are rows;
+// values come out of their layout through LDS, whole pieces for runs of
+// consecutive slots.
+// ---------------------------------------------------------------------------
+template <int D, bool I8>
+__global__ __launch_bounds__(kThreads) void read_kernel(CacheView c, const int64_t* __restrict__ slots, int n,
+                                                        uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out) {
+  constexpr int LR = D / 8;
+  constexpr int kRows = kThreads / LR;
+  constexpr int U = kUnit<I8>;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int l = tid % LR, g = tid / LR;
+  const int HK = c.kv_heads;
+  const int h = (int)(blockIdx.x % (unsigned)HK);
+  const int t0 = (int)(blockIdx.x / (unsigned)HK) * kWindow;
+  const int mask = (1 << c.page_shift) - 1;
+  __shared__ int64_t s_slot[kWindow];
+  __shared__ __align__(16) uint8_t s_rows[kWindow * D * (I8 ? 1 : 2)];
+  if (tid < kWindow) s_slot[tid] = t0 + tid < n ? checked_slot(c, slots[t0 + tid]) : -1;
+  __syncthreads();
+  uint64_t single;
+  uint64_t pieces = whole_pieces<U>(s_slot[lane], lane, &single);
+  for (int i = 0; pieces; ++i) {
+    const int t = next_bit(pieces);
+    if ((i & 3) != wave) continue;
+    const int64_t slot = uniform64(s_slot[t]);
+    const uint8_t* src = c.v + (block_of(c, slot >> c.page_shift, h) + ((int)slot & mask) * D) * (I8 ? 1 : 2);
+    for (int d = lane; d < D; d += 64) {
+      const u32x4 w = *(const u32x4*)(src + d * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!I8) {
+          uint16_t* s = (uint16_t*)s_rows + (t + 2 * j) * D + d;
+          s[0] = (uint16_t)w[j];
+          s[D] = (uint16_t)(w[j] >> 16);
+        } else {
+          uint8_t* s = s_rows + (t + 4 * j) * D + d;
+          s[0] = (uint8_t)w[j];
+          s[D] = (uint8_t)(w[j] >> 8);
+          s[2 * D] = (uint8_t)(w[j] >> 16);
+          s[3 * D] = (uint8_t)(w[j] >> 24);
+        }
+      }
+    }
+  }
+  for (int i = 0; single; ++i) {
+    const int t = next_bit(single);
+    if ((i & 3) != wave) continue;
+    const int64_t slot = uniform64(s_slot[t]);
+    const int off = (int)slot & mask;
+    const int64_t at = block_of(c, slot >> c.page_shift, h) + (off & ~(U - 1)) * D + (off & (U - 1));
+    for (int d = lane; d < D; d += 64) {
+      if (!I8)
+        ((uint16_t*)s_rows)[t * D + d] = ((const uint16_t*)c.v)[at + d * U];
+      else
+        s_rows[t * D + d] = c.v[at + d * U];
+    }
+  }
+  __syncthreads();
+  for (int r = g; r < kWindow && t0 + r < n; r += kRows) {
+    const int64_t slot = s_slot[r];
+    const bool ok = slot >= 0;
+    u32x4 kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
+    if (ok) {
+      const int64_t at = block_of(c, slot >> c.page_shift, h) + ((int)slot & mask) * D + 8 * l;
+      if (!I8) {
+        kw = *(const u32x4*)((const uint16_t*)c.k + at);
+        vw = *(const u32x4*)(s_rows + (r * D + 8 * l) * 2);
+      } else {
+        const int64_t sa = scale_of(c, slot, h);
+        const float ks = c.k_scales[sa], vs = c.v_scales[sa];
+        const u32x2 kc = *(const u32x2*)(c.k + at);
+        const u32x2 vc = *(const u32x2*)(s_rows + r * D + 8 * l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int sh = 16 * (i & 1);
+          kw[i] = pack_bf16x2((float)(int8_t)(kc[i >> 1] >> sh) * ks, (float)(int8_t)(kc[i >> 1] >> (sh + 8)) * ks);
+          vw[i] = pack_bf16x2((float)(int8_t)(vc[i >> 1] >> sh) * vs, (float)(int8_t)(vc[i >> 1] >> (sh + 8)) * vs);
+        }
+      }
+    }
+    const int64_t to = ((int64_t)(t0 + r) * HK + h) * D + 8 * l;
+    *(u32x4*)(k_out + to) = kw;
+    *(u32x4*)(v_out + to) = vw;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Keep: one workgroup per (sequence, head).  A token only ever moves towards
+// the context (kept[i] >= i), so a row still to be read (kept[j] >= j) lies
+// past every row written for an earlier i < j: rows are taken in chunks, each
+// read whole before any of it is written.
+// ---------------------------------------------------------------------------
+constexpr int kKeepChunk = 16;
+
+template <int D, bool I8>
+__global__ __launch_bounds__(kThreads) void keep_kernel(CacheView c, const int32_t* __restrict__ table, int width,
+                                                        const int32_t* __restrict__ context,
+                                                        const int32_t* __restrict__ kept, int kept_width,
+                                                        const int32_t* __restrict__ counts) {
+  constexpr int U = kUnit<I8>;
+  constexpr int LR = 16;  // lanes per row
+  const int b = (int)(blockIdx.x / (unsigned)c.kv_heads), h = (int)(blockIdx.x % (unsigned)c.kv_heads);
+  const int l = threadIdx.x % LR, g = threadIdx.x / LR;  // 16 rows of a chunk
+  const int mask = (1 << c.page_shift) - 1;
+  const int64_t most = (int64_t)width << c.page_shift;
+  const int64_t base = context[b];
+  int count = counts[b];
+  if (count > kept_width || base < 0) {
+    if (threadIdx.x == 0) report(c.status, kBadKept);
+    count = base < 0 ? 0 : kept_width;
+  }
+  auto slot_of = [&](int64_t pos) -> int64_t {
+    const int64_t page = table[(int64_t)b * width + (pos >> c.page_shift)];
+    if (page < 0 || page >= c.num_pages) {
+      report(c.status, kBadPage);
+      return -1;
+    }
+    return (page << c.page_shift) | (pos & mask);
+  };
+  for (int i0 = 0; i0 < count; i0 += kKeepChunk) {
+    const int i = i0 + g;
+    int64_t from = -1, to = -1;
+    if (i < count) {
+      const int64_t src = kept[(int64_t)b * kept_width + i];
+      if (src < i || base + src >= most) {
+        if (l == 0) report(c.status, kBadKept);
+      } else if (src != i) {
+        from = slot_of(base + src);
+        to = slot_of(base + i);
+      }
+    }
+    const bool moves = from >= 0 && to >= 0;
+    uint16_t kr[D / LR], vr[D / LR];
+    float ks = 0.f, vs = 0.f;
+    if (moves) {
+      const int off = (int)from & mask;
+      const int64_t blk = block_of(c, from >> c.page_shift, h);
+      const int64_t va = blk + (off & ~(U - 1)) * D + (off & (U - 1));
+#pragma unroll
+      for (int j = 0; j < D / LR; ++j) {
+        const int d = l + LR * j;
+        kr[j] = I8 ? c.k[blk + off * D + d] : ((const uint16_t*)c.k)[blk + off * D + d];
+        vr[j] = I8 ? c.v[va + d * U] : ((const uint16_t*)c.v)[va + d * U];
+      }
+      if (I8 && l == 0) {
+        ks = c.k_scales[scale_of(c, from, h)];
+        vs = c.v_scales[scale_of(c, from, h)];
+      }
+    }
+    __syncthreads();
+    if (moves) {
+      const int off = (int)to & mask;
+      const int64_t blk = block_of(c, to >> c.page_shift, h);
+      const int64_t va = blk + (off & ~(U - 1)) * D + (off & (U - 1));
+#pragma unroll
+      for (int j = 0; j < D / LR; ++j) {
+        const int d = l + LR * j;
+        if (I8) {
+          c.k[blk + off * D + d] = (uint8_t)kr[j];
+          c.v[va + d * U] = (uint8_t)vr[j];
+        } else {
+          ((uint16_t*)c.k)[blk + off * D + d] = kr[j];
+          ((uint16_t*)c.v)[va + d * U] = vr[j];
+        }
+      }
+      if (I8 && l == 0) {
+        c.k_scales[scale_of(c, to, h)] = ks;
+        c.v_scales[scale_of(c, to, h)] = vs;
+      }
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_cache_write(const CacheView& c, const WriteArgs& a, hipStream_t stream) {
+  by_layout(c, [&](auto dim, auto int8) {
+    constexpr int D = decltype(dim)::value;
+    constexpr bool I8 = decltype(int8)::value;
+    constexpr int kRows = kThreads / (D / 8);
+    const int rope_blocks = (a.tokens * (a.heads + c.kv_heads) + kRows - 1) / kRows;
+    const int value_blocks = (a.tokens + kWindow - 1) / kWindow * c.kv_heads;
+    hipLaunchKernelGGL((write_kernel<D, I8>), dim3(rope_blocks + value_blocks), dim3(kThreads), 0, stream, c, a,
+                       rope_blocks);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_read(const CacheView& c, const int64_t* slots, int n, uint16_t* k_out, uint16_t* v_out,
+                             hipStream_t stream) {
+  by_layout(c, [&](auto dim, auto int8) {
+    hipLaunchKernelGGL((read_kernel<decltype(dim)::value, decltype(int8)::value>),
+                       dim3((n + kWindow - 1) / kWindow * c.kv_heads), dim3(kThreads), 0, stream, c, slots, n, k_out,
+                       v_out);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_keep(const CacheView& c, const int32_t* table, int width, const int32_t* context,
+                             const int32_t* kept, int kept_width, const int32_t* counts, int seqs,
+                             hipStream_t stream) {
+  by_layout(c, [&](auto dim, auto int8) {
+    hipLaunchKernelGGL((keep_kernel<decltype(dim)::value, decltype(int8)::value>), dim3(seqs * c.kv_heads),
+                       dim3(kThreads), 0, stream, c, table, width, context, kept, kept_width, counts);
+  });
+  return hipGetLastError();
+}
+
+}  // namespace nkt

@@ -1,4 +1,4 @@
-"""ctypes binding of the gfx950 MoE library (C ABI: include/nkt_moe.h).
+"""ctypes binding of the gfx950 library (C ABI: include/nkt_moe.h, include/nkt_attn.h).
 
 The binding style (explicit argtypes/restype, handle + error buffer + int
 return code) follows the reference's native bridge binding in
@@ -89,6 +89,38 @@ EXPORTED_SYMBOLS = (
     "nkt_moe_version",
 )
 
+# nkt_attn.h: cache formats, device buffers, status bits
+CACHE_BF16 = 0
+CACHE_INT8 = 1
+
+ATTN_BUF_K = 0
+ATTN_BUF_V = 1
+ATTN_BUF_K_SCALES = 2
+ATTN_BUF_V_SCALES = 3
+ATTN_BUF_STATUS = 4
+ATTN_NUM_BUFS = 5
+
+ATTN_STATUS = {
+    "bad_slot": 1,
+    "bad_position": 2,
+    "bad_page": 4,
+    "bad_length": 8,
+    "bad_kept": 16,
+}
+
+ATTN_SYMBOLS = (
+    "nkt_attn_create",
+    "nkt_attn_destroy",
+    "nkt_attn_cache_bytes",
+    "nkt_attn_bind_cache",
+    "nkt_attn_write",
+    "nkt_attn_read",
+    "nkt_attn_keep",
+    "nkt_attn_workspace_bytes",
+    "nkt_attn_forward",
+    "nkt_attn_forward_tree",
+)
+
 # bytes of the static scratch behind nkt_moe_forward_noalloc (NKT_NOALLOC_SCRATCH_BYTES)
 NOALLOC_SCRATCH_BYTES = 64 << 20
 
@@ -158,8 +190,28 @@ def lib() -> ctypes.CDLL:
     L.nkt_moe_forward_noalloc.restype = i
     L.nkt_moe_version.argtypes = []
     L.nkt_moe_version.restype = ctypes.c_char_p
+    _declare_attention(L)
     _lib = L
     return L
+
+
+def _declare_attention(L: ctypes.CDLL) -> None:
+    vp, sz, cp, i, l = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_char_p, ctypes.c_int, ctypes.c_int64
+    szp, f = ctypes.POINTER(ctypes.c_size_t), ctypes.c_float
+    L.nkt_attn_create.argtypes = [i, i, i, i, i, l, cp, sz]
+    L.nkt_attn_create.restype = vp
+    L.nkt_attn_destroy.argtypes = [vp]
+    L.nkt_attn_destroy.restype = None
+    L.nkt_attn_cache_bytes.argtypes = [vp, i, szp, cp, sz]
+    L.nkt_attn_bind_cache.argtypes = [vp, ctypes.POINTER(vp), cp, sz]
+    L.nkt_attn_write.argtypes = [vp, vp, l, vp, l, vp, l, vp, vp, vp, l, vp, vp, f, i, vp, vp, cp, sz]
+    L.nkt_attn_read.argtypes = [vp, vp, i, vp, vp, vp, cp, sz]
+    L.nkt_attn_keep.argtypes = [vp, vp, i, vp, vp, i, vp, i, vp, cp, sz]
+    L.nkt_attn_workspace_bytes.argtypes = [vp, i, i, i, i, szp, cp, sz]
+    L.nkt_attn_forward.argtypes = [vp, vp, vp, i, vp, vp, i, i, i, i, f, vp, vp, sz, vp, cp, sz]
+    L.nkt_attn_forward_tree.argtypes = [vp, vp, vp, i, vp, i, vp, vp, i, i, i, i, f, vp, vp, sz, vp, cp, sz]
+    for name in ATTN_SYMBOLS[2:]:
+        getattr(L, name).restype = i
 
 
 class ErrBuf:
