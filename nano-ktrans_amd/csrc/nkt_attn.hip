@@ -82,6 +82,11 @@ __device__ __forceinline__ float max_xor32(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+__device__ __forceinline__ float max_xor16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -1.0e38f;  // the running maximum before any score
 // The running maximum moves only when a score passes it by this much (in
@@ -101,6 +106,55 @@ __device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t* lo, uint32_t
   *hi = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u);
 }
 
+constexpr int kTileRows = 128, kTileKeys = 64;  // of the tile form
+constexpr int kRowRows = 16;                    // of the row form
+
+// How a launch is cut: items (a tile of rows of one head) x splits (of chunk
+// positions each).  Where an item's rows see more than one chunk, each split
+// leaves its weighted sum of values (fp32, not divided), running maximum and
+// sum in the workspace, and join_kernel adds them in order.
+struct Parts {
+  int items, splits, chunk;
+  float* o;   // [items, kv_heads, splits, rows, D]
+  float* ml;  // [items, kv_heads, splits, rows, 2]
+  __device__ __forceinline__ int64_t row(int item, int h, int kv_heads, int split, int rows, int r) const {
+    return (((int64_t)item * kv_heads + h) * splits + split) * rows + r;
+  }
+};
+
+__device__ __forceinline__ int first_row(const AttnArgs& a, int b) { return a.starts ? a.starts[b] : b; }
+
+// The sequence of a tile of kTileRows rows, and the tile's number in it (which
+// may lie past its rows).  Sequence b's tiles start at starts[b] G / 128 + b,
+// which ascends and leaves room for its ceil(n G / 128) tiles: the last b that
+// starts at or before this tile, found by 64 lanes at a time.
+__device__ __forceinline__ bool sequence_of_tile(const AttnArgs& a, int G, int tile, int lane, int* seq, int* block) {
+  int b = 0;
+  for (int n = a.seqs; n > 1;) {
+    const int step = (n + 63) / 64;
+    const int i = b + lane * step;
+    const bool before =
+        lane * step < n && (int64_t)first_row(a, i < a.seqs ? i : a.seqs - 1) * G / kTileRows + i <= tile;
+    const int count = __popcll(__ballot(before));
+    if (count == 0) return false;
+    const int skip = (count - 1) * step;
+    b += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  *seq = __builtin_amdgcn_readfirstlane(b);
+  *block = tile - ((int)((int64_t)first_row(a, *seq) * G / kTileRows) + *seq);
+  return *block >= 0;
+}
+
+// One past the last position that some row of rows r0 .. r0 + count - 1 sees.
+template <bool TREE>
+__device__ __forceinline__ int end_of_rows(const Seq& s, int G, int r0, int count) {
+  const int rows = s.n * G;
+  const int last = (r0 + count < rows ? r0 + count : rows) - 1;
+  const int end = s.context + last / G + 1;
+  return TREE || end > s.len ? s.len : end;
+}
+
 // ---------------------------------------------------------------------------
 // Tile form: one workgroup takes 128 rows (32 per wave) against tiles of 64
 // tokens, double-buffered in LDS.
@@ -117,7 +171,6 @@ __device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t* lo, uint32_t
 // bf16 tiles go straight from global memory into LDS, int8 ones through
 // registers (exact bf16 integers; the scales multiply scores and weights).
 // ---------------------------------------------------------------------------
-constexpr int kTileRows = 128, kTileKeys = 64;
 
 template <int D, bool I8>
 struct TileLds {
@@ -129,7 +182,7 @@ struct TileLds {
 };
 
 template <int D, bool I8, bool TREE>
-__global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, int tiles) {
+__global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int kQ = D / 16;       // Q fragments, and key products per subtile
   constexpr int kO = D / 32;       // output tiles
   constexpr int kChunks = D / 8;   // 16-byte chunks of a key row
@@ -142,30 +195,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   // on XCD i % 8) and find its keys in their L2; late tiles, which see the
   // most, first
   const int h = (int)(blockIdx.x % (unsigned)HK);
-  const int tile = tiles - 1 - (int)(blockIdx.x / (unsigned)HK);
-  // sequence b's tiles start at starts[b] G / 128 + b, ascending and with room
-  // for its ceil(n G / 128): the last b that starts at or before this tile
-  int b = 0, block;
-  if (a.starts) {
-    for (int n = a.seqs; n > 1;) {
-      const int step = (n + 63) / 64;
-      const int i = b + lane * step;
-      const bool before =
-          lane * step < n && (int64_t)a.starts[i < a.seqs ? i : a.seqs] * G / kTileRows + i <= tile;
-      const int count = __popcll(__ballot(before));
-      if (count == 0) return;
-      const int skip = (count - 1) * step;
-      b += skip;
-      n = n - skip < step ? n - skip : step;
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    block = tile - ((int)((int64_t)a.starts[b] * G / kTileRows) + b);
-  } else {
-    const int per = (G + kTileRows - 1) / kTileRows;
-    b = tile / per;
-    block = tile - b * per;
-  }
-  const Seq s = sequence(c, a, b, h == 0 && block == 0 && tid == 0);
+  const int rest = (int)(blockIdx.x / (unsigned)HK);
+  const int split = rest % part.splits;
+  const int tile = part.items - 1 - rest / part.splits;
+  int b, block;
+  if (!sequence_of_tile(a, G, tile, lane, &b, &block)) return;
+  const Seq s = sequence(c, a, b, h == 0 && block == 0 && split == 0 && tid == 0);
   const int rows = s.n * G;
   const int r0 = block * kTileRows;
   if (block < 0 || r0 >= rows) return;
@@ -178,17 +213,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 #pragma unroll
   for (int i = 0; i < kQ; ++i) qf[i] = *(const u32x4*)(a.q + qo + i * 16 + half * 8);
 
-  // the tokens that the workgroup's rows see, and what no row has to mask
-  const int first_token = r0 / G;
-  const int last_row = r0 + kTileRows < rows ? r0 + kTileRows - 1 : rows - 1;
-  const int last_token = last_row / G;
-  int end = s.len;
-  if (!TREE && s.context + last_token + 1 < end) end = s.context + last_token + 1;
-  const int open = TREE ? s.context : s.context + first_token + 1;  // positions below are seen by all
+  // the positions that the workgroup takes: its part of those that its rows see
+  const int row_end = end_of_rows<TREE>(s, G, r0, kTileRows);
+  const int begin = split * part.chunk;
+  if (split > 0 && begin >= row_end) return;
+  const int end = row_end - begin > part.chunk ? begin + part.chunk : row_end;
+  const int open = TREE ? s.context : s.context + r0 / G + 1;  // positions below are seen by all
   const int wave_first = (r0 + wave * 32 < rows ? r0 + wave * 32 : rows - 1) / G;
   const int wave_open = TREE ? s.context : s.context + wave_first + 1;
   const int wave_last = (r0 + wave * 32 + 31 < rows ? r0 + wave * 32 + 31 : rows - 1) / G;
-  const int wave_end = TREE ? end : s.context + wave_last + 1;
+  const int wave_end = TREE ? s.len : s.context + wave_last + 1;
 
   f32x16 o[kO];
 #pragma unroll
@@ -273,7 +307,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   };
 
   int buf = 0;
-  int p = find(0);
+  int p = find(begin);
   if (p < end) {
     stage(0);
     land(0);
@@ -422,6 +456,20 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   }
   l = add_xor32(l);
   if (my_row >= rows) return;
+  if (row_end > part.chunk) {  // the join adds the parts
+    const int64_t at = part.row(tile, h, HK, split, kTileRows, wave * 32 + col);
+#pragma unroll
+    for (int i = 0; i < kO; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(f32x4*)(part.o + at * D + i * 32 + 8 * (r >> 2) + 4 * half) =
+            f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+    if (half == 0) {
+      part.ml[2 * at] = m;
+      part.ml[2 * at + 1] = l;
+    }
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
   for (int i = 0; i < kO; ++i)
@@ -431,128 +479,404 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
           u32x2{pack_p(o[i][r] * inv, o[i][r + 1] * inv), pack_p(o[i][r + 2] * inv, o[i][r + 3] * inv)};
 }
 
-// One wave per (row, query head): tiles of 64 tokens, one per lane for the
-// scores (running maximum and sum in fp32), one dimension per lane for P . V.
+// ---------------------------------------------------------------------------
+// Row form: up to 16 rows of a sequence (the G heads of a decode step's token),
+// where reading keys and values is all there is.  The workgroup's four waves
+// take steps of 32 (bf16) or 64 (int8) tokens in turn, 16 KB of D = 128, and
+// load them straight into the operands of 16x16x32 matrix instructions, one
+// step ahead: no LDS and no barrier until the waves' results are added.
+//   S^T = K . Q^T, O^T = V^T . P^T as in the tile form: key row r of tile t is
+//   token (r / 4) KS / 4 + 4 t + r % 4 of the step, so that a lane's scores are
+//   the KS / 4 consecutive tokens that it must supply as P^T and whose values
+//   lie in the 16 bytes that it loads.
+// ---------------------------------------------------------------------------
 template <int D, bool I8, bool TREE>
-__global__ __launch_bounds__(64) void attn_row_kernel(CacheView c, AttnArgs a) {
-  constexpr int U = I8 ? 16 : 8;
-  const int lane = threadIdx.x;
-  const int row = (int)(blockIdx.x / (unsigned)a.heads), qh = (int)(blockIdx.x % (unsigned)a.heads);
-  const int h = qh / (a.heads / c.kv_heads);
-  __shared__ float s_q[D];
-  __shared__ float s_p[64];
-  // the row's sequence
-  int b = row, first = row, n = 1;
-  if (a.starts) {
-    b = -1;
-    for (int i0 = 0; i0 < a.seqs; i0 += 64) {
-      const int i = i0 + lane;
-      const bool mine = i < a.seqs && a.starts[i] <= row && row < a.starts[i + 1];
-      const uint64_t m = __ballot(mine);
-      if (m) b = i0 + __builtin_ctzll(m);
-    }
-    if (b < 0) return;
-    first = a.starts[b];
-    n = a.starts[b + 1] - first;
-    if (row - first >= a.max_queries) {
-      if (lane == 0) report(c.status, kBadLength);
-      return;
-    }
-  }
-  int64_t most = (int64_t)a.width << c.page_shift;
-  most = most < a.max_len ? most : a.max_len;
-  int len = a.lens[b];
-  if (len < 0 || len > most) {
-    if (lane == 0) report(c.status, kBadLength);
-    len = len < 0 ? 0 : (int)most;
-  }
-  const int context = a.lens[b] < 0 ? 0 - n : a.lens[b] - n;
-  const int last = TREE ? len - 1 : context + row - first;  // last position that may be seen
-  const int64_t qo = ((int64_t)row * a.heads + qh) * D;
-  for (int d = lane; d < D; d += 64) s_q[d] = bf16_bits_to_f32(a.q[qo + d]) * a.scale;
-  __syncthreads();
-  float m = -__builtin_huge_valf(), l = 0.f;
-  float acc[D / 64];
+__global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs a, Parts part, int blocks) {
+  constexpr int KS = I8 ? 64 : 32;  // tokens per step
+  constexpr int NT = KS / 16;       // key tiles per step
+  constexpr int KL = I8 ? D / 64 : D / 32;  // 16-byte loads per key row and lane
+  constexpr int kO = D / 16;
+  constexpr int kPad = D + 4;
+  __shared__ __align__(16) float s_o[4][kRowRows][kPad];
+  __shared__ float s_m[4][kRowRows], s_l[4][kRowRows];
+  __shared__ __align__(16) float s_scale[I8 ? 4 : 1][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int g = lane >> 4, col = lane & 15;
+  const int HK = c.kv_heads, G = a.heads / HK;
+  const int h = (int)(blockIdx.x % (unsigned)HK);
+  const int rest = (int)(blockIdx.x / (unsigned)HK);
+  const int split = rest % part.splits;
+  const int item = rest / part.splits;
+  const int b = item / blocks, block = item - b * blocks;
+  const Seq s = sequence(c, a, b, h == 0 && block == 0 && split == 0 && tid == 0);
+  const int rows = s.n * G, r0 = block * kRowRows;
+  if (r0 >= rows) return;
+  const int row_end = end_of_rows<TREE>(s, G, r0, kRowRows);
+  const int begin = split * part.chunk;
+  if (split > 0 && begin >= row_end) return;
+  const int end = row_end - begin > part.chunk ? begin + part.chunk : row_end;
+  const int row = r0 + col < rows ? r0 + col : rows - 1;
+  const int token = row / G;
+  const uint16_t* q = a.q + ((int64_t)(s.first + token) * a.heads + h * G + (row - token * G)) * D;
+  u32x4 qf[D / 32];
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j) acc[j] = 0.f;
+  for (int i = 0; i < D / 32; ++i)
+    qf[i] = *(const u32x4*)(q + (I8 ? (i >> 1) * 64 + g * 16 + (i & 1) * 8 : i * 32 + g * 8));
+  const int open = TREE ? s.context : s.context + r0 / G + 1;  // positions below are seen by all rows
+
+  f32x4 o[kO];
+#pragma unroll
+  for (int i = 0; i < kO; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = kLowest, l = 0.f;
+  const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
-  for (int p0 = 0; p0 <= last && p0 < len; p0 += 64) {
-    const int64_t page = a.table[(int64_t)b * a.width + (p0 >> c.page_shift)];
-    if (page < 0 || page >= c.num_pages) {
-      if (lane == 0) report(c.status, kBadPage);
-      continue;
-    }
-    const int64_t blk = block_of(c, page, h);
-    const int off = p0 & mask;
-    const int pos = p0 + lane;
-    bool sees = pos <= last && pos < len;
-    if (TREE && sees && pos >= context) {
-      const int j = pos - context;
-      sees = j / 64 < a.words && ((a.tree[(int64_t)row * a.words + j / 64] >> (j & 63)) & 1);
-    }
-    float s = 0.f, vs = 1.f;
-    for (int d = 0; d < D; ++d)
-      s += s_q[d] * (I8 ? (float)(int8_t)c.k[blk + (off + lane) * D + d]
-                        : bf16_bits_to_f32(((const uint16_t*)c.k)[blk + (off + lane) * D + d]));
-    if (I8) {
-      const int64_t sa = ((page * c.kv_heads + h) << c.page_shift) + off + lane;
-      s *= c.k_scales[sa];
-      vs = c.v_scales[sa];
-    }
-    s = sees ? s : -__builtin_huge_valf();
-    const float top = fmaxf(m, wave_max(s));
-    const float use = top == -__builtin_huge_valf() ? 0.f : top;
-    const float p = sees ? __expf(s - use) : 0.f;
-    const float fix = __expf(m - use);
-    l = l * fix + wave_sum_butterfly(p);
-    m = top;
-    s_p[lane] = sees ? p * vs : 0.f;
-    const uint64_t seen = __ballot(sees);
-    __syncthreads();
+  const int krow = (col >> 2) * (KS / 4) + (col & 3);
+
+  struct Step {
+    u32x4 k[NT * KL], v[kO];
+    float ks, vs;  // int8: lane's token
+    bool ok;       // the page is in the cache
+    int64_t at;    // its first token's place
+  };
+  auto load = [&](int p, Step& x) {
+    const int page = a.table[(int64_t)b * a.width + (p >> c.page_shift)];
+    x.ok = page >= 0 && page < c.num_pages;
+    x.at = (((int64_t)(x.ok ? page : 0) * HK + h) << c.page_shift) + (p & mask);
+    const uint8_t* kb = c.k + x.at * (D * (I8 ? 1 : 2)) + krow * (D * (I8 ? 1 : 2)) + g * 16;
+    const uint8_t* vb = c.v + x.at * (D * (I8 ? 1 : 2)) + (g * D + col) * 16;
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const int d = lane + 64 * j;
-      float o = acc[j] * fix;
-      for (int t = 0; t < 64; ++t) {
-        if (!(seen >> t & 1)) continue;
-        const int64_t at = blk + ((off + t) & ~(U - 1)) * D + d * U + ((off + t) & (U - 1));
-        o += s_p[t] * (I8 ? (float)(int8_t)c.v[at] : bf16_bits_to_f32(((const uint16_t*)c.v)[at]));
-      }
-      acc[j] = o;
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < KL; ++i) x.k[t * KL + i] = *(const u32x4*)(kb + t * 4 * (D * (I8 ? 1 : 2)) + i * 64);
+    if (I8) {
+      x.ks = c.k_scales[x.at + lane];
+      x.vs = c.v_scales[x.at + lane];
     }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kO; ++i) x.v[i] = *(const u32x4*)(vb + i * 256);
+  };
+  auto compute = [&](int p, Step& x) {
+    if (I8) {
+      // the codes become bf16 here, not where they are loaded (four times the registers)
+#pragma unroll
+      for (int i = 0; i < NT * KL; ++i) __asm__ volatile("" : "+v"(x.k[i]));
+    }
+    f32x4 st[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        if (!I8) {
+          st[t] = mfma_bf16(x.k[t * KL + i], qf[i], st[t]);
+        } else {
+          u32x4 lo, hi;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            uint32_t e0, e1;
+            bf16_of_codes(x.k[t * KL + i][w], &e0, &e1);
+            lo[2 * w] = e0, lo[2 * w + 1] = e1;
+            bf16_of_codes(x.k[t * KL + i][w + 2], &e0, &e1);
+            hi[2 * w] = e0, hi[2 * w + 1] = e1;
+          }
+          st[t] = mfma_bf16(lo, qf[2 * i], st[t]);
+          st[t] = mfma_bf16(hi, qf[2 * i + 1], st[t]);
+        }
+      }
+      // (one tile's bf16 operands at a time: hoisted together they spill)
+      if (I8) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (I8) {
+      // the lane's tokens' scales, by way of the wave's own LDS
+      s_scale[wave][0][lane] = x.ks * scale2;
+      s_scale[wave][1][lane] = x.vs;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const f32x4 f = *(const f32x4*)&s_scale[wave][0][g * 16 + t * 4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[t][r] *= f[r];
+      }
+    }
+    const int valid = x.ok ? s.len - p : 0;  // tokens of the step that exist
+    const bool masks = p + KS > open || valid < KS;
+    uint32_t vis = ~0u;
+    if (masks) {
+      uint64_t bits = visible<TREE>(a, s, token, p);
+      if (valid < KS) bits &= (1ull << valid) - 1;
+      vis = (uint32_t)(bits >> (g * (KS / 4)));
+      if (!x.ok && lane == 0) report(c.status, kBadPage);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[t][r] = vis >> (t * 4 + r) & 1 ? st[t][r] : -__builtin_huge_valf();
+      if (!I8) {
+        // values past the end become zero; one that is not finite, which some
+        // row may not see, is added by hand to the rows that do (0 x NaN)
+        const int inside = valid - g * 8;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kO; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t keep = (2 * j < inside ? 0xffffu : 0u) | (2 * j + 1 < inside ? 0xffff0000u : 0u);
+            x.v[i][j] &= keep;
+            odd |= non_finite_pair(x.v[i][j]);
+          }
+        if (__any(odd)) {
+          for (int t = 0; t < KS && t < valid; ++t) {
+            const uint16_t* src = (const uint16_t*)c.v + x.at * D + (t >> 3) * D * 8 + (t & 7);
+            const bool sees = bits >> t & 1;
+#pragma unroll
+            for (int i = 0; i < kO; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const uint32_t e = src[(i * 16 + g * 4 + r) * 8];
+                o[i][r] += sees && (e & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(e) : 0.f;
+              }
+          }
+#pragma unroll
+          for (int i = 0; i < kO; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if ((x.v[i][j] & 0x7f80u) == 0x7f80u) x.v[i][j] &= 0xffff0000u;
+              if ((x.v[i][j] & 0x7f800000u) == 0x7f800000u) x.v[i][j] &= 0xffffu;
+            }
+        }
+      }
+    }
+    float top = st[0][0];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, st[t][r]);
+    top = max_xor32(max_xor16(top));
+    if (!I8) top *= scale2;
+    const bool moves = top > m + kSlack;
+    if (__any(moves)) {
+      const float to = moves ? top : m;
+      const float fix = __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= fix;
+#pragma unroll
+      for (int i = 0; i < kO; ++i) o[i] *= fix;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        st[t][r] = __builtin_amdgcn_exp2f(I8 ? st[t][r] - m : st[t][r] * scale2 - m);
+        l += st[t][r];
+      }
+    if (I8) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const f32x4 f = *(const f32x4*)&s_scale[wave][1][g * 16 + t * 4];
+        // (an unseen value's scale may be anything: 0 x NaN)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[t][r] = !masks || (vis >> (t * 4 + r) & 1) ? st[t][r] * f[r] : 0.f;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    u32x4 pf[NT / 2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      pf[t >> 1][2 * (t & 1)] = pack_p(st[t][0], st[t][1]);
+      pf[t >> 1][2 * (t & 1) + 1] = pack_p(st[t][2], st[t][3]);
+    }
+#pragma unroll
+    for (int i = 0; i < kO; ++i) {
+      if (!I8) {
+        o[i] = mfma_bf16(x.v[i], pf[0], o[i]);
+      } else {
+        __asm__ volatile("" : "+v"(x.v[i]));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          u32x4 vf;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            uint32_t e0, e1;
+            bf16_of_codes(x.v[i][2 * j + w], &e0, &e1);
+            vf[2 * w] = e0, vf[2 * w + 1] = e1;
+          }
+          o[i] = mfma_bf16(vf, pf[j], o[i]);
+        }
+        if (i & 1) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  Step x0, x1;
+  int p = begin + wave * KS;
+  if (p < end) load(p, x0);
+  while (p < end) {
+    if (p + 4 * KS < end) load(p + 4 * KS, x1);
+    compute(p, x0);
+    p += 4 * KS;
+    if (p >= end) break;
+    if (p + 4 * KS < end) load(p + 4 * KS, x0);
+    compute(p, x1);
+    p += 4 * KS;
+  }
+
+  // the four waves' results, added in order
+  l = add_xor32(add_xor16(l));
+  if (g == 0) {
+    s_m[wave][col] = m;
+    s_l[wave][col] = l;
   }
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j)
-    a.out[qo + lane + 64 * j] = (uint16_t)f32_to_bf16_bits(l > 0.f || l != l ? acc[j] / l : 0.f);
+  for (int i = 0; i < kO; ++i) *(f32x4*)&s_o[wave][col][i * 16 + g * 4] = o[i];
+  __syncthreads();
+  const int r = tid >> 4, d0 = (tid & 15) * (D / 16);
+  if (r0 + r >= rows) return;
+  float top = s_m[0][r];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][r]);
+  float sum = 0.f, out[D / 16];
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) out[d] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = __builtin_amdgcn_exp2f(s_m[w][r] - top);
+    sum += s_l[w][r] * f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) out[d] += s_o[w][r][d0 + d] * f;
+  }
+  if (row_end > part.chunk) {
+    const int64_t at = part.row(item, h, HK, split, kRowRows, r);
+#pragma unroll
+    for (int d = 0; d < D / 16; d += 4)
+      *(f32x4*)(part.o + at * D + d0 + d) = f32x4{out[d], out[d + 1], out[d + 2], out[d + 3]};
+    if (d0 == 0) {
+      part.ml[2 * at] = top;
+      part.ml[2 * at + 1] = sum;
+    }
+    return;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const int tok = (r0 + r) / G;
+  uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
+#pragma unroll
+  for (int d = 0; d < D / 16; d += 4)
+    *(u32x2*)(dst + d) = u32x2{pack_p(out[d] * inv, out[d + 1] * inv), pack_p(out[d + 2] * inv, out[d + 3] * inv)};
+}
+
+// Adds the splits of one item's rows, in order: 16 rows per workgroup.
+template <int D, bool TREE, int ROWS>
+__global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Parts part, int blocks) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int HK = c.kv_heads, G = a.heads / HK;
+  constexpr int kBlocks = ROWS / 16;
+  const int h = (int)(blockIdx.x % (unsigned)HK);
+  const int rest = (int)(blockIdx.x / (unsigned)HK);
+  const int item = rest / kBlocks;
+  int b, block;
+  if (ROWS == kRowRows) {
+    b = item / blocks;
+    block = item - b * blocks;
+  } else if (!sequence_of_tile(a, G, item, lane, &b, &block)) {
+    return;
+  }
+  const Seq s = sequence(c, a, b, false);
+  const int rows = s.n * G, r0 = block * ROWS;
+  const int r = rest % kBlocks * 16 + (tid >> 4), d0 = (tid & 15) * (D / 16);
+  if (r0 >= rows) return;
+  const int row_end = end_of_rows<TREE>(s, G, r0, ROWS);
+  if (row_end <= part.chunk || r0 + r >= rows) return;
+  const int splits = (row_end + part.chunk - 1) / part.chunk;
+  float top = kLowest;
+  for (int i = 0; i < splits; ++i) top = fmaxf(top, part.ml[2 * part.row(item, h, HK, i, ROWS, r)]);
+  float sum = 0.f, out[D / 16];
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) out[d] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < splits; ++i) {
+    const int64_t at = part.row(item, h, HK, i, ROWS, r);
+    const float f = __builtin_amdgcn_exp2f(part.ml[2 * at] - top);
+    sum += part.ml[2 * at + 1] * f;
+#pragma unroll
+    for (int d = 0; d < D / 16; d += 4) {
+      const f32x4 x = *(const f32x4*)(part.o + at * D + d0 + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[d + j] += x[j] * f;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const int tok = (r0 + r) / G;
+  uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
+#pragma unroll
+  for (int d = 0; d < D / 16; d += 4)
+    *(u32x2*)(dst + d) = u32x2{pack_p(out[d] * inv, out[d + 1] * inv), pack_p(out[d + 2] * inv, out[d + 3] * inv)};
+}
+
+// The launch of a forward call: by what the caller knows without asking the
+// device (its rows and bounds).
+struct Plan {
+  bool row_form;
+  int blocks;  // row form: row blocks of a sequence
+  int rows;    // of an item
+  Parts part;
+};
+
+Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len) {
+  Plan p = {};
+  const int64_t G = heads / c.kv_heads;
+  p.row_form = max_queries * G <= kRowRows;
+  p.rows = p.row_form ? kRowRows : kTileRows;
+  p.blocks = 1;
+  p.part.items = (int)(p.row_form ? seqs : tokens * G / kTileRows + seqs);
+  const int64_t wgs = (int64_t)p.part.items * c.kv_heads;
+  // enough workgroups for the chip
+  const int64_t want = p.row_form ? 2048 : 512;
+  const int least = 256, most = p.row_form ? 1024 : 1 << 30;
+  int64_t chunk = max_len;
+  if (wgs < want) {
+    const int64_t splits = (want + wgs - 1) / wgs;
+    chunk = (max_len + splits - 1) / splits;
+  }
+  chunk = chunk < most ? chunk : most;
+  chunk = (chunk + least - 1) / least * least;
+  if (chunk < least) chunk = least;
+  p.part.chunk = (int)chunk;
+  p.part.splits = (int)((max_len + chunk - 1) / chunk);
+  if (p.part.splits < 1) p.part.splits = 1;
+  return p;
+}
+
+size_t plan_rows(const CacheView& c, const Plan& p) {
+  return p.part.splits > 1 ? (size_t)p.part.items * c.kv_heads * p.part.splits * p.rows : 0;
 }
 
 }  // namespace
 
 size_t attn_workspace_bytes(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len) {
-  return 0;
+  return plan_rows(c, plan_of(c, heads, tokens, seqs, max_queries, max_len)) * (c.dim + 2) * sizeof(float);
 }
 
 hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, hipStream_t stream) {
+  Plan p = plan_of(c, a.heads, a.tokens, a.seqs, a.max_queries, a.max_len);
+  p.part.o = (float*)workspace;
+  p.part.ml = (float*)workspace + plan_rows(c, p) * c.dim;
+  const dim3 grid((unsigned)((int64_t)p.part.items * c.kv_heads * p.part.splits));
+  const dim3 join_grid((unsigned)((int64_t)p.part.items * c.kv_heads * (p.rows / 16)));
   by_layout(c, [&](auto dim, auto int8) {
     constexpr int D = decltype(dim)::value;
     constexpr bool I8 = decltype(int8)::value;
-    const int G = a.heads / c.kv_heads;
-    if (a.max_queries * (int64_t)G > 16) {
-      const int64_t tiles = a.starts ? (int64_t)a.tokens * G / kTileRows + a.seqs
-                                     : (int64_t)a.seqs * ((G + kTileRows - 1) / kTileRows);
-      const dim3 tile_grid((unsigned)(tiles * c.kv_heads));
-      if (a.tree)
-        hipLaunchKernelGGL((attn_tile_kernel<D, I8, true>), tile_grid, dim3(256), 0, stream, c, a, (int)tiles);
+    auto launch = [&](auto tree) {
+      constexpr bool TREE = decltype(tree)::value;
+      if (p.row_form)
+        hipLaunchKernelGGL((attn_row_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part, p.blocks);
       else
-        hipLaunchKernelGGL((attn_tile_kernel<D, I8, false>), tile_grid, dim3(256), 0, stream, c, a, (int)tiles);
-      return;
-    }
-    const dim3 grid((unsigned)a.tokens * a.heads);
-    if (a.tree)
-      hipLaunchKernelGGL((attn_row_kernel<D, I8, true>), grid, dim3(64), 0, stream, c, a);
-    else
-      hipLaunchKernelGGL((attn_row_kernel<D, I8, false>), grid, dim3(64), 0, stream, c, a);
+        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
+      if (p.part.splits > 1) {
+        if (p.row_form)
+          hipLaunchKernelGGL((join_kernel<D, TREE, kRowRows>), join_grid, dim3(256), 0, stream, c, a, p.part, p.blocks);
+        else
+          hipLaunchKernelGGL((join_kernel<D, TREE, kTileRows>), join_grid, dim3(256), 0, stream, c, a, p.part, p.blocks);
+      }
+    };
+    a.tree ? launch(std::true_type{}) : launch(std::false_type{});
   });
   return hipGetLastError();
 }
