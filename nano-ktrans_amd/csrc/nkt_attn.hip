@@ -17,19 +17,21 @@ struct Seq {
   int context;  // position of its first token here (negative: more rows than tokens)
 };
 
+// (b is the same in all lanes; so is the result, held in scalar registers)
 __device__ __forceinline__ Seq sequence(const CacheView& c, const AttnArgs& a, int b, bool reports) {
   Seq s;
   s.first = b;
   s.n = 1;
   bool bad = false;
   if (a.starts) {
-    const int s0 = a.starts[b], s1 = a.starts[b + 1];
+    const int s0 = __builtin_amdgcn_readfirstlane(a.starts[b]);
+    const int s1 = __builtin_amdgcn_readfirstlane(a.starts[b + 1]);
     s.first = s0 < 0 ? 0 : s0 > a.tokens ? a.tokens : s0;
     const int end = s1 > a.tokens ? a.tokens : s1;
     s.n = end > s.first ? end - s.first : 0;
     bad = s.n > a.max_queries;
   }
-  const int len = a.lens[b];
+  const int len = __builtin_amdgcn_readfirstlane(a.lens[b]);
   s.context = (len < 0 ? 0 : len) - s.n;
   if (s.n > a.max_queries) s.n = a.max_queries;
   const int64_t table = (int64_t)a.width << c.page_shift;
@@ -66,6 +68,13 @@ __device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+
+// c + lo(w) + hi(w) of a pair of bf16
+__device__ __forceinline__ float add_pair(uint32_t w, float c) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), ones, c, false);
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -142,7 +151,8 @@ __device__ __forceinline__ bool sequence_of_tile(const AttnArgs& a, int G, int t
     n = n - skip < step ? n - skip : step;
   }
   *seq = __builtin_amdgcn_readfirstlane(b);
-  *block = tile - ((int)((int64_t)first_row(a, *seq) * G / kTileRows) + *seq);
+  const int first = __builtin_amdgcn_readfirstlane(first_row(a, *seq));
+  *block = tile - ((int)((int64_t)first * G / kTileRows) + *seq);
   return *block >= 0;
 }
 
@@ -166,27 +176,40 @@ __device__ __forceinline__ int end_of_rows(const Seq& s, int G, int r0, int coun
 //   holds token r with bits 2 and 3 swapped, which makes the scores that a lane
 //   gets the 8 consecutive tokens that it must supply as P^T, and the value
 //   layout's 16-byte pieces the V^T operand: nothing moves between lanes.
-// Keys lie in LDS as rows of 16-byte chunks, chunk c of row r at c ^ (r & 7)
-// (consecutive rows' same chunk in different banks); values as they come.
+// Keys lie in LDS as rows of 16-byte chunks, chunk c of row r at c ^ key(r):
+// the same chunk of 16 rows lies in 16 places of the 256 bytes that LDS reads
+// at a time; values as they come.
 // bf16 tiles go straight from global memory into LDS, int8 ones through
 // registers (exact bf16 integers; the scales multiply scores and weights).
 // ---------------------------------------------------------------------------
 
+// The steps of a wave form a pipeline over half tiles u of 32 tokens:
+//   S(u + 1) = K(u + 1) Q  beside the exponentials of u,
+//   O += V(u) P(u)         beside the maximum of u + 1,
+// so that the matrix cores and the vector unit work at the same time; keys run
+// one tile ahead of values, and one barrier per tile covers both.
 template <int D, bool I8>
 struct TileLds {
   __align__(16) uint8_t k[2][kTileKeys * D * 2];
   __align__(16) uint8_t v[2][kTileKeys * D * 2];
-  __align__(16) float ks[2][I8 ? kTileKeys : 4];
+  __align__(16) float ks[4][I8 ? kTileKeys : 4];  // of tile t at t & 3: read until the end of tile t
   __align__(16) float vs[2][I8 ? kTileKeys : 4];
   int flag;
 };
 
+template <int D>
+__device__ __forceinline__ int chunk_key(int r) {
+  return D == 128 ? r & 15 : r >> 1 & 7;
+}
+
 template <int D, bool I8, bool TREE>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, Parts part) {
-  constexpr int kQ = D / 16;       // Q fragments, and key products per subtile
+  constexpr int kQ = D / 16;       // Q fragments, and key products per half tile
   constexpr int kO = D / 32;       // output tiles
   constexpr int kChunks = D / 8;   // 16-byte chunks of a key row
   constexpr int kLoads = kTileKeys * D * 2 / 4096;  // 16-byte loads per thread, keys or values
+  // value fragments read ahead, in 16 tokens (int8's staging needs the registers)
+  constexpr int kVAhead = I8 && D == 128 ? 1 : 2;
   __shared__ TileLds<D, I8> lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int half = lane >> 5, col = lane & 31;
@@ -203,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const Seq s = sequence(c, a, b, h == 0 && block == 0 && split == 0 && tid == 0);
   const int rows = s.n * G;
   const int r0 = block * kTileRows;
-  if (block < 0 || r0 >= rows) return;
+  if (r0 >= rows) return;
   // this lane's row (rows past the end repeat the last one and are not stored)
   const int my_row = r0 + wave * 32 + col;
   const int row = my_row < rows ? my_row : rows - 1;
@@ -218,11 +241,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const int begin = split * part.chunk;
   if (split > 0 && begin >= row_end) return;
   const int end = row_end - begin > part.chunk ? begin + part.chunk : row_end;
-  const int open = TREE ? s.context : s.context + r0 / G + 1;  // positions below are seen by all
-  const int wave_first = (r0 + wave * 32 < rows ? r0 + wave * 32 : rows - 1) / G;
-  const int wave_open = TREE ? s.context : s.context + wave_first + 1;
-  const int wave_last = (r0 + wave * 32 + 31 < rows ? r0 + wave * 32 + 31 : rows - 1) / G;
-  const int wave_end = TREE ? s.len : s.context + wave_last + 1;
+  // positions below are seen by all rows
+  const int all_see = TREE ? s.context : s.context + r0 / G + 1;
+  const int open = all_see < s.len ? all_see : s.len;
 
   f32x16 o[kO];
 #pragma unroll
@@ -233,255 +254,362 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
 
-  // the first tile at or after p whose page is in the cache; its (page, head) block
-  int64_t block_at = 0;
-  auto find = [&](int p) {
+  // 64 entries of the page table, one per lane
+  int pages = -1, pages_at = -1;
+  // the first tile at or after p whose page is in the cache (or some p >= end); its (page, head) block
+  auto find = [&](int p, int64_t* at) __attribute__((always_inline)) {
     for (; p < end; p += kTileKeys) {
-      const int page = a.table[(int64_t)b * a.width + (p >> c.page_shift)];
+      const int i = p >> c.page_shift;
+      if (pages_at < 0 || i - pages_at >= 64) {
+        pages_at = i;
+        pages = i + lane < a.width ? a.table[(int64_t)b * a.width + i + lane] : -1;
+      }
+      const int page = __builtin_amdgcn_readlane(pages, i - pages_at);
       if (page >= 0 && page < c.num_pages) {
-        block_at = (((int64_t)page * HK + h) << c.page_shift) + (p & mask);
+        *at = (((int64_t)page * HK + h) << c.page_shift) + (p & mask);
         break;
       }
       if (tid == 0) report(c.status, kBadPage);
     }
     return p;
   };
-  // LDS row of a key tile that this thread's j-th 16 bytes belong to, and the token there
-  u32x4 kreg[I8 ? kLoads / 2 : 1], vreg[I8 ? kLoads / 2 : 1];
-  float sreg = 0.f;
-  auto stage = [&](int buf) {  // the tile of block_at
+  // Staging.  bf16: straight into LDS.  int8: into registers (load_*), from
+  // there converted into LDS (land_*): values in the first half of a tile's
+  // step and keys in the second, so that they share the registers.
+  u32x4 raw[I8 ? kLoads / 2 : 1];
+  float raw_scale = 0.f;
+  auto load_k = [&](int64_t at, int buf) __attribute__((always_inline)) {
     if (!I8) {
-      const uint8_t* kb = c.k + block_at * (D * 2);
-      const uint8_t* vb = c.v + block_at * (D * 2);
+      const uint8_t* kb = c.k + at * (D * 2);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int slot = (wave * kLoads + j) * 64 + lane;
-        const int r = slot / kChunks, ch = (slot % kChunks) ^ (r & 7);
+        const int r = slot / kChunks, ch = (slot % kChunks) ^ chunk_key<D>(r);
         const int t = (r & ~12) | (r & 4) << 1 | (r & 8) >> 1;
         load16_to_lds(kb + t * (D * 2) + ch * 16, lds.k[buf] + (wave * kLoads + j) * 1024);
-        load16_to_lds(vb + slot * 16, lds.v[buf] + (wave * kLoads + j) * 1024);
       }
     } else {
-      const uint8_t* kb = c.k + block_at * D;
-      const uint8_t* vb = c.v + block_at * D;
+      const uint8_t* kb = c.k + at * D;
 #pragma unroll
-      for (int j = 0; j < kLoads / 2; ++j) {
-        kreg[j] = *(const u32x4*)(kb + (j * 256 + tid) * 16);
-        vreg[j] = *(const u32x4*)(vb + (j * 256 + tid) * 16);
-      }
-      if (tid < 2 * kTileKeys) sreg = (tid < kTileKeys ? c.k_scales : c.v_scales)[block_at + (tid & (kTileKeys - 1))];
+      for (int j = 0; j < kLoads / 2; ++j) raw[j] = *(const u32x4*)(kb + (j * 256 + tid) * 16);
+      if (tid < kTileKeys) raw_scale = c.k_scales[at + tid];
     }
   };
-  auto land = [&](int buf) {  // int8: the staged registers into LDS
-    if (!I8) return;
+  auto load_v = [&](int64_t at, int buf) __attribute__((always_inline)) {
+    if (!I8) {
+      const uint8_t* vb = c.v + at * (D * 2);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        load16_to_lds(vb + ((wave * kLoads + j) * 64 + lane) * 16, lds.v[buf] + (wave * kLoads + j) * 1024);
+    } else {
+      const uint8_t* vb = c.v + at * D;
+#pragma unroll
+      for (int j = 0; j < kLoads / 2; ++j) raw[j] = *(const u32x4*)(vb + (j * 256 + tid) * 16);
+      if (tid < kTileKeys) raw_scale = c.v_scales[at + tid];
+    }
+  };
+  auto widen = [&](u32x4 w, u32x4* x) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t lo, hi;
+      bf16_of_codes(w[j], &lo, &hi);
+      x[j >> 1][2 * (j & 1)] = lo;
+      x[j >> 1][2 * (j & 1) + 1] = hi;
+    }
+  };
+  auto land_k = [&](int buf, int n) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kLoads / 2; ++j) {
       const int piece = j * 256 + tid;
       u32x4 x[2];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t lo, hi;
-        bf16_of_codes(kreg[j][w], &lo, &hi);
-        x[w >> 1][2 * (w & 1)] = lo;
-        x[w >> 1][2 * (w & 1) + 1] = hi;
-      }
+      __asm__ volatile("" : "+v"(raw[j]));  // (widened here, not where it is loaded)
+      widen(raw[j], x);
       const int t = piece / (D / 16), ch = piece % (D / 16) * 2;
       const int r = (t & ~12) | (t & 4) << 1 | (t & 8) >> 1;
-      *(u32x4*)(lds.k[buf] + (r * kChunks + (ch ^ (r & 7))) * 16) = x[0];
-      *(u32x4*)(lds.k[buf] + (r * kChunks + ((ch + 1) ^ (r & 7))) * 16) = x[1];
+      *(u32x4*)(lds.k[buf] + (r * kChunks + (ch ^ chunk_key<D>(r))) * 16) = x[0];
+      *(u32x4*)(lds.k[buf] + (r * kChunks + ((ch + 1) ^ chunk_key<D>(r))) * 16) = x[1];
+    }
+    if (tid < kTileKeys) lds.ks[n & 3][tid] = raw_scale * scale2;
+  };
+  auto land_v = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t lo, hi;
-        bf16_of_codes(vreg[j][w], &lo, &hi);
-        x[w >> 1][2 * (w & 1)] = lo;
-        x[w >> 1][2 * (w & 1) + 1] = hi;
-      }
+    for (int j = 0; j < kLoads / 2; ++j) {
+      const int piece = j * 256 + tid;
+      u32x4 x[2];
+      __asm__ volatile("" : "+v"(raw[j]));
+      widen(raw[j], x);
       const int g16 = piece / D, d = piece % D;
       *(u32x4*)(lds.v[buf] + ((2 * g16) * D + d) * 16) = x[0];
       *(u32x4*)(lds.v[buf] + ((2 * g16 + 1) * D + d) * 16) = x[1];
     }
-    if (tid < kTileKeys)
-      lds.ks[buf][tid] = sreg * scale2;
-    else if (tid < 2 * kTileKeys)
-      lds.vs[buf][tid - kTileKeys] = sreg;
+    if (tid < kTileKeys) lds.vs[buf][tid] = raw_scale;
   };
 
-  int buf = 0;
-  int p = find(begin);
+  // Fragments of half tile sub (register r of its scores: token sub 32 + (r >>
+  // 3) 16 + half 8 + (r & 7) of the tile).
+  u32x4 kf[kQ], vf[2 * kO];
+  auto read_k = [&](int buf, int sub) {
+    // (key rows of both half tiles have the same chunk keys)
+    int at = col * (D * 2) + (half ^ chunk_key<D>(col)) * 16;
+    if (I8 && D == 128) __asm__ volatile("" : "+v"(at));  // (no registers to hold every chunk's place)
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) kf[i] = *(const u32x4*)(lds.k[buf] + sub * 32 * (D * 2) + (at ^ 32 * i));
+  };
+  auto read_v = [&](int buf, int sub, int from, int to) {
+#pragma unroll
+    for (int kk = from; kk < to; ++kk)
+#pragma unroll
+      for (int i = 0; i < kO; ++i)
+        vf[kk * kO + i] = *(const u32x4*)(lds.v[buf] + ((sub * 4 + 2 * kk + half) * D + i * 32 + col) * 16);
+  };
+  f32x16 st;    // scores of the next half tile
+  u32x4 pf[2];  // weights of the present one
+  auto scores = [&](int from, int to) {
+    if (from == 0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[r] = 0.f;
+    }
+#pragma unroll
+    for (int i = from; i < to; ++i) st = mfma32_bf16(kf[i], qf[i], st);
+  };
+  // int8: the key scales of the scores of half tile sub
+  auto scale_scores = [&](int n, int sub) {
+    if (I8) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const f32x4 f = *(const f32x4*)(lds.ks[n & 3] + sub * 32 + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) st[q4 * 4 + j] *= f[j];
+      }
+    }
+  };
+  // the mask of half tile sub of the tile at p, where it needs one: true if so
+  auto mask_scores = [&](int sub, int p) {
+    const bool masks = p + sub * 32 + 32 > open || p + sub * 32 + 32 > end;
+    if (masks) {
+      const uint32_t vis = p < end ? (uint32_t)(visible<TREE>(a, s, token, p) >> (sub * 32 + half * 8)) : 0u;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        st[r] = vis >> ((r >> 3) * 16 + (r & 7)) & 1 ? st[r] : -__builtin_huge_valf();
+    }
+    return masks;
+  };
+  auto maximum = [&] {
+    float top = fmaxf(fmaxf(st[0], st[1]), st[2]);
+#pragma unroll
+    for (int r = 3; r < 15; r += 2) top = fmaxf(fmaxf(top, st[r]), st[r + 1]);
+    top = max_xor32(fmaxf(top, st[15]));
+    return I8 ? top : top * scale2;
+  };
+  auto rescale = [&](float top) {
+    const bool moves = top > m + kSlack;
+    if (__any(moves)) {
+      const float to = moves ? top : m;
+      const float fix = __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= fix;
+#pragma unroll
+      for (int i = 0; i < kO; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= fix;
+    }
+  };
+  // scores -> pf (buf, sub: the half tile's value scales)
+  auto weights = [&](const f32x16& x, int buf, int sub) {
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      float w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = x[q4 * 4 + j];
+        w[j] = __builtin_amdgcn_exp2f(I8 ? e - m : e * scale2 - m);
+        if (I8) l += w[j];
+      }
+      if (I8) {
+        const f32x4 f = *(const f32x4*)(lds.vs[buf] + sub * 32 + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] *= f[j];
+      }
+      pf[q4 >> 1][2 * (q4 & 1)] = pack_p(w[0], w[1]);
+      pf[q4 >> 1][2 * (q4 & 1) + 1] = pack_p(w[2], w[3]);
+      if (!I8) l = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], l));
+    }
+  };
+  auto products = [&](int from, int to) {
+#pragma unroll
+    for (int i = from; i < to; ++i) o[i % kO] = mfma32_bf16(vf[i], pf[i / kO], o[i % kO]);
+  };
+  // Values that some row must not see (or that lie past the sequence's end)
+  // would still meet a weight of zero in the matrix products: 0 x NaN.  In
+  // tiles with masked tokens, values past the end become zero, and if a
+  // value is not finite, it is added by hand to the rows that see it (int8:
+  // values' scales instead, and such rows are NaN).
+  auto clean = [&](int buf, int p) __attribute__((always_inline)) {
+    if (I8) {
+      const float f = lds.vs[buf][lane];
+      const bool odd = !(__builtin_fabsf(f) < __builtin_huge_valf());
+      const uint64_t odds = __ballot(odd);
+      if (odds == 0) return;
+      if (visible<TREE>(a, s, token, p) & odds) l = __builtin_nanf("");
+      lds_barrier();  // every wave has read the scales
+      if (wave == 0 && odd) lds.vs[buf][lane] = 0.f;
+      lds_barrier();
+      return;
+    }
+    if (tid == 0) lds.flag = 0;
+    lds_barrier();
+    bool odd = false;
+    for (int i = tid; i < kTileKeys * kChunks; i += 256) {
+      u32x4 w = *(const u32x4*)(lds.v[buf] + i * 16);
+      const int inside = s.len - p - i / D * 8;
+      if (inside < 8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] &= (2 * j < inside ? 0xffffu : 0u) | (2 * j + 1 < inside ? 0xffff0000u : 0u);
+        *(u32x4*)(lds.v[buf] + i * 16) = w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd |= non_finite_pair(w[j]);
+    }
+    if (odd) lds.flag = 1;
+    lds_barrier();
+    if (!lds.flag) return;
+    const uint64_t vis = visible<TREE>(a, s, token, p);
+    for (int t = 0; t < kTileKeys; ++t) {
+      const uint16_t* src = (const uint16_t*)lds.v[buf] + (t >> 3) * D * 8 + (t & 7);
+      const bool sees = vis >> t & 1;
+#pragma unroll
+      for (int i = 0; i < kO; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t x = src[(i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * 8];
+          o[i][r] += sees && (x & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(x) : 0.f;
+        }
+    }
+    lds_barrier();
+    for (int i = tid; i < kTileKeys * kChunks; i += 256) {
+      u32x4 w = *(const u32x4*)(lds.v[buf] + i * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
+        if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu;
+      }
+      *(u32x4*)(lds.v[buf] + i * 16) = w;
+    }
+    lds_barrier();
+  };
+
+  // tile t: at position p, in key and value buffer buf; tile t + 1: p1, its
+  // keys in the other key buffer by the time of tile t
+  int64_t at = 0, at1 = 0, at2 = 0;
+  int p = find(begin, &at);
+  int p1 = find(p + kTileKeys, &at1);
+  int n = 0;  // the tile's number; its buffers are n & 1
+  float top = kLowest;
   if (p < end) {
-    stage(0);
-    land(0);
-  }
-  while (p < end) {
+    load_k(at, 0);
+    if (I8) land_k(0, 0);
     wait_vmem();
     lds_barrier();
-    const int next = find(p + kTileKeys);
-    if (next < end) stage(buf ^ 1);
-    // Values that some row must not see (or that lie past the sequence's end)
-    // would still meet a weight of zero in the matrix products: 0 x NaN.  In
-    // tiles with masked tokens, values past the end become zero, and if a
-    // value is not finite, it is added by hand to the rows that see it.
-    uint64_t vis = ~0ull;
-    if (!I8 && p + kTileKeys > open) {
-      if (tid == 0) lds.flag = 0;
-      lds_barrier();
-      bool odd = false;
-      for (int i = tid; i < kTileKeys * kChunks; i += 256) {
-        const int t = i / D * 8;
-        u32x4 w = *(const u32x4*)(lds.v[buf] + i * 16);
-        const int inside = s.len - p - t;
-        if (inside < 8) {
+    load_v(at, 0);
+    if (I8) land_v(0);
+    if (p1 < end) load_k(at1, 1);
+    read_k(0, 0);
+    scores(0, kQ);
+    scale_scores(0, 0);
+    mask_scores(0, p);
+    top = maximum();
+    read_k(0, 1);
+    if (I8) land_k(1, 1);
+  }
+  auto tile_step = [&](auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
+    wait_vmem();
+    lds_barrier();
+    const int p2 = find(p1 + kTileKeys, &at2);
+    if (p1 < end) load_v(at1, buf ^ 1);
+    if (p + kTileKeys > open) clean(buf, p);
+    // Each group of LDS reads is issued behind the first product that waits for
+    // the group before it (the wait is for all that are under way), and the
+    // scheduler must not move it.
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t keep = (2 * j < inside ? 0xffffu : 0u) | (2 * j + 1 < inside ? 0xffff0000u : 0u);
-            w[j] &= keep;
-          }
-          *(u32x4*)(lds.v[buf] + i * 16) = w;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) odd |= non_finite_pair(w[j]);
+    for (int sub = 0; sub < 2; ++sub) {
+      rescale(top);
+      const f32x16 x = st;
+      scores(0, 1);  // of half tile 1 here, or 0 of the next tile
+      __builtin_amdgcn_sched_barrier(0);
+      read_v(buf, sub, 0, kVAhead);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(1, kQ);
+      weights(x, buf, sub);
+      __builtin_amdgcn_sched_barrier(0);
+      if (kVAhead == 1) {
+        products(0, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        read_v(buf, sub, 1, 2);
+        __builtin_amdgcn_sched_barrier(0);
+        products(1, kO);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (odd) lds.flag = 1;
-      lds_barrier();
-      if (lds.flag) {
-        vis = visible<TREE>(a, s, token, p);
-        for (int t = 0; t < kTileKeys; ++t) {
-          const uint16_t* src = (const uint16_t*)lds.v[buf] + (t >> 3) * D * 8 + (t & 7);
-          const bool sees = vis >> t & 1;
-#pragma unroll
-          for (int i = 0; i < kO; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const uint32_t x = src[(i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * 8];
-              o[i][r] += sees && (x & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(x) : 0.f;
-            }
-        }
-        lds_barrier();
-        for (int i = tid; i < kTileKeys * kChunks; i += 256) {
-          u32x4 w = *(const u32x4*)(lds.v[buf] + i * 16);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
-            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu;
-          }
-          *(u32x4*)(lds.v[buf] + i * 16) = w;
-        }
-        lds_barrier();
+      constexpr int kDone = kVAhead == 1 ? kO : 0;
+      products(kDone, kDone + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      read_k(buf ^ 1, sub);
+      __builtin_amdgcn_sched_barrier(0);
+      products(kDone + 1, 2 * kO);
+      scale_scores(n + sub, sub ^ 1);
+      top = maximum();
+      if (mask_scores(sub ^ 1, sub ? p1 : p)) top = maximum();
+      if (sub == 0) {
+        if (I8) land_v(buf ^ 1);
+        if (p2 < end) load_k(at2, buf);
       }
     }
-    if (p < wave_end) {
-      f32x16 st[2];
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[sub][r] = 0.f;
-        const int kr = sub * 32 + col;
-        const uint8_t* krow = lds.k[buf] + kr * (D * 2);
-#pragma unroll
-        for (int i = 0; i < kQ; ++i) {
-          const u32x4 kf = *(const u32x4*)(krow + ((2 * i + half) ^ (kr & 7)) * 16);
-          st[sub] = mfma32_bf16(kf, qf[i], st[sub]);
-        }
-      }
-      // register r of subtile sub: token sub 32 + (r >> 3) 16 + half 8 + (r & 7)
-      if (I8) {
-#pragma unroll
-        for (int q4 = 0; q4 < 8; ++q4) {
-          const f32x4 f = *(const f32x4*)(lds.ks[buf] + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) st[q4 >> 2][(q4 & 3) * 4 + j] *= f[j];
-        }
-      }
-      const bool masks = p + kTileKeys > wave_open || p + kTileKeys > s.len;
-      if (masks) {
-        vis = visible<TREE>(a, s, token, p) >> (8 * half);
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            st[sub][r] = vis >> (sub * 32 + (r >> 3) * 16 + (r & 7)) & 1 ? st[sub][r] : -__builtin_huge_valf();
-      }
-      float top = st[0][0];
-#pragma unroll
-      for (int r = 1; r < 32; ++r) top = fmaxf(top, st[r >> 4][r & 15]);
-      top = max_xor32(top);
-      if (!I8) top *= scale2;
-      const bool moves = top > m + kSlack;
-      if (__any(moves)) {
-        const float to = moves ? top : m;
-        const float fix = __builtin_amdgcn_exp2f(m - to);
-        m = to;
-        l *= fix;
-#pragma unroll
-        for (int i = 0; i < kO; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][r] *= fix;
-      }
-      u32x4 pf[4];
-#pragma unroll
-      for (int r = 0; r < 32; r += 2) {
-        const float s0 = st[r >> 4][r & 15], s1 = st[r >> 4][(r & 15) + 1];
-        const float p0 = __builtin_amdgcn_exp2f(I8 ? s0 - m : s0 * scale2 - m);
-        const float p1 = __builtin_amdgcn_exp2f(I8 ? s1 - m : s1 * scale2 - m);
-        l += p0 + p1;
-        st[r >> 4][r & 15] = p0;
-        st[r >> 4][(r & 15) + 1] = p1;
-      }
-      if (I8) {
-#pragma unroll
-        for (int q4 = 0; q4 < 8; ++q4) {
-          const f32x4 f = *(const f32x4*)(lds.vs[buf] + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) st[q4 >> 2][(q4 & 3) * 4 + j] *= f[j];
-        }
-        if (masks) {  // an unseen value's scale may be anything: 0 x NaN
-#pragma unroll
-          for (int r = 0; r < 32; ++r)
-            st[r >> 4][r & 15] = vis >> ((r >> 3) * 16 + (r & 7)) & 1 ? st[r >> 4][r & 15] : 0.f;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 32; r += 2) pf[r >> 3][(r & 7) >> 1] = pack_p(st[r >> 4][r & 15], st[r >> 4][(r & 15) + 1]);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-        for (int i = 0; i < kO; ++i) {
-          const u32x4 vf = *(const u32x4*)(lds.v[buf] + ((2 * kk + half) * D + i * 32 + col) * 16);
-          o[i] = mfma32_bf16(vf, pf[kk], o[i]);
-        }
-    }
-    if (next < end) land(buf ^ 1);
-    buf ^= 1;
-    p = next;
+    if (I8) land_k(buf, n + 2);
+    ++n;
+    p = p1;
+    p1 = p2;
+    at1 = at2;
+  };
+  while (p < end) {
+    tile_step(std::integral_constant<int, 0>{});
+    if (p >= end) break;
+    tile_step(std::integral_constant<int, 1>{});
   }
   l = add_xor32(l);
-  if (my_row >= rows) return;
+  // (the row again, rather than held through the loop)
+  int again = col;
+  __asm__ volatile("" : "+v"(again));
+  const int out_row = r0 + wave * 32 + again;
+  if (out_row >= rows) return;
   if (row_end > part.chunk) {  // the join adds the parts
-    const int64_t at = part.row(tile, h, HK, split, kTileRows, wave * 32 + col);
+    const int64_t to = part.row(tile, h, HK, split, kTileRows, wave * 32 + again);
 #pragma unroll
     for (int i = 0; i < kO; ++i)
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
-        *(f32x4*)(part.o + at * D + i * 32 + 8 * (r >> 2) + 4 * half) =
+        *(f32x4*)(part.o + to * D + i * 32 + 8 * (r >> 2) + 4 * half) =
             f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
     if (half == 0) {
-      part.ml[2 * at] = m;
-      part.ml[2 * at + 1] = l;
+      part.ml[2 * to] = m;
+      part.ml[2 * to + 1] = l;
     }
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const int out_token = out_row / G;
+  uint16_t* out = a.out + ((int64_t)(s.first + out_token) * a.heads + h * G + (out_row - out_token * G)) * D;
 #pragma unroll
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 16; r += 4)
-      *(u32x2*)(a.out + qo + i * 32 + 8 * (r >> 2) + 4 * half) =
+      *(u32x2*)(out + i * 32 + 8 * (r >> 2) + 4 * half) =
           u32x2{pack_p(o[i][r] * inv, o[i][r + 1] * inv), pack_p(o[i][r + 2] * inv, o[i][r + 3] * inv)};
 }
 
 // ---------------------------------------------------------------------------
 // Row form: up to 16 rows of a sequence (the G heads of a decode step's token),
-// where reading keys and values is all there is.  The workgroup's four waves
+// where reading keys and values is all there is.  The workgroup's waves
 // take steps of 32 (bf16) or 64 (int8) tokens in turn, 16 KB of D = 128, and
 // load them straight into the operands of 16x16x32 matrix instructions, one
 // step ahead: no LDS and no barrier until the waves' results are added.
@@ -491,11 +619,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 //   lie in the 16 bytes that it loads.
 // ---------------------------------------------------------------------------
 template <int D, bool I8, bool TREE>
-__global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs a, Parts part, int blocks) {
+__global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int KS = I8 ? 64 : 32;  // tokens per step
   constexpr int NT = KS / 16;       // key tiles per step
   constexpr int KL = I8 ? D / 64 : D / 32;  // 16-byte loads per key row and lane
   constexpr int kO = D / 16;
+  constexpr int kNext = 4 * KS;  // from a wave's step to its next
   constexpr int kPad = D + 4;
   __shared__ __align__(16) float s_o[4][kRowRows][kPad];
   __shared__ float s_m[4][kRowRows], s_l[4][kRowRows];
@@ -506,23 +635,26 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   const int h = (int)(blockIdx.x % (unsigned)HK);
   const int rest = (int)(blockIdx.x / (unsigned)HK);
   const int split = rest % part.splits;
-  const int item = rest / part.splits;
-  const int b = item / blocks, block = item - b * blocks;
-  const Seq s = sequence(c, a, b, h == 0 && block == 0 && split == 0 && tid == 0);
-  const int rows = s.n * G, r0 = block * kRowRows;
-  if (r0 >= rows) return;
-  const int row_end = end_of_rows<TREE>(s, G, r0, kRowRows);
+  const int b = rest / part.splits;
   const int begin = split * part.chunk;
+  // 64 entries of the page table, one per lane: all that a chunk needs (asked
+  // for before anything is known of the sequence)
+  const int page0 = begin >> c.page_shift;
+  const int pages = page0 + lane < a.width ? a.table[(int64_t)b * a.width + page0 + lane] : -1;
+  const Seq s = sequence(c, a, b, h == 0 && split == 0 && tid == 0);
+  const int rows = s.n * G;
+  if (rows == 0) return;
+  const int row_end = end_of_rows<TREE>(s, G, 0, kRowRows);
   if (split > 0 && begin >= row_end) return;
   const int end = row_end - begin > part.chunk ? begin + part.chunk : row_end;
-  const int row = r0 + col < rows ? r0 + col : rows - 1;
+  const int row = col < rows ? col : rows - 1;
   const int token = row / G;
   const uint16_t* q = a.q + ((int64_t)(s.first + token) * a.heads + h * G + (row - token * G)) * D;
   u32x4 qf[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
     qf[i] = *(const u32x4*)(q + (I8 ? (i >> 1) * 64 + g * 16 + (i & 1) * 8 : i * 32 + g * 8));
-  const int open = TREE ? s.context : s.context + r0 / G + 1;  // positions below are seen by all rows
+  const int open = TREE ? s.context : s.context + 1;  // positions below are seen by all rows
 
   f32x4 o[kO];
 #pragma unroll
@@ -538,12 +670,16 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     bool ok;       // the page is in the cache
     int64_t at;    // its first token's place
   };
+  // (where there is no such step, every lane asks for the same 16 bytes of the
+  // last one: loads behind a branch would make the waits for the step before
+  // them wait for these as well)
   auto load = [&](int p, Step& x) {
-    const int page = a.table[(int64_t)b * a.width + (p >> c.page_shift)];
+    const bool real = p < end;
+    const int page = __builtin_amdgcn_readlane(pages, ((real ? p : end - 1) >> c.page_shift) - page0);
     x.ok = page >= 0 && page < c.num_pages;
-    x.at = (((int64_t)(x.ok ? page : 0) * HK + h) << c.page_shift) + (p & mask);
-    const uint8_t* kb = c.k + x.at * (D * (I8 ? 1 : 2)) + krow * (D * (I8 ? 1 : 2)) + g * 16;
-    const uint8_t* vb = c.v + x.at * (D * (I8 ? 1 : 2)) + (g * D + col) * 16;
+    x.at = (((int64_t)(x.ok ? page : 0) * HK + h) << c.page_shift) + (real ? p & mask : 0);
+    const uint8_t* kb = c.k + x.at * (D * (I8 ? 1 : 2)) + (real ? krow * (D * (I8 ? 1 : 2)) + g * 16 : 0);
+    const uint8_t* vb = c.v + x.at * (D * (I8 ? 1 : 2)) + (real ? (g * D + col) * 16 : 0);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -710,16 +846,16 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   int p = begin + wave * KS;
   if (p < end) load(p, x0);
   while (p < end) {
-    if (p + 4 * KS < end) load(p + 4 * KS, x1);
+    load(p + kNext, x1);
     compute(p, x0);
-    p += 4 * KS;
+    p += kNext;
     if (p >= end) break;
-    if (p + 4 * KS < end) load(p + 4 * KS, x0);
+    load(p + kNext, x0);
     compute(p, x1);
-    p += 4 * KS;
+    p += kNext;
   }
 
-  // the four waves' results, added in order
+  // the waves' results, added in order
   l = add_xor32(add_xor16(l));
   if (g == 0) {
     s_m[wave][col] = m;
@@ -729,7 +865,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   for (int i = 0; i < kO; ++i) *(f32x4*)&s_o[wave][col][i * 16 + g * 4] = o[i];
   __syncthreads();
   const int r = tid >> 4, d0 = (tid & 15) * (D / 16);
-  if (r0 + r >= rows) return;
+  if (r >= rows) return;
   float top = s_m[0][r];
 #pragma unroll
   for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][r]);
@@ -744,7 +880,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     for (int d = 0; d < D / 16; ++d) out[d] += s_o[w][r][d0 + d] * f;
   }
   if (row_end > part.chunk) {
-    const int64_t at = part.row(item, h, HK, split, kRowRows, r);
+    const int64_t at = part.row(b, h, HK, split, kRowRows, r);
 #pragma unroll
     for (int d = 0; d < D / 16; d += 4)
       *(f32x4*)(part.o + at * D + d0 + d) = f32x4{out[d], out[d + 1], out[d + 2], out[d + 3]};
@@ -755,58 +891,80 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     return;
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  const int tok = (r0 + r) / G;
-  uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
+  const int tok = r / G;
+  uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r - tok * G)) * D + d0;
 #pragma unroll
   for (int d = 0; d < D / 16; d += 4)
     *(u32x2*)(dst + d) = u32x2{pack_p(out[d] * inv, out[d + 1] * inv), pack_p(out[d + 2] * inv, out[d + 3] * inv)};
 }
 
-// Adds the splits of one item's rows, in order: 16 rows per workgroup.
-template <int D, bool TREE, int ROWS>
-__global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Parts part, int blocks) {
+// Adds the splits of an item's rows.  A workgroup takes 16 / SP rows, each by
+// SP x 16 threads: thread group i the splits i, i + SP, ... in order, then the
+// groups in order (the same sums whatever the batch).
+template <int D, bool TREE, int ROWS, int SP>
+__global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Parts part, int row_blocks) {
+  constexpr int kRows = 16 / SP, kN = D / 16;
+  __shared__ float s_m[16], s_l[16];
+  __shared__ __align__(16) float s_o[16][D];
   const int tid = threadIdx.x, lane = tid & 63;
   const int HK = c.kv_heads, G = a.heads / HK;
-  constexpr int kBlocks = ROWS / 16;
   const int h = (int)(blockIdx.x % (unsigned)HK);
   const int rest = (int)(blockIdx.x / (unsigned)HK);
-  const int item = rest / kBlocks;
-  int b, block;
-  if (ROWS == kRowRows) {
-    b = item / blocks;
-    block = item - b * blocks;
-  } else if (!sequence_of_tile(a, G, item, lane, &b, &block)) {
-    return;
-  }
+  const int item = rest / row_blocks;
+  int b = item, block = 0;
+  if (ROWS != kRowRows && !sequence_of_tile(a, G, item, lane, &b, &block)) return;
   const Seq s = sequence(c, a, b, false);
   const int rows = s.n * G, r0 = block * ROWS;
-  const int r = rest % kBlocks * 16 + (tid >> 4), d0 = (tid & 15) * (D / 16);
   if (r0 >= rows) return;
   const int row_end = end_of_rows<TREE>(s, G, r0, ROWS);
-  if (row_end <= part.chunk || r0 + r >= rows) return;
-  const int splits = (row_end + part.chunk - 1) / part.chunk;
-  float top = kLowest;
-  for (int i = 0; i < splits; ++i) top = fmaxf(top, part.ml[2 * part.row(item, h, HK, i, ROWS, r)]);
-  float sum = 0.f, out[D / 16];
+  if (row_end <= part.chunk) return;
+  const int group = tid >> 4, d0 = (tid & 15) * kN;
+  const int sp = group % SP;
+  const int r = rest % row_blocks * kRows + group / SP;
+  const bool live = r < ROWS && r0 + r < rows;
+  const int splits = live ? (row_end + part.chunk - 1) / part.chunk : 0;
+  float m = kLowest, l = 0.f, out[kN];
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) out[d] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < splits; ++i) {
+  for (int d = 0; d < kN; ++d) out[d] = 0.f;
+  for (int i = sp; i < splits; i += SP) {
     const int64_t at = part.row(item, h, HK, i, ROWS, r);
-    const float f = __builtin_amdgcn_exp2f(part.ml[2 * at] - top);
-    sum += part.ml[2 * at + 1] * f;
+    const float mi = part.ml[2 * at], li = part.ml[2 * at + 1];
+    const float to = fmaxf(m, mi);
+    const float f = __builtin_amdgcn_exp2f(m - to), fi = __builtin_amdgcn_exp2f(mi - to);
+    m = to;
+    l = l * f + li * fi;
 #pragma unroll
-    for (int d = 0; d < D / 16; d += 4) {
+    for (int d = 0; d < kN; d += 4) {
       const f32x4 x = *(const f32x4*)(part.o + at * D + d0 + d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) out[d + j] += x[j] * f;
+      for (int j = 0; j < 4; ++j) out[d + j] = out[d + j] * f + x[j] * fi;
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  if ((tid & 15) == 0) {
+    s_m[group] = m;
+    s_l[group] = l;
+  }
+#pragma unroll
+  for (int d = 0; d < kN; d += 4) *(f32x4*)&s_o[group][d0 + d] = f32x4{out[d], out[d + 1], out[d + 2], out[d + 3]};
+  __syncthreads();
+  if (sp != 0 || !live) return;
+#pragma unroll
+  for (int i = 1; i < SP; ++i) m = fmaxf(m, s_m[group + i]);
+  l = 0.f;
+#pragma unroll
+  for (int d = 0; d < kN; ++d) out[d] = 0.f;
+#pragma unroll
+  for (int i = 0; i < SP; ++i) {
+    const float f = __builtin_amdgcn_exp2f(s_m[group + i] - m);
+    l += s_l[group + i] * f;
+#pragma unroll
+    for (int d = 0; d < kN; ++d) out[d] += s_o[group + i][d0 + d] * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
   const int tok = (r0 + r) / G;
   uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
 #pragma unroll
-  for (int d = 0; d < D / 16; d += 4)
+  for (int d = 0; d < kN; d += 4)
     *(u32x2*)(dst + d) = u32x2{pack_p(out[d] * inv, out[d + 1] * inv), pack_p(out[d + 2] * inv, out[d + 3] * inv)};
 }
 
@@ -814,8 +972,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
 // device (its rows and bounds).
 struct Plan {
   bool row_form;
-  int blocks;  // row form: row blocks of a sequence
-  int rows;    // of an item
+  int rows;  // of an item
   Parts part;
 };
 
@@ -824,23 +981,30 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
   const int64_t G = heads / c.kv_heads;
   p.row_form = max_queries * G <= kRowRows;
   p.rows = p.row_form ? kRowRows : kTileRows;
-  p.blocks = 1;
   p.part.items = (int)(p.row_form ? seqs : tokens * G / kTileRows + seqs);
   const int64_t wgs = (int64_t)p.part.items * c.kv_heads;
-  // enough workgroups for the chip
-  const int64_t want = p.row_form ? 2048 : 512;
-  const int least = 256, most = p.row_form ? 1024 : 1 << 30;
-  int64_t chunk = max_len;
-  if (wgs < want) {
-    const int64_t splits = (want + wgs - 1) / wgs;
-    chunk = (max_len + splits - 1) / splits;
+  int64_t splits = 1, most = (int64_t)1 << 30;
+  if (p.row_form) {
+    // One workgroup reads about 57 GB/s, 100 of them what HBM gives: fewer
+    // share the contexts (one request, bf16, D = 128, in us: 1000 tokens 8.9
+    // against 13.6, 2000 9.2 against 22), but under 640 tokens a second launch
+    // costs what the split gains (517 tokens: 8.3 for both launches, 9.0 for
+    // one).  More only split what would run on after the others: chunks of
+    // 2048 against 4096 tokens, 32 x 4000 tokens 52 against 60.
+    if (wgs < 100 && max_len > 640) splits = (256 + wgs - 1) / wgs;
+    most = 2048;
+  } else if (wgs < 1536) {
+    // Three rounds of workgroups (two run on a CU at a time) even out what
+    // they see: three chunks of 1021 on up to 9000 tokens, int8, 648 workgroups:
+    // 494 us, in three parts 446, in six 447.
+    splits = (1536 + wgs - 1) / wgs;
   }
+  int64_t chunk = (max_len + splits - 1) / splits;
   chunk = chunk < most ? chunk : most;
-  chunk = (chunk + least - 1) / least * least;
-  if (chunk < least) chunk = least;
+  chunk = (chunk + 255) / 256 * 256;
+  if (chunk < 256) chunk = 256;
   p.part.chunk = (int)chunk;
-  p.part.splits = (int)((max_len + chunk - 1) / chunk);
-  if (p.part.splits < 1) p.part.splits = 1;
+  p.part.splits = max_len > chunk ? (int)((max_len + chunk - 1) / chunk) : 1;
   return p;
 }
 
@@ -859,22 +1023,31 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
   p.part.o = (float*)workspace;
   p.part.ml = (float*)workspace + plan_rows(c, p) * c.dim;
   const dim3 grid((unsigned)((int64_t)p.part.items * c.kv_heads * p.part.splits));
-  const dim3 join_grid((unsigned)((int64_t)p.part.items * c.kv_heads * (p.rows / 16)));
   by_layout(c, [&](auto dim, auto int8) {
     constexpr int D = decltype(dim)::value;
     constexpr bool I8 = decltype(int8)::value;
     auto launch = [&](auto tree) {
       constexpr bool TREE = decltype(tree)::value;
       if (p.row_form)
-        hipLaunchKernelGGL((attn_row_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part, p.blocks);
+        hipLaunchKernelGGL((attn_row_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
       else
         hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
-      if (p.part.splits > 1) {
-        if (p.row_form)
-          hipLaunchKernelGGL((join_kernel<D, TREE, kRowRows>), join_grid, dim3(256), 0, stream, c, a, p.part, p.blocks);
-        else
-          hipLaunchKernelGGL((join_kernel<D, TREE, kTileRows>), join_grid, dim3(256), 0, stream, c, a, p.part, p.blocks);
-      }
+      if (p.part.splits == 1) return;
+      auto join = [&](auto rows, auto sp, int used) {
+        constexpr int ROWS = decltype(rows)::value, SP = decltype(sp)::value;
+        const int row_blocks = (used + 16 / SP - 1) / (16 / SP);
+        hipLaunchKernelGGL((join_kernel<D, TREE, ROWS, SP>), dim3((unsigned)(p.part.items * c.kv_heads * row_blocks)),
+                           dim3(256), 0, stream, c, a, p.part, row_blocks);
+      };
+      const int G = a.heads / c.kv_heads;
+      typedef std::integral_constant<int, 4> Few;
+      typedef std::integral_constant<int, 16> Many;
+      if (!p.row_form)
+        join(std::integral_constant<int, kTileRows>{}, Few{}, kTileRows);
+      else if (p.part.splits <= 8)
+        join(std::integral_constant<int, kRowRows>{}, Few{}, a.max_queries * G);
+      else
+        join(std::integral_constant<int, kRowRows>{}, Many{}, a.max_queries * G);
     };
     a.tree ? launch(std::true_type{}) : launch(std::false_type{});
   });
