@@ -64,12 +64,6 @@ __device__ __forceinline__ uint64_t visible(const AttnArgs& a, const Seq& s, int
   return bits & valid;
 }
 
-__device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
-}
-
 // c + lo(w) + hi(w) of a pair of bf16
 __device__ __forceinline__ float add_pair(uint32_t w, float c) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -430,8 +424,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] *= f[j];
       }
-      pf[q4 >> 1][2 * (q4 & 1)] = pack_p(w[0], w[1]);
-      pf[q4 >> 1][2 * (q4 & 1) + 1] = pack_p(w[2], w[3]);
+      pf[q4 >> 1][2 * (q4 & 1)] = pack_pair(w[0], w[1]);
+      pf[q4 >> 1][2 * (q4 & 1) + 1] = pack_pair(w[2], w[3]);
       if (!I8) l = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], l));
     }
   };
@@ -604,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 #pragma unroll
     for (int r = 0; r < 16; r += 4)
       *(u32x2*)(out + i * 32 + 8 * (r >> 2) + 4 * half) =
-          u32x2{pack_p(o[i][r] * inv, o[i][r + 1] * inv), pack_p(o[i][r + 2] * inv, o[i][r + 3] * inv)};
+          u32x2{pack_pair(o[i][r] * inv, o[i][r + 1] * inv), pack_pair(o[i][r + 2] * inv, o[i][r + 3] * inv)};
 }
 
 // ---------------------------------------------------------------------------
@@ -817,8 +811,8 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     u32x4 pf[NT / 2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      pf[t >> 1][2 * (t & 1)] = pack_p(st[t][0], st[t][1]);
-      pf[t >> 1][2 * (t & 1) + 1] = pack_p(st[t][2], st[t][3]);
+      pf[t >> 1][2 * (t & 1)] = pack_pair(st[t][0], st[t][1]);
+      pf[t >> 1][2 * (t & 1) + 1] = pack_pair(st[t][2], st[t][3]);
     }
 #pragma unroll
     for (int i = 0; i < kO; ++i) {
@@ -895,7 +889,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r - tok * G)) * D + d0;
 #pragma unroll
   for (int d = 0; d < D / 16; d += 4)
-    *(u32x2*)(dst + d) = u32x2{pack_p(out[d] * inv, out[d + 1] * inv), pack_p(out[d + 2] * inv, out[d + 3] * inv)};
+    *(u32x2*)(dst + d) = u32x2{pack_pair(out[d] * inv, out[d + 1] * inv), pack_pair(out[d + 2] * inv, out[d + 3] * inv)};
 }
 
 // Adds the splits of an item's rows.  A workgroup takes 16 / SP rows, each by
@@ -965,7 +959,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
   uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
 #pragma unroll
   for (int d = 0; d < kN; d += 4)
-    *(u32x2*)(dst + d) = u32x2{pack_p(out[d] * inv, out[d + 1] * inv), pack_p(out[d + 2] * inv, out[d + 3] * inv)};
+    *(u32x2*)(dst + d) = u32x2{pack_pair(out[d] * inv, out[d + 1] * inv), pack_pair(out[d + 2] * inv, out[d + 3] * inv)};
 }
 
 // The launch of a forward call: by what the caller knows without asking the

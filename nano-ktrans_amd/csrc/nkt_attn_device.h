@@ -35,6 +35,13 @@ __device__ __forceinline__ int64_t scale_of(const CacheView& c, int64_t slot, in
   return ((page * c.kv_heads + head) << c.page_shift) + off;
 }
 
+// Two floats -> packed bf16 pair (lo = first), round to nearest even.
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+
 // fn(dim, int8) as constants: the cache's two head sizes and formats
 template <typename Fn>
 void by_layout(const CacheView& c, Fn fn) {
