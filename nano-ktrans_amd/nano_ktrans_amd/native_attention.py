@@ -26,6 +26,10 @@ from . import _native as N
 
 _FORMATS = {"bf16": N.CACHE_BF16, "int8": N.CACHE_INT8}
 
+# the current stream's handle without building a Stream object (2 us of a 12 us call)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def rope_table(max_position: int, head_dim: int, theta: float = 1e6, device=None) -> torch.Tensor:
     """fp32 [max_position, head_dim]: the cosines, then the sines, of position * theta^(-2 i / head_dim),
@@ -98,6 +102,8 @@ class NativeAttention:
         if not h:
             raise N.NativeError(f"nkt_attn_create failed: {self.err.buf.value.decode()}")
         self.handle = ctypes.c_void_p(h)
+        self._entry = {name: getattr(self.lib, name) for name in N.ATTN_SYMBOLS}
+        self._ws_bytes: Dict[Tuple[int, int, int, int], int] = {}
         int8 = cache_format == "int8"
         unit = 16 if int8 else 8
         dtype = torch.int8 if int8 else torch.bfloat16
@@ -127,15 +133,14 @@ class NativeAttention:
     # ------------------------------------------------------------------ arguments
     def _call(self, name: str, *args) -> None:
         """An entry point on this layer's device and torch's current stream there."""
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        fn = getattr(self.lib, name)
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(self.handle, *args, stream, self.err.buf, self.err.size)
+        fn, index, err = self._entry[name], self.device.index, self.err
+        if torch.cuda.current_device() == index:
+            rc = fn(self.handle, *args, _current_stream(index), err.buf, err.size)
         else:
             with torch.cuda.device(self.device):
-                rc = fn(self.handle, *args, stream, self.err.buf, self.err.size)
+                rc = fn(self.handle, *args, _current_stream(index), err.buf, err.size)
         if rc != N.NKT_OK:
-            self.err.check(rc, name)
+            err.check(rc, name)
 
     def _on_device(self, t: torch.Tensor, name: str) -> None:
         if t.device != self.device:
@@ -147,7 +152,7 @@ class NativeAttention:
             if t.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"{name} must be an integer tensor, got {t.dtype}")
             t = t.to(dtype)
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} is {tuple(t.shape)}, expected {shape}")
         return t if t.is_contiguous() else t.contiguous()
 
@@ -156,10 +161,11 @@ class NativeAttention:
         self._on_device(t, name)
         if t.dtype != torch.bfloat16:
             raise ValueError(f"{name} dtype {t.dtype}, attention expects {torch.bfloat16}")
-        if t.dim() == 2 and t.shape[1] == heads * self.head_dim:
-            t = t.unflatten(1, (heads, self.head_dim))
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim:
-            raise ValueError(f"{name} is {tuple(t.shape)}, expected [tokens, {heads}, {self.head_dim}]")
+        shape = t.shape
+        if len(shape) == 2 and shape[1] == heads * self.head_dim:
+            return t.unflatten(1, (heads, self.head_dim))
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim:
+            raise ValueError(f"{name} is {tuple(shape)}, expected [tokens, {heads}, {self.head_dim}]")
         return t
 
     def _strided(self, t: torch.Tensor, heads: int, name: str) -> torch.Tensor:
@@ -187,11 +193,11 @@ class NativeAttention:
         if w is None:
             return None
         self._on_device(w, name)
-        w = w.detach()
         if w.numel() != self.head_dim:
             raise ValueError(f"{name} must have {self.head_dim} entries, got {w.numel()}")
-        w = w.to(torch.bfloat16).reshape(-1).contiguous()
-        return w if w.data_ptr() % 8 == 0 else w.clone()
+        if w.dtype != torch.bfloat16 or w.dim() != 1 or not w.is_contiguous() or w.data_ptr() % 8:
+            w = w.detach().to(torch.bfloat16).reshape(-1).clone(memory_format=torch.contiguous_format)
+        return w
 
     # ------------------------------------------------------------------ cache
     def slots(self, page_table: torch.Tensor, seqs: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
@@ -241,7 +247,7 @@ class NativeAttention:
     def _table(self, page_table: torch.Tensor) -> torch.Tensor:
         if page_table.dim() != 2:
             raise ValueError(f"page_table is {tuple(page_table.shape)}, expected [sequences, pages]")
-        return self._ints(page_table, torch.int32, tuple(page_table.shape), "page_table")
+        return self._ints(page_table, torch.int32, page_table.shape, "page_table")
 
     def keep(self, page_table: torch.Tensor, context_lens: torch.Tensor, kept: torch.Tensor,
              counts: torch.Tensor) -> None:
@@ -259,6 +265,18 @@ class NativeAttention:
                    kept.shape[1], counts.data_ptr(), B)
 
     # ------------------------------------------------------------------ attention
+    def _workspace_bytes(self, *sizes: int) -> int:
+        """nkt_attn_workspace_bytes of a forward call's sizes (a serving loop has few of them)."""
+        need = self._ws_bytes.get(sizes)
+        if need is None:
+            nbytes = ctypes.c_size_t(0)
+            self.err.check(self.lib.nkt_attn_workspace_bytes(self.handle, *sizes, ctypes.byref(nbytes), self.err.buf,
+                                                             self.err.size), "nkt_attn_workspace_bytes")
+            if len(self._ws_bytes) >= 4096:
+                self._ws_bytes.clear()
+            need = self._ws_bytes[sizes] = nbytes.value
+        return need
+
     def _attend(self, name: str, q, head_args, page_table, seq_lens, query_starts, max_queries, max_seq_len, out):
         q = self._dense(q, self.num_heads, "q")
         T = q.shape[0]
@@ -277,14 +295,11 @@ class NativeAttention:
         out = self._out(out, T, self.num_heads)
         if T == 0 or B == 0:
             return out
-        need = ctypes.c_size_t(0)
-        self.err.check(self.lib.nkt_attn_workspace_bytes(self.handle, T, B, max_queries, max_seq_len,
-                                                         ctypes.byref(need), self.err.buf, self.err.size),
-                       "nkt_attn_workspace_bytes")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
+        need = self._workspace_bytes(T, B, max_queries, max_seq_len)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._call(name, q.data_ptr(), *head_args, page_table.data_ptr(), W, seq_lens.data_ptr(),
                    query_starts.data_ptr() if query_starts is not None else None, T, B, max_queries, max_seq_len,
-                   self.scale, out.data_ptr(), ws.data_ptr() if ws is not None else None, need.value)
+                   self.scale, out.data_ptr(), ws.data_ptr() if ws is not None else None, need)
         return out
 
     def forward(self, q: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
