@@ -892,14 +892,14 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     *(u32x2*)(dst + d) = u32x2{pack_pair(out[d] * inv, out[d + 1] * inv), pack_pair(out[d + 2] * inv, out[d + 3] * inv)};
 }
 
-// Adds the splits of an item's rows.  A workgroup takes 16 / SP rows, each by
-// SP x 16 threads: thread group i the splits i, i + SP, ... in order, then the
-// groups in order (the same sums whatever the batch).
+// Adds the splits of an item's rows.  A workgroup takes 16 / SP rows at a time,
+// each by SP x 16 threads: thread group i the splits i, i + SP, ... in order,
+// then the groups in order (the same sums whatever the batch).
 template <int D, bool TREE, int ROWS, int SP>
 __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Parts part, int row_blocks) {
   constexpr int kRows = 16 / SP, kN = D / 16;
   __shared__ float s_m[16], s_l[16];
-  __shared__ __align__(16) float s_o[16][D];
+  __shared__ __align__(16) float s_o[16][SP > 1 ? D : 4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int HK = c.kv_heads, G = a.heads / HK;
   const int h = (int)(blockIdx.x % (unsigned)HK);
@@ -912,54 +912,64 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
   if (r0 >= rows) return;
   const int row_end = end_of_rows<TREE>(s, G, r0, ROWS);
   if (row_end <= part.chunk) return;
+  const int splits = (row_end + part.chunk - 1) / part.chunk;
+  const int used = rows - r0 < ROWS ? rows - r0 : ROWS;
   const int group = tid >> 4, d0 = (tid & 15) * kN;
   const int sp = group % SP;
-  const int r = rest % row_blocks * kRows + group / SP;
-  const bool live = r < ROWS && r0 + r < rows;
-  const int splits = live ? (row_end + part.chunk - 1) / part.chunk : 0;
-  float m = kLowest, l = 0.f, out[kN];
+  for (int base = rest % row_blocks * kRows; base < used; base += row_blocks * kRows) {
+    const int r = base + group / SP;
+    float m = kLowest, l = 0.f, out[kN];
 #pragma unroll
-  for (int d = 0; d < kN; ++d) out[d] = 0.f;
-  for (int i = sp; i < splits; i += SP) {
-    const int64_t at = part.row(item, h, HK, i, ROWS, r);
-    const float mi = part.ml[2 * at], li = part.ml[2 * at + 1];
-    const float to = fmaxf(m, mi);
-    const float f = __builtin_amdgcn_exp2f(m - to), fi = __builtin_amdgcn_exp2f(mi - to);
-    m = to;
-    l = l * f + li * fi;
+    for (int d = 0; d < kN; ++d) out[d] = 0.f;
+    for (int i = sp; i < splits && r < used; i += SP) {
+      const int64_t at = part.row(item, h, HK, i, ROWS, r);
+      const float mi = part.ml[2 * at], li = part.ml[2 * at + 1];
+      const float to = fmaxf(m, mi);
+      const float f = __builtin_amdgcn_exp2f(m - to), fi = __builtin_amdgcn_exp2f(mi - to);
+      m = to;
+      l = l * f + li * fi;
 #pragma unroll
-    for (int d = 0; d < kN; d += 4) {
-      const f32x4 x = *(const f32x4*)(part.o + at * D + d0 + d);
+      for (int d = 0; d < kN; d += 4) {
+        const f32x4 x = *(const f32x4*)(part.o + at * D + d0 + d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) out[d + j] = out[d + j] * f + x[j] * fi;
+        for (int j = 0; j < 4; ++j) out[d + j] = out[d + j] * f + x[j] * fi;
+      }
+    }
+    if (SP > 1) {
+      __syncthreads();  // (of the rows before, the sums are read)
+      if ((tid & 15) == 0) {
+        s_m[group] = m;
+        s_l[group] = l;
+      }
+#pragma unroll
+      for (int d = 0; d < kN; d += 4)
+        *(f32x4*)&s_o[group][SP > 1 ? d0 + d : 0] = f32x4{out[d], out[d + 1], out[d + 2], out[d + 3]};
+      __syncthreads();
+      if (sp == 0) {
+#pragma unroll
+        for (int i = 1; i < SP; ++i) m = fmaxf(m, s_m[group + i]);
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < kN; ++d) out[d] = 0.f;
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+          const float f = __builtin_amdgcn_exp2f(s_m[group + i] - m);
+          l += s_l[group + i] * f;
+#pragma unroll
+          for (int d = 0; d < kN; ++d) out[d] += s_o[group + i][SP > 1 ? d0 + d : 0] * f;
+        }
+      }
+    }
+    if (sp == 0 && r < used) {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const int tok = (r0 + r) / G;
+      uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
+#pragma unroll
+      for (int d = 0; d < kN; d += 4)
+        *(u32x2*)(dst + d) =
+            u32x2{pack_pair(out[d] * inv, out[d + 1] * inv), pack_pair(out[d + 2] * inv, out[d + 3] * inv)};
     }
   }
-  if ((tid & 15) == 0) {
-    s_m[group] = m;
-    s_l[group] = l;
-  }
-#pragma unroll
-  for (int d = 0; d < kN; d += 4) *(f32x4*)&s_o[group][d0 + d] = f32x4{out[d], out[d + 1], out[d + 2], out[d + 3]};
-  __syncthreads();
-  if (sp != 0 || !live) return;
-#pragma unroll
-  for (int i = 1; i < SP; ++i) m = fmaxf(m, s_m[group + i]);
-  l = 0.f;
-#pragma unroll
-  for (int d = 0; d < kN; ++d) out[d] = 0.f;
-#pragma unroll
-  for (int i = 0; i < SP; ++i) {
-    const float f = __builtin_amdgcn_exp2f(s_m[group + i] - m);
-    l += s_l[group + i] * f;
-#pragma unroll
-    for (int d = 0; d < kN; ++d) out[d] += s_o[group + i][d0 + d] * f;
-  }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const int tok = (r0 + r) / G;
-  uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
-#pragma unroll
-  for (int d = 0; d < kN; d += 4)
-    *(u32x2*)(dst + d) = u32x2{pack_pair(out[d] * inv, out[d + 1] * inv), pack_pair(out[d + 2] * inv, out[d + 3] * inv)};
 }
 
 // The launch of a forward call: by what the caller knows without asking the
@@ -977,7 +987,7 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
   p.rows = p.row_form ? kRowRows : kTileRows;
   p.part.items = (int)(p.row_form ? seqs : tokens * G / kTileRows + seqs);
   const int64_t wgs = (int64_t)p.part.items * c.kv_heads;
-  int64_t splits = 1, most = (int64_t)1 << 30;
+  int64_t splits = 1, least = 256, most = (int64_t)1 << 30;
   if (p.row_form) {
     // One workgroup reads about 57 GB/s, 100 of them what HBM gives: fewer
     // share the contexts (one request, bf16, D = 128, in us: 1000 tokens 8.9
@@ -987,16 +997,24 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
     // 2048 against 4096 tokens, 32 x 4000 tokens 52 against 60.
     if (wgs < 100 && max_len > 640) splits = (256 + wgs - 1) / wgs;
     most = 2048;
-  } else if (wgs < 1536) {
-    // Three rounds of workgroups (two run on a CU at a time) even out what
-    // they see: three chunks of 1021 on up to 9000 tokens, int8, 648 workgroups:
-    // 494 us, in three parts 446, in six 447.
+  } else if (wgs < 512) {
+    // About one and a half rounds of workgroups (two run on a CU at a time);
+    // in us, for 512, 768 and 1536 of them: 1000 tokens bf16 33, 31, 42; four
+    // drafts of 32 on 8000 tokens 41, 39, 52.  Parts of fewer than 256 tokens
+    // cost more than they give (512 tokens 20, in parts of 128 24), but for the
+    // least launches (a draft of 12 on 500 tokens 13.5, in parts of 128 11.5).
+    splits = (768 + wgs / 2) / wgs;
+    if (wgs <= 64) least = 128;
+  } else if (wgs < 1536 && max_len >= 4096) {
+    // Up to three rounds of long ones: parts even out the last round (chunks
+    // of 1021 on up to 9000 tokens, int8, 648 workgroups: 494 us, in three
+    // parts 440); short ones lose by it (8 x 512 tokens 41 us, in two parts 72).
     splits = (1536 + wgs - 1) / wgs;
   }
   int64_t chunk = (max_len + splits - 1) / splits;
   chunk = chunk < most ? chunk : most;
-  chunk = (chunk + 255) / 256 * 256;
-  if (chunk < 256) chunk = 256;
+  chunk = (chunk + least - 1) / least * least;
+  if (chunk < least) chunk = least;
   p.part.chunk = (int)chunk;
   p.part.splits = max_len > chunk ? (int)((max_len + chunk - 1) / chunk) : 1;
   return p;
@@ -1027,21 +1045,27 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
       else
         hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
       if (p.part.splits == 1) return;
-      auto join = [&](auto rows, auto sp, int used) {
+      auto join = [&](auto rows, auto sp, int64_t row_blocks) {
         constexpr int ROWS = decltype(rows)::value, SP = decltype(sp)::value;
-        const int row_blocks = (used + 16 / SP - 1) / (16 / SP);
         hipLaunchKernelGGL((join_kernel<D, TREE, ROWS, SP>), dim3((unsigned)(p.part.items * c.kv_heads * row_blocks)),
-                           dim3(256), 0, stream, c, a, p.part, row_blocks);
+                           dim3(256), 0, stream, c, a, p.part, (int)row_blocks);
       };
-      const int G = a.heads / c.kv_heads;
+      typedef std::integral_constant<int, 1> One;
       typedef std::integral_constant<int, 4> Few;
       typedef std::integral_constant<int, 16> Many;
-      if (!p.row_form)
-        join(std::integral_constant<int, kTileRows>{}, Few{}, kTileRows);
-      else if (p.part.splits <= 8)
-        join(std::integral_constant<int, kRowRows>{}, Few{}, a.max_queries * G);
+      typedef std::integral_constant<int, kRowRows> RowForm;
+      typedef std::integral_constant<int, kTileRows> TileForm;
+      // thread groups for a row's splits while workgroups are few; most of
+      // many would find nothing to do (a workgroup that does costs about 2 us)
+      const int row_form_rows = a.max_queries * (a.heads / c.kv_heads);
+      if (p.row_form && p.part.splits <= 8)
+        join(RowForm{}, Few{}, (row_form_rows + 3) / 4);
+      else if (p.row_form)
+        join(RowForm{}, Many{}, row_form_rows);
+      else if ((int64_t)p.part.items * c.kv_heads <= 64)
+        join(TileForm{}, Few{}, kTileRows / 4);
       else
-        join(std::integral_constant<int, kRowRows>{}, Many{}, a.max_queries * G);
+        join(TileForm{}, One{}, 2);
     };
     a.tree ? launch(std::true_type{}) : launch(std::false_type{});
   });
