@@ -109,12 +109,15 @@ int nkt_attn_keep(void* handle, const int32_t* page_table, int table_width, cons
                   const int32_t* kept, int kept_width, const int32_t* counts, int num_seqs, void* stream, char* err,
                   size_t err_len);
 
-/* Workspace of a forward call (may be 0).  max_queries: at least the most rows
- * of one sequence; max_seq_len: at least the longest sequence. */
+/* Workspace of a forward call (may be 0) of the same sizes.  max_queries: at
+ * least the most rows of one sequence (1 for calls without query_starts);
+ * max_seq_len: at least the longest sequence.  They choose the launch, so bounds
+ * far above what comes cost time.  Refused: over 2^27 rows x heads, 2^30 tokens
+ * of a sequence, or 2^24 workgroups of a launch. */
 int nkt_attn_workspace_bytes(void* handle, int num_tokens, int num_seqs, int max_queries, int max_seq_len,
                              size_t* bytes, char* err, size_t err_len);
 
-/* Causal attention over the cache: out[i] = sum_j softmax_j(scale q_i . k_j) v_j
+/* Causal attention over the cache (scale > 0): out[i] = sum_j softmax_j(scale q_i . k_j) v_j
  * over the positions j <= seq_len - n + i of the sequence's i-th row (i < n).
  * q and out bf16 [num_tokens, num_heads, D], contiguous, 16-byte aligned.  A row
  * that sees nothing is zero; rows behind the last sequence are left as they

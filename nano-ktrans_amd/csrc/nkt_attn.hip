@@ -221,14 +221,26 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const int rows = s.n * G;
   const int r0 = block * kTileRows;
   if (r0 >= rows) return;
-  // this lane's row (rows past the end repeat the last one and are not stored)
-  const int my_row = r0 + wave * 32 + col;
-  const int row = my_row < rows ? my_row : rows - 1;
-  const int token = row / G;
-  const int64_t qo = ((int64_t)(s.first + token) * a.heads + h * G + (row - token * G)) * D;
+  // This lane's row; rows past the end repeat the last one and are not stored.
+  // (Worked out again where it is needed, rather than held in registers that
+  // the loop has no room for.)
+  auto my_row = [&] {
+    int lane_col = col;
+    __asm__ volatile("" : "+v"(lane_col));
+    return r0 + wave * 32 + lane_col;
+  };
+  auto my_token = [&] {
+    const int row = my_row();
+    return (row < rows ? row : rows - 1) / G;
+  };
   u32x4 qf[kQ];
+  {
+    const int row = my_row() < rows ? my_row() : rows - 1;
+    const int token = row / G;
+    const uint16_t* q = a.q + ((int64_t)(s.first + token) * a.heads + h * G + (row - token * G)) * D;
 #pragma unroll
-  for (int i = 0; i < kQ; ++i) qf[i] = *(const u32x4*)(a.q + qo + i * 16 + half * 8);
+    for (int i = 0; i < kQ; ++i) qf[i] = *(const u32x4*)(q + i * 16 + half * 8);
+  }
 
   // the positions that the workgroup takes: its part of those that its rows see
   const int row_end = end_of_rows<TREE>(s, G, r0, kTileRows);
@@ -244,7 +256,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  float m = kLowest, l = 0.f;
+  // Running maximum (log2), sum, and what a score must pass m by for m to move:
+  // -infinity until the row has seen a token, then kSlack.
+  float m = 0.f, l = 0.f, limit = -__builtin_huge_valf();
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
 
@@ -366,22 +380,21 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 #pragma unroll
     for (int i = from; i < to; ++i) st = mfma32_bf16(kf[i], qf[i], st);
   };
-  // int8: the key scales of the scores of half tile sub
-  auto scale_scores = [&](int n, int sub) {
-    if (I8) {
+  // the scores of half tile sub (int8: of tile n) less the running maximum, in log2
+  auto less_maximum = [&](int n, int sub) {
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const f32x4 f = *(const f32x4*)(lds.ks[n & 3] + sub * 32 + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
+    for (int q4 = 0; q4 < 4; ++q4) {
+      f32x4 f = {scale2, scale2, scale2, scale2};
+      if (I8) f = *(const f32x4*)(lds.ks[n & 3] + sub * 32 + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) st[q4 * 4 + j] *= f[j];
-      }
+      for (int j = 0; j < 4; ++j) st[q4 * 4 + j] = __builtin_fmaf(st[q4 * 4 + j], f[j], -m);
     }
   };
   // the mask of half tile sub of the tile at p, where it needs one: true if so
   auto mask_scores = [&](int sub, int p) {
     const bool masks = p + sub * 32 + 32 > open || p + sub * 32 + 32 > end;
     if (masks) {
-      const uint32_t vis = p < end ? (uint32_t)(visible<TREE>(a, s, token, p) >> (sub * 32 + half * 8)) : 0u;
+      const uint32_t vis = p < end ? (uint32_t)(visible<TREE>(a, s, my_token(), p) >> (sub * 32 + half * 8)) : 0u;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         st[r] = vis >> ((r >> 3) * 16 + (r & 7)) & 1 ? st[r] : -__builtin_huge_valf();
@@ -392,16 +405,18 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     float top = fmaxf(fmaxf(st[0], st[1]), st[2]);
 #pragma unroll
     for (int r = 3; r < 15; r += 2) top = fmaxf(fmaxf(top, st[r]), st[r + 1]);
-    top = max_xor32(fmaxf(top, st[15]));
-    return I8 ? top : top * scale2;
+    return max_xor32(fmaxf(top, st[15]));
   };
   auto rescale = [&](float top) {
-    const bool moves = top > m + kSlack;
+    const bool moves = top > limit;
     if (__any(moves)) {
-      const float to = moves ? top : m;
-      const float fix = __builtin_amdgcn_exp2f(m - to);
-      m = to;
+      const float by = moves ? top : 0.f;
+      const float fix = limit == kSlack ? __builtin_amdgcn_exp2f(-by) : 1.f;  // (nothing to rescale before)
+      m += by;
+      limit = moves ? kSlack : limit;
       l *= fix;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[r] -= by;
 #pragma unroll
       for (int i = 0; i < kO; ++i)
 #pragma unroll
@@ -415,8 +430,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       float w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float e = x[q4 * 4 + j];
-        w[j] = __builtin_amdgcn_exp2f(I8 ? e - m : e * scale2 - m);
+        w[j] = __builtin_amdgcn_exp2f(x[q4 * 4 + j]);
         if (I8) l += w[j];
       }
       if (I8) {
@@ -444,7 +458,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       const bool odd = !(__builtin_fabsf(f) < __builtin_huge_valf());
       const uint64_t odds = __ballot(odd);
       if (odds == 0) return;
-      if (visible<TREE>(a, s, token, p) & odds) l = __builtin_nanf("");
+      if (visible<TREE>(a, s, my_token(), p) & odds) l = __builtin_nanf("");
       lds_barrier();  // every wave has read the scales
       if (wave == 0 && odd) lds.vs[buf][lane] = 0.f;
       lds_barrier();
@@ -468,7 +482,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     if (odd) lds.flag = 1;
     lds_barrier();
     if (!lds.flag) return;
-    const uint64_t vis = visible<TREE>(a, s, token, p);
+    const uint64_t vis = visible<TREE>(a, s, my_token(), p);
     for (int t = 0; t < kTileKeys; ++t) {
       const uint16_t* src = (const uint16_t*)lds.v[buf] + (t >> 3) * D * 8 + (t & 7);
       const bool sees = vis >> t & 1;
@@ -510,7 +524,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     if (p1 < end) load_k(at1, 1);
     read_k(0, 0);
     scores(0, kQ);
-    scale_scores(0, 0);
+    less_maximum(0, 0);
     mask_scores(0, p);
     top = maximum();
     read_k(0, 1);
@@ -551,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       read_k(buf ^ 1, sub);
       __builtin_amdgcn_sched_barrier(0);
       products(kDone + 1, 2 * kO);
-      scale_scores(n + sub, sub ^ 1);
+      less_maximum(n + sub, sub ^ 1);
       top = maximum();
       if (mask_scores(sub ^ 1, sub ? p1 : p)) top = maximum();
       if (sub == 0) {
@@ -571,13 +585,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     tile_step(std::integral_constant<int, 1>{});
   }
   l = add_xor32(l);
-  // (the row again, rather than held through the loop)
-  int again = col;
-  __asm__ volatile("" : "+v"(again));
-  const int out_row = r0 + wave * 32 + again;
+  const int out_row = my_row();
   if (out_row >= rows) return;
   if (row_end > part.chunk) {  // the join adds the parts
-    const int64_t to = part.row(tile, h, HK, split, kTileRows, wave * 32 + again);
+    const int64_t to = part.row(tile, h, HK, split, kTileRows, out_row - r0);
 #pragma unroll
     for (int i = 0; i < kO; ++i)
 #pragma unroll
@@ -585,7 +596,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
         *(f32x4*)(part.o + to * D + i * 32 + 8 * (r >> 2) + 4 * half) =
             f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
     if (half == 0) {
-      part.ml[2 * to] = m;
+      part.ml[2 * to] = limit == kSlack ? m : kLowest;
       part.ml[2 * to + 1] = l;
     }
     return;
@@ -986,6 +997,7 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
   p.row_form = max_queries * G <= kRowRows;
   p.rows = p.row_form ? kRowRows : kTileRows;
   p.part.items = (int)(p.row_form ? seqs : tokens * G / kTileRows + seqs);
+  if (p.part.items < 1) p.part.items = 1;
   const int64_t wgs = (int64_t)p.part.items * c.kv_heads;
   int64_t splits = 1, least = 256, most = (int64_t)1 << 30;
   if (p.row_form) {
@@ -1024,7 +1036,29 @@ size_t plan_rows(const CacheView& c, const Plan& p) {
   return p.part.splits > 1 ? (size_t)p.part.items * c.kv_heads * p.part.splits * p.rows : 0;
 }
 
+// Workgroups per item and head of the join, and its thread groups per row:
+// several for a row's splits while workgroups are few; most of many would find
+// nothing to do (a workgroup that does costs about 2 us).
+struct JoinPlan {
+  int groups;
+  int64_t row_blocks;
+};
+JoinPlan join_of(const CacheView& c, int heads, const Plan& p, int max_queries) {
+  const int64_t rows = (int64_t)max_queries * (heads / c.kv_heads);  // of the row form
+  if (p.row_form && p.part.splits <= 8) return {4, (rows + 3) / 4};
+  if (p.row_form) return {16, rows};
+  if ((int64_t)p.part.items * c.kv_heads <= 64) return {4, kTileRows / 4};
+  return {1, 2};
+}
+
 }  // namespace
+
+int64_t attn_workgroups(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len) {
+  const Plan p = plan_of(c, heads, tokens, seqs, max_queries, max_len);
+  const int64_t items = (int64_t)p.part.items * c.kv_heads;
+  const int64_t join = p.part.splits > 1 ? join_of(c, heads, p, max_queries).row_blocks : 0;
+  return items * (p.part.splits > join ? p.part.splits : join);
+}
 
 size_t attn_workspace_bytes(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len) {
   return plan_rows(c, plan_of(c, heads, tokens, seqs, max_queries, max_len)) * (c.dim + 2) * sizeof(float);
@@ -1045,27 +1079,23 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
       else
         hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
       if (p.part.splits == 1) return;
-      auto join = [&](auto rows, auto sp, int64_t row_blocks) {
-        constexpr int ROWS = decltype(rows)::value, SP = decltype(sp)::value;
-        hipLaunchKernelGGL((join_kernel<D, TREE, ROWS, SP>), dim3((unsigned)(p.part.items * c.kv_heads * row_blocks)),
-                           dim3(256), 0, stream, c, a, p.part, (int)row_blocks);
+      const JoinPlan j = join_of(c, a.heads, p, a.max_queries);
+      const dim3 join_grid((unsigned)(p.part.items * c.kv_heads * j.row_blocks));
+      auto join = [&](auto rows, auto groups) {
+        constexpr int ROWS = decltype(rows)::value, SP = decltype(groups)::value;
+        hipLaunchKernelGGL((join_kernel<D, TREE, ROWS, SP>), join_grid, dim3(256), 0, stream, c, a, p.part,
+                           (int)j.row_blocks);
       };
-      typedef std::integral_constant<int, 1> One;
-      typedef std::integral_constant<int, 4> Few;
-      typedef std::integral_constant<int, 16> Many;
-      typedef std::integral_constant<int, kRowRows> RowForm;
-      typedef std::integral_constant<int, kTileRows> TileForm;
-      // thread groups for a row's splits while workgroups are few; most of
-      // many would find nothing to do (a workgroup that does costs about 2 us)
-      const int row_form_rows = a.max_queries * (a.heads / c.kv_heads);
-      if (p.row_form && p.part.splits <= 8)
-        join(RowForm{}, Few{}, (row_form_rows + 3) / 4);
+      std::integral_constant<int, kRowRows> row_form;
+      std::integral_constant<int, kTileRows> tile_form;
+      if (p.row_form && j.groups == 4)
+        join(row_form, std::integral_constant<int, 4>{});
       else if (p.row_form)
-        join(RowForm{}, Many{}, row_form_rows);
-      else if ((int64_t)p.part.items * c.kv_heads <= 64)
-        join(TileForm{}, Few{}, kTileRows / 4);
+        join(row_form, std::integral_constant<int, 16>{});
+      else if (j.groups == 4)
+        join(tile_form, std::integral_constant<int, 4>{});
       else
-        join(TileForm{}, One{}, 2);
+        join(tile_form, std::integral_constant<int, 1>{});
     };
     a.tree ? launch(std::true_type{}) : launch(std::false_type{});
   });

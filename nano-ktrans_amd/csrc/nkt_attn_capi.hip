@@ -47,8 +47,11 @@ AttnHandle* bound_handle(void* handle, char* err, size_t len) {
   return h;
 }
 
-// rows x heads of a launch, in 32 bits
-constexpr int64_t kMaxItems = (int64_t)1 << 30;
+// Rows x heads of a call, tokens of a sequence, and workgroups of a launch
+// (whose threads HIP counts in 32 bits).
+constexpr int64_t kMaxRows = (int64_t)1 << 27;
+constexpr int64_t kMaxTokens = (int64_t)1 << 30;
+constexpr int64_t kMaxGroups = ((int64_t)1 << 24) - 1;
 
 // the sizes of a forward call
 bool check_sizes(const AttnHandle* h, int num_tokens, int num_seqs, int max_queries, int max_seq_len, char* err,
@@ -57,12 +60,16 @@ bool check_sizes(const AttnHandle* h, int num_tokens, int num_seqs, int max_quer
     set_err(err, len, "num_tokens=%d, num_seqs=%d: negative", num_tokens, num_seqs);
     return false;
   }
-  if ((int64_t)num_tokens * h->heads > kMaxItems || (int64_t)num_seqs * h->heads > kMaxItems) {
-    set_err(err, len, "num_tokens=%d, num_seqs=%d: over 2^30 rows of %d heads", num_tokens, num_seqs, h->heads);
+  if ((int64_t)num_tokens * h->heads > kMaxRows || (int64_t)num_seqs * h->heads > kMaxRows) {
+    set_err(err, len, "num_tokens=%d, num_seqs=%d: over 2^27 rows of %d heads", num_tokens, num_seqs, h->heads);
     return false;
   }
-  if (max_queries < 0 || max_seq_len < 0 || max_seq_len > kMaxItems) {
+  if (max_queries < 0 || max_seq_len < 0 || max_seq_len > kMaxTokens) {
     set_err(err, len, "max_queries=%d, max_seq_len=%d: outside [0, 2^30]", max_queries, max_seq_len);
+    return false;
+  }
+  if (attn_workgroups(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len) > kMaxGroups) {
+    set_err(err, len, "num_seqs=%d of up to max_seq_len=%d tokens: over 2^24 workgroups", num_seqs, max_seq_len);
     return false;
   }
   return true;
@@ -73,8 +80,9 @@ int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_word
             int max_queries, int max_seq_len, float scale, void* out, void* workspace, size_t workspace_bytes,
             void* stream, char* err, size_t len) {
   AttnHandle* h = bound_handle(handle, err, len);
+  if (!query_starts) max_queries = 1;
   if (!h || !check_sizes(h, num_tokens, num_seqs, max_queries, max_seq_len, err, len)) return NKT_ATTN_ERR;
-  if (table_width < 0 || ((int64_t)table_width << h->cache.page_shift) > kMaxItems) {
+  if (table_width < 0 || ((int64_t)table_width << h->cache.page_shift) > kMaxTokens) {
     set_err(err, len, "table_width=%d: outside [0, 2^30 tokens]", table_width);
     return NKT_ATTN_ERR;
   }
@@ -85,6 +93,10 @@ int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_word
   if (num_tokens == 0 || num_seqs == 0) return NKT_ATTN_OK;
   if (!q || !out || !seq_lens || (!page_table && table_width > 0)) {
     set_err(err, len, "null q, out, seq_lens or page_table");
+    return NKT_ATTN_ERR;
+  }
+  if (!(scale > 0.f) || !(scale < 1e30f)) {
+    set_err(err, len, "scale=%g: a positive number wanted", (double)scale);
     return NKT_ATTN_ERR;
   }
   if (!aligned(q, 16) || !aligned(out, 16)) {
@@ -108,7 +120,7 @@ int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_word
   a.tokens = num_tokens;
   a.seqs = num_seqs;
   a.heads = h->heads;
-  a.max_queries = query_starts ? max_queries : 1;
+  a.max_queries = max_queries;
   a.max_len = max_seq_len;
   a.scale = scale;
   if (!check_hip(launch_attn(h->cache, a, workspace, (hipStream_t)stream), "attention kernel", err, len))
@@ -208,8 +220,8 @@ int nkt_attn_write(void* handle, const void* q, int64_t q_stride, const void* k,
                    void* stream, char* err, size_t err_len) {
   AttnHandle* h = bound_handle(handle, err, err_len);
   if (!h) return NKT_ATTN_ERR;
-  if (num_tokens < 0 || (int64_t)num_tokens * (h->heads + 2 * h->cache.kv_heads) > kMaxItems) {
-    set_err(err, err_len, "num_tokens=%d: negative, or over 2^30 rows of all heads", num_tokens);
+  if (num_tokens < 0 || (int64_t)num_tokens * (h->heads + 2 * h->cache.kv_heads) > kMaxRows) {
+    set_err(err, err_len, "num_tokens=%d: negative, or over 2^27 rows of all heads", num_tokens);
     return NKT_ATTN_ERR;
   }
   if (rope_rows < 1) {
@@ -252,8 +264,8 @@ int nkt_attn_read(void* handle, const int64_t* slots, int num_slots, void* k_out
                   size_t err_len) {
   AttnHandle* h = bound_handle(handle, err, err_len);
   if (!h) return NKT_ATTN_ERR;
-  if (num_slots < 0 || (int64_t)num_slots * h->cache.kv_heads > kMaxItems) {
-    set_err(err, err_len, "num_slots=%d: negative, or over 2^30 rows of all heads", num_slots);
+  if (num_slots < 0 || (int64_t)num_slots * h->cache.kv_heads > kMaxRows) {
+    set_err(err, err_len, "num_slots=%d: negative, or over 2^27 rows of all heads", num_slots);
     return NKT_ATTN_ERR;
   }
   if (num_slots == 0) return NKT_ATTN_OK;
@@ -273,11 +285,11 @@ int nkt_attn_keep(void* handle, const int32_t* page_table, int table_width, cons
                   size_t err_len) {
   AttnHandle* h = bound_handle(handle, err, err_len);
   if (!h) return NKT_ATTN_ERR;
-  if (num_seqs < 0 || (int64_t)num_seqs * h->cache.kv_heads > kMaxItems) {
-    set_err(err, err_len, "num_seqs=%d: negative, or over 2^30 rows of all heads", num_seqs);
+  if (num_seqs < 0 || (int64_t)num_seqs * h->cache.kv_heads > kMaxGroups) {
+    set_err(err, err_len, "num_seqs=%d: negative, or over 2^24 workgroups", num_seqs);
     return NKT_ATTN_ERR;
   }
-  if (table_width < 0 || kept_width < 0 || ((int64_t)table_width << h->cache.page_shift) > kMaxItems) {
+  if (table_width < 0 || kept_width < 0 || ((int64_t)table_width << h->cache.page_shift) > kMaxTokens) {
     set_err(err, err_len, "table_width=%d, kept_width=%d: negative, or over 2^30 tokens", table_width, kept_width);
     return NKT_ATTN_ERR;
   }
@@ -318,7 +330,7 @@ int nkt_attn_forward_tree(void* handle, const void* q, const int64_t* tree_mask,
                           const int32_t* query_starts, int num_tokens, int num_seqs, int max_queries, int max_seq_len,
                           float scale, void* out, void* workspace, size_t workspace_bytes, void* stream, char* err,
                           size_t err_len) {
-  if ((num_tokens > 0 && !tree_mask) || mask_words < 1 || (int64_t)num_tokens * mask_words > kMaxItems) {
+  if ((num_tokens > 0 && !tree_mask) || mask_words < 1 || (int64_t)num_tokens * mask_words > kMaxTokens) {
     set_err(err, err_len, "tree_mask of at least one word per row (and at most 2^30 in all) wanted, got %d", mask_words);
     return NKT_ATTN_ERR;
   }

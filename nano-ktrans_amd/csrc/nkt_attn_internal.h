@@ -61,6 +61,8 @@ struct AttnArgs {
   float scale;
 };
 
+// Workgroups of the call's largest launch.
+int64_t attn_workgroups(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len);
 size_t attn_workspace_bytes(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len);
 hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, hipStream_t stream);
 

@@ -96,7 +96,9 @@ class NativeAttention:
         self.num_pages = num_pages
         self.page_size = page_size
         self.cache_format = cache_format
-        self.scale = float(scale) if scale is not None else head_dim ** -0.5
+        self.scale = float(scale) if scale is not None else max(head_dim, 1) ** -0.5
+        if not 0.0 < self.scale < 1e30:
+            raise ValueError(f"scale must be a positive number, got {scale}")
         h = self.lib.nkt_attn_create(num_heads, num_kv_heads, head_dim, _FORMATS[cache_format], page_size, num_pages,
                                      self.err.buf, self.err.size)
         if not h:

@@ -127,8 +127,8 @@ FORWARD = [0x1000, 0x1000, 4, 0x1000, 0x1000, 4, 2, 3, 200, 1.0, 0x1000, None, 0
 @pytest.mark.parametrize("at,value,msg", [
     (0, None, b"null"), (1, None, b"null"), (3, None, b"null"), (10, None, b"null"), (0, 0x1008, b"aligned"),
     (10, 0x1004, b"aligned"), (2, -1, b"table_width"), (2, 1 << 25, b"table_width"), (4, None, b"query_starts"),
-    (5, -1, b"num_tokens"), (6, -1, b"num_seqs"), (5, 1 << 28, b"2^30"), (7, -1, b"max_queries"),
-    (8, -1, b"max_seq_len"),
+    (5, -1, b"num_tokens"), (6, -1, b"num_seqs"), (5, 1 << 28, b"2^27"), (7, -1, b"max_queries"),
+    (8, -1, b"max_seq_len"), (9, 0.0, b"scale"), (9, -1.0, b"scale"), (9, float("nan"), b"scale"), (9, float("inf"), b"scale"),
 ])
 def test_forward_rejects(bound, at, value, msg):
     L, eb = N.lib(), ctypes.create_string_buffer(256)
@@ -138,6 +138,15 @@ def test_forward_rejects(bound, at, value, msg):
     assert msg in eb.value
     assert L.nkt_attn_forward_tree(bound, args[0], 0x1000, 1, *args[1:], None, eb, 256) == -1
     assert msg in eb.value
+
+
+def test_forward_rejects_more_workgroups_than_a_launch_holds(bound):
+    """Many sequences of a long bound: 2^23 sequences x 2 heads x 512 chunks."""
+    L, eb, sz = N.lib(), ctypes.create_string_buffer(256), ctypes.c_size_t()
+    assert L.nkt_attn_workspace_bytes(bound, 1 << 23, 1 << 23, 1, 1 << 20, ctypes.byref(sz), eb, 256) == -1
+    assert b"workgroups" in eb.value
+    assert L.nkt_attn_workspace_bytes(bound, 64, 64, 1, 1 << 20, ctypes.byref(sz), eb, 256) == 0 and sz.value > 0
+    assert L.nkt_attn_workspace_bytes(bound, 0, 0, 0, 1 << 20, ctypes.byref(sz), eb, 256) == 0
 
 
 @pytest.mark.parametrize("mask,words", [(None, 1), (0x1000, 0), (0x1000, -1), (0x1000, 1 << 29)])

@@ -283,6 +283,40 @@ def test_past_32_bit_offsets(gpu_device):
             check_rows(got[rows], *reference(q[rows], ks[b], vs[b], causal(counts[b], lengths[b]), attn.scale))
 
 
+@pytest.mark.parametrize("scale", [0.02, 1.0])
+def test_other_scales(gpu_device, scale):
+    announce(f"scale {scale}")
+    p = make_problem([300, 77], heads=8, kv_heads=2, dim=64, fmt="bf16", page=64, seed=18, spread=0.3)
+    p.attn.scale = scale
+    q = randn(generator(18), 45, 8, 64)
+    for counts in ([1, 1], [40, 5]):
+        check_attention(p, counts, q[:sum(counts)], p.attn.forward(q[:sum(counts)], p.table, p.lens, starts_of(counts)))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_scores_far_below_zero(gpu_device, fmt):
+    """Every score of a row is far below zero: the maximum has to come down to it."""
+    announce(f"scores far below zero {fmt}")
+    lengths = [1000, 70]
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=128, fmt=fmt, page=64, seed=19)
+    g = generator(20)
+    base = 4 * randn(g, 1, 2, 128).float()
+    for b, n in enumerate(lengths):
+        at = torch.arange(n, device=DEV)
+        slots = p.attn.slots(p.table, torch.full_like(at, b), at)
+        put(p.attn, slots, base + 0.1 * randn(g, n, 2, 128).float(), randn(g, n, 2, 128).float())
+        p.k[b], p.v[b] = dense(p.attn, slots)
+    for counts in ([1, 1], [5, 40]):
+        q = (-4 * base.repeat_interleave(4, dim=1) / 4).expand(sum(counts), -1, -1).to(torch.bfloat16).contiguous()
+        got = p.attn.forward(q, p.table, p.lens, starts_of(counts))
+        at = split_rows(counts)
+        for b in range(2):
+            rows = slice(at[b], at[b + 1])
+            want, A = reference(q[rows], p.k[b], p.v[b], causal(counts[b], lengths[b]), p.attn.scale)
+            # scores of about -16 |base|^2 / sqrt(128) = -180: fp32 off by 2^-24 * 136 * 180 at most, 2^-9.4
+            assert bool(((got[rows].double() - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -7) * A).all())
+
+
 def test_rows_do_not_depend_on_the_batch(gpu_device):
     """The same sequence alone, among others and in other rows gives the same bits (fixed launch bounds)."""
     announce("batch independence")
@@ -368,6 +402,9 @@ def test_forward_refusals(gpu_device):
             attn.forward_tree(q, bad, table, lens)
     with pytest.raises(RuntimeError):
         attn.forward_tree(q, mask[:, :0], table, lens)
+    for scale in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            make_attention(8, 2, 128, "bf16", 64, 4, scale=scale)
     # rows one element off 16 bytes, and transposed ones, are copied
     p = make_problem([70, 3, 9], heads=8, kv_heads=2, dim=128, fmt="bf16", page=64, seed=30)
     want = p.attn.forward(q, p.table, p.lens)
