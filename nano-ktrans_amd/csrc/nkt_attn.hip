@@ -17,21 +17,31 @@ struct Seq {
   int context;  // position of its first token here (negative: more rows than tokens)
 };
 
-// (b is the same in all lanes; so is the result, held in scalar registers)
-__device__ __forceinline__ Seq sequence(const CacheView& c, const AttnArgs& a, int b, bool reports) {
+// What the sequence is made from, asked for together (b is the same in all
+// lanes): one round trip, and the caller's own loads may go beside it.
+struct SeqWords {
+  int start, next, len;
+};
+__device__ __forceinline__ SeqWords sequence_words(const AttnArgs& a, int b) {
+  const int32_t* at = a.starts ? a.starts + b : a.lens + b;
+  return {at[0], at[a.starts ? 1 : 0], a.lens[b]};
+}
+
+// (the result is held in scalar registers)
+__device__ __forceinline__ Seq sequence(const CacheView& c, const AttnArgs& a, int b, const SeqWords& w, bool reports) {
   Seq s;
   s.first = b;
   s.n = 1;
   bool bad = false;
   if (a.starts) {
-    const int s0 = __builtin_amdgcn_readfirstlane(a.starts[b]);
-    const int s1 = __builtin_amdgcn_readfirstlane(a.starts[b + 1]);
+    const int s0 = __builtin_amdgcn_readfirstlane(w.start);
+    const int s1 = __builtin_amdgcn_readfirstlane(w.next);
     s.first = s0 < 0 ? 0 : s0 > a.tokens ? a.tokens : s0;
     const int end = s1 > a.tokens ? a.tokens : s1;
     s.n = end > s.first ? end - s.first : 0;
     bad = s.n > a.max_queries;
   }
-  const int len = __builtin_amdgcn_readfirstlane(a.lens[b]);
+  const int len = __builtin_amdgcn_readfirstlane(w.len);
   s.context = (len < 0 ? 0 : len) - s.n;
   if (s.n > a.max_queries) s.n = a.max_queries;
   const int64_t table = (int64_t)a.width << c.page_shift;
@@ -39,6 +49,11 @@ __device__ __forceinline__ Seq sequence(const CacheView& c, const AttnArgs& a, i
   s.len = len < 0 ? 0 : len > most ? most : len;
   if (reports && (bad || len < 0 || len > most)) report(c.status, kBadLength);
   return s;
+}
+
+// 64 entries of sequence b's page table from entry i on, one per lane
+__device__ __forceinline__ int table_entries(const AttnArgs& a, int b, int i, int lane) {
+  return i + lane < a.width ? a.table[(int64_t)b * a.width + i + lane] : -1;
 }
 
 // Positions p0 .. p0 + 63 that a token of the sequence sees, as bits.
@@ -118,20 +133,22 @@ constexpr int kRowRows = 16;                    // of the row form
 // sum in the workspace, and join_kernel adds them in order.
 struct Parts {
   int items, splits, chunk;
+  int rows;   // of an item
   float* o;   // [items, kv_heads, splits, rows, D]
   float* ml;  // [items, kv_heads, splits, rows, 2]
-  __device__ __forceinline__ int64_t row(int item, int h, int kv_heads, int split, int rows, int r) const {
+  __device__ __forceinline__ int64_t row(int item, int h, int kv_heads, int split, int r) const {
     return (((int64_t)item * kv_heads + h) * splits + split) * rows + r;
   }
 };
 
 __device__ __forceinline__ int first_row(const AttnArgs& a, int b) { return a.starts ? a.starts[b] : b; }
 
-// The sequence of a tile of kTileRows rows, and the tile's number in it (which
-// may lie past its rows).  Sequence b's tiles start at starts[b] G / 128 + b,
-// which ascends and leaves room for its ceil(n G / 128) tiles: the last b that
-// starts at or before this tile, found by 64 lanes at a time.
-__device__ __forceinline__ bool sequence_of_tile(const AttnArgs& a, int G, int tile, int lane, int* seq, int* block) {
+// The sequence of a tile of kTileRows rows.  Sequence b's tiles start at
+// starts[b] G / 128 + b, which ascends and leaves room for its ceil(n G / 128)
+// tiles: the last b that starts at or before this tile, found by 64 lanes at a
+// time.  block_of_tile: the tile's number in its sequence (which may lie past
+// its rows, or before them where starts does not ascend from 0).
+__device__ __forceinline__ int sequence_of_tile(const AttnArgs& a, int G, int tile, int lane) {
   int b = 0;
   for (int n = a.seqs; n > 1;) {
     const int step = (n + 63) / 64;
@@ -139,15 +156,15 @@ __device__ __forceinline__ bool sequence_of_tile(const AttnArgs& a, int G, int t
     const bool before =
         lane * step < n && (int64_t)first_row(a, i < a.seqs ? i : a.seqs - 1) * G / kTileRows + i <= tile;
     const int count = __popcll(__ballot(before));
-    if (count == 0) return false;
-    const int skip = (count - 1) * step;
+    const int skip = count > 0 ? (count - 1) * step : 0;
     b += skip;
     n = n - skip < step ? n - skip : step;
   }
-  *seq = __builtin_amdgcn_readfirstlane(b);
-  const int first = __builtin_amdgcn_readfirstlane(first_row(a, *seq));
-  *block = tile - ((int)((int64_t)first * G / kTileRows) + *seq);
-  return *block >= 0;
+  return __builtin_amdgcn_readfirstlane(b);
+}
+__device__ __forceinline__ int block_of_tile(const AttnArgs& a, int G, int tile, int b, const SeqWords& w) {
+  const int first = a.starts ? __builtin_amdgcn_readfirstlane(w.start) : b;
+  return tile - ((int)((int64_t)first * G / kTileRows) + b);
 }
 
 // One past the last position that some row of rows r0 .. r0 + count - 1 sees.
@@ -215,12 +232,17 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const int rest = (int)(blockIdx.x / (unsigned)HK);
   const int split = rest % part.splits;
   const int tile = part.items - 1 - rest / part.splits;
-  int b, block;
-  if (!sequence_of_tile(a, G, tile, lane, &b, &block)) return;
-  const Seq s = sequence(c, a, b, h == 0 && block == 0 && split == 0 && tid == 0);
+  const int begin = split * part.chunk;
+  const int b = sequence_of_tile(a, G, tile, lane);
+  const SeqWords words = sequence_words(a, b);
+  // 64 entries of the page table from pages_at on
+  int pages_at = begin >> c.page_shift;
+  int pages = table_entries(a, b, pages_at, lane);
+  const int block = block_of_tile(a, G, tile, b, words);
+  const Seq s = sequence(c, a, b, words, h == 0 && block == 0 && split == 0 && tid == 0);
   const int rows = s.n * G;
   const int r0 = block * kTileRows;
-  if (r0 >= rows) return;
+  if (block < 0 || r0 >= rows) return;
   // This lane's row; rows past the end repeat the last one and are not stored.
   // (Worked out again where it is needed, rather than held in registers that
   // the loop has no room for.)
@@ -244,7 +266,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 
   // the positions that the workgroup takes: its part of those that its rows see
   const int row_end = end_of_rows<TREE>(s, G, r0, kTileRows);
-  const int begin = split * part.chunk;
   if (split > 0 && begin >= row_end) return;
   const int end = row_end - begin > part.chunk ? begin + part.chunk : row_end;
   // positions below are seen by all rows
@@ -262,15 +283,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
 
-  // 64 entries of the page table, one per lane
-  int pages = -1, pages_at = -1;
   // the first tile at or after p whose page is in the cache (or some p >= end); its (page, head) block
   auto find = [&](int p, int64_t* at) __attribute__((always_inline)) {
     for (; p < end; p += kTileKeys) {
       const int i = p >> c.page_shift;
-      if (pages_at < 0 || i - pages_at >= 64) {
+      if (i - pages_at >= 64) {
         pages_at = i;
-        pages = i + lane < a.width ? a.table[(int64_t)b * a.width + i + lane] : -1;
+        pages = table_entries(a, b, i, lane);
       }
       const int page = __builtin_amdgcn_readlane(pages, i - pages_at);
       if (page >= 0 && page < c.num_pages) {
@@ -284,9 +303,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   // Staging.  bf16: straight into LDS.  int8: into registers (load_*), from
   // there converted into LDS (land_*): values in the first half of a tile's
   // step and keys in the second, so that they share the registers.
-  u32x4 raw[I8 ? kLoads / 2 : 1];
-  float raw_scale = 0.f;
-  auto load_k = [&](int64_t at, int buf) __attribute__((always_inline)) {
+  struct Raw {
+    u32x4 w[I8 ? kLoads / 2 : 1];
+    float scale;
+  };
+  auto load_k = [&](int64_t at, int buf, Raw& raw) __attribute__((always_inline)) {
     if (!I8) {
       const uint8_t* kb = c.k + at * (D * 2);
 #pragma unroll
@@ -299,11 +320,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     } else {
       const uint8_t* kb = c.k + at * D;
 #pragma unroll
-      for (int j = 0; j < kLoads / 2; ++j) raw[j] = *(const u32x4*)(kb + (j * 256 + tid) * 16);
-      if (tid < kTileKeys) raw_scale = c.k_scales[at + tid];
+      for (int j = 0; j < kLoads / 2; ++j) raw.w[j] = *(const u32x4*)(kb + (j * 256 + tid) * 16);
+      if (tid < kTileKeys) raw.scale = c.k_scales[at + tid];
     }
   };
-  auto load_v = [&](int64_t at, int buf) __attribute__((always_inline)) {
+  auto load_v = [&](int64_t at, int buf, Raw& raw) __attribute__((always_inline)) {
     if (!I8) {
       const uint8_t* vb = c.v + at * (D * 2);
 #pragma unroll
@@ -312,8 +333,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     } else {
       const uint8_t* vb = c.v + at * D;
 #pragma unroll
-      for (int j = 0; j < kLoads / 2; ++j) raw[j] = *(const u32x4*)(vb + (j * 256 + tid) * 16);
-      if (tid < kTileKeys) raw_scale = c.v_scales[at + tid];
+      for (int j = 0; j < kLoads / 2; ++j) raw.w[j] = *(const u32x4*)(vb + (j * 256 + tid) * 16);
+      if (tid < kTileKeys) raw.scale = c.v_scales[at + tid];
     }
   };
   auto widen = [&](u32x4 w, u32x4* x) {
@@ -325,32 +346,32 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       x[j >> 1][2 * (j & 1) + 1] = hi;
     }
   };
-  auto land_k = [&](int buf, int n) __attribute__((always_inline)) {
+  auto land_k = [&](int buf, int n, Raw& raw) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kLoads / 2; ++j) {
       const int piece = j * 256 + tid;
       u32x4 x[2];
-      __asm__ volatile("" : "+v"(raw[j]));  // (widened here, not where it is loaded)
-      widen(raw[j], x);
+      __asm__ volatile("" : "+v"(raw.w[j]));  // (widened here, not where it is loaded)
+      widen(raw.w[j], x);
       const int t = piece / (D / 16), ch = piece % (D / 16) * 2;
       const int r = (t & ~12) | (t & 4) << 1 | (t & 8) >> 1;
       *(u32x4*)(lds.k[buf] + (r * kChunks + (ch ^ chunk_key<D>(r))) * 16) = x[0];
       *(u32x4*)(lds.k[buf] + (r * kChunks + ((ch + 1) ^ chunk_key<D>(r))) * 16) = x[1];
     }
-    if (tid < kTileKeys) lds.ks[n & 3][tid] = raw_scale * scale2;
+    if (tid < kTileKeys) lds.ks[n & 3][tid] = raw.scale * scale2;
   };
-  auto land_v = [&](int buf) __attribute__((always_inline)) {
+  auto land_v = [&](int buf, Raw& raw) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kLoads / 2; ++j) {
       const int piece = j * 256 + tid;
       u32x4 x[2];
-      __asm__ volatile("" : "+v"(raw[j]));
-      widen(raw[j], x);
+      __asm__ volatile("" : "+v"(raw.w[j]));
+      widen(raw.w[j], x);
       const int g16 = piece / D, d = piece % D;
       *(u32x4*)(lds.v[buf] + ((2 * g16) * D + d) * 16) = x[0];
       *(u32x4*)(lds.v[buf] + ((2 * g16 + 1) * D + d) * 16) = x[1];
     }
-    if (tid < kTileKeys) lds.vs[buf][tid] = raw_scale;
+    if (tid < kTileKeys) lds.vs[buf][tid] = raw.scale;
   };
 
   // Fragments of half tile sub (register r of its scores: token sub 32 + (r >>
@@ -514,28 +535,38 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   int p1 = find(p + kTileKeys, &at1);
   int n = 0;  // the tile's number; its buffers are n & 1
   float top = kLowest;
+  Raw raw = {};
   if (p < end) {
-    load_k(at, 0);
-    if (I8) land_k(0, 0);
-    wait_vmem();
+    // the first keys, values and second keys, all asked for at once
+    Raw raw_v = {}, raw_k1 = {};
+    load_k(at, 0, raw);
+    load_v(at, 0, raw_v);
+    if (p1 < end) load_k(at1, 1, raw_k1);
+    if (I8) {
+      land_k(0, 0, raw);
+    } else if (p1 < end) {
+      wait_vmem_but<2 * kLoads>();
+    } else {
+      wait_vmem_but<kLoads>();
+    }
     lds_barrier();
-    load_v(at, 0);
-    if (I8) land_v(0);
-    if (p1 < end) load_k(at1, 1);
     read_k(0, 0);
     scores(0, kQ);
     less_maximum(0, 0);
     mask_scores(0, p);
     top = maximum();
     read_k(0, 1);
-    if (I8) land_k(1, 1);
+    if (I8) {
+      land_v(0, raw_v);
+      land_k(1, 1, raw_k1);
+    }
   }
   auto tile_step = [&](auto buffer) __attribute__((always_inline)) {
     constexpr int buf = decltype(buffer)::value;
     wait_vmem();
     lds_barrier();
     const int p2 = find(p1 + kTileKeys, &at2);
-    if (p1 < end) load_v(at1, buf ^ 1);
+    if (p1 < end) load_v(at1, buf ^ 1, raw);
     if (p + kTileKeys > open) clean(buf, p);
     // Each group of LDS reads is issued behind the first product that waits for
     // the group before it (the wait is for all that are under way), and the
@@ -569,11 +600,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       top = maximum();
       if (mask_scores(sub ^ 1, sub ? p1 : p)) top = maximum();
       if (sub == 0) {
-        if (I8) land_v(buf ^ 1);
-        if (p2 < end) load_k(at2, buf);
+        if (I8) land_v(buf ^ 1, raw);
+        if (p2 < end) load_k(at2, buf, raw);
       }
     }
-    if (I8) land_k(buf, n + 2);
+    if (I8) land_k(buf, n + 2, raw);
     ++n;
     p = p1;
     p1 = p2;
@@ -588,7 +619,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const int out_row = my_row();
   if (out_row >= rows) return;
   if (row_end > part.chunk) {  // the join adds the parts
-    const int64_t to = part.row(tile, h, HK, split, kTileRows, out_row - r0);
+    const int64_t to = part.row(tile, h, HK, split, out_row - r0);
 #pragma unroll
     for (int i = 0; i < kO; ++i)
 #pragma unroll
@@ -645,8 +676,8 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   // 64 entries of the page table, one per lane: all that a chunk needs (asked
   // for before anything is known of the sequence)
   const int page0 = begin >> c.page_shift;
-  const int pages = page0 + lane < a.width ? a.table[(int64_t)b * a.width + page0 + lane] : -1;
-  const Seq s = sequence(c, a, b, h == 0 && split == 0 && tid == 0);
+  const int pages = table_entries(a, b, page0, lane);
+  const Seq s = sequence(c, a, b, sequence_words(a, b), h == 0 && split == 0 && tid == 0);
   const int rows = s.n * G;
   if (rows == 0) return;
   const int row_end = end_of_rows<TREE>(s, G, 0, kRowRows);
@@ -885,7 +916,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     for (int d = 0; d < D / 16; ++d) out[d] += s_o[w][r][d0 + d] * f;
   }
   if (row_end > part.chunk) {
-    const int64_t at = part.row(b, h, HK, split, kRowRows, r);
+    const int64_t at = part.row(b, h, HK, split, r);
 #pragma unroll
     for (int d = 0; d < D / 16; d += 4)
       *(f32x4*)(part.o + at * D + d0 + d) = f32x4{out[d], out[d + 1], out[d + 2], out[d + 3]};
@@ -916,11 +947,12 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
   const int h = (int)(blockIdx.x % (unsigned)HK);
   const int rest = (int)(blockIdx.x / (unsigned)HK);
   const int item = rest / row_blocks;
-  int b = item, block = 0;
-  if (ROWS != kRowRows && !sequence_of_tile(a, G, item, lane, &b, &block)) return;
-  const Seq s = sequence(c, a, b, false);
+  const int b = ROWS == kRowRows ? item : sequence_of_tile(a, G, item, lane);
+  const SeqWords words = sequence_words(a, b);
+  const int block = ROWS == kRowRows ? 0 : block_of_tile(a, G, item, b, words);
+  const Seq s = sequence(c, a, b, words, false);
   const int rows = s.n * G, r0 = block * ROWS;
-  if (r0 >= rows) return;
+  if (block < 0 || r0 >= rows) return;
   const int row_end = end_of_rows<TREE>(s, G, r0, ROWS);
   if (row_end <= part.chunk) return;
   const int splits = (row_end + part.chunk - 1) / part.chunk;
@@ -933,7 +965,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
 #pragma unroll
     for (int d = 0; d < kN; ++d) out[d] = 0.f;
     for (int i = sp; i < splits && r < used; i += SP) {
-      const int64_t at = part.row(item, h, HK, i, ROWS, r);
+      const int64_t at = part.row(item, h, HK, i, r);
       const float mi = part.ml[2 * at], li = part.ml[2 * at + 1];
       const float to = fmaxf(m, mi);
       const float f = __builtin_amdgcn_exp2f(m - to), fi = __builtin_amdgcn_exp2f(mi - to);
@@ -987,7 +1019,6 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
 // device (its rows and bounds).
 struct Plan {
   bool row_form;
-  int rows;  // of an item
   Parts part;
 };
 
@@ -995,7 +1026,7 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
   Plan p = {};
   const int64_t G = heads / c.kv_heads;
   p.row_form = max_queries * G <= kRowRows;
-  p.rows = p.row_form ? kRowRows : kTileRows;
+  p.part.rows = p.row_form ? (int)(max_queries > 0 ? max_queries * G : G) : kTileRows;
   p.part.items = (int)(p.row_form ? seqs : tokens * G / kTileRows + seqs);
   if (p.part.items < 1) p.part.items = 1;
   const int64_t wgs = (int64_t)p.part.items * c.kv_heads;
@@ -1006,9 +1037,11 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
     // against 13.6, 2000 9.2 against 22), but under 640 tokens a second launch
     // costs what the split gains (517 tokens: 8.3 for both launches, 9.0 for
     // one).  More only split what would run on after the others: chunks of
-    // 2048 against 4096 tokens, 32 x 4000 tokens 52 against 60.
+    // 2048 against 4096 tokens, 32 x 4000 tokens 52 against 60; over two
+    // rounds of workgroups chunks of 4096, the most that a wave holds page
+    // numbers for.
     if (wgs < 100 && max_len > 640) splits = (256 + wgs - 1) / wgs;
-    most = 2048;
+    most = wgs <= 1024 ? 2048 : 4096;
   } else if (wgs < 512) {
     // About one and a half rounds of workgroups (two run on a CU at a time);
     // in us, for 512, 768 and 1536 of them: 1000 tokens bf16 33, 31, 42; four
@@ -1033,7 +1066,7 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
 }
 
 size_t plan_rows(const CacheView& c, const Plan& p) {
-  return p.part.splits > 1 ? (size_t)p.part.items * c.kv_heads * p.part.splits * p.rows : 0;
+  return p.part.splits > 1 ? (size_t)p.part.items * c.kv_heads * p.part.splits * p.part.rows : 0;
 }
 
 // Workgroups per item and head of the join, and its thread groups per row:
@@ -1043,10 +1076,9 @@ struct JoinPlan {
   int groups;
   int64_t row_blocks;
 };
-JoinPlan join_of(const CacheView& c, int heads, const Plan& p, int max_queries) {
-  const int64_t rows = (int64_t)max_queries * (heads / c.kv_heads);  // of the row form
-  if (p.row_form && p.part.splits <= 8) return {4, (rows + 3) / 4};
-  if (p.row_form) return {16, rows};
+JoinPlan join_of(const CacheView& c, const Plan& p) {
+  if (p.row_form && p.part.splits <= 8) return {4, (p.part.rows + 3) / 4};
+  if (p.row_form) return {16, p.part.rows};
   if ((int64_t)p.part.items * c.kv_heads <= 64) return {4, kTileRows / 4};
   return {1, 2};
 }
@@ -1056,7 +1088,7 @@ JoinPlan join_of(const CacheView& c, int heads, const Plan& p, int max_queries) 
 int64_t attn_workgroups(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len) {
   const Plan p = plan_of(c, heads, tokens, seqs, max_queries, max_len);
   const int64_t items = (int64_t)p.part.items * c.kv_heads;
-  const int64_t join = p.part.splits > 1 ? join_of(c, heads, p, max_queries).row_blocks : 0;
+  const int64_t join = p.part.splits > 1 ? join_of(c, p).row_blocks : 0;
   return items * (p.part.splits > join ? p.part.splits : join);
 }
 
@@ -1079,7 +1111,7 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
       else
         hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
       if (p.part.splits == 1) return;
-      const JoinPlan j = join_of(c, a.heads, p, a.max_queries);
+      const JoinPlan j = join_of(c, p);
       const dim3 join_grid((unsigned)(p.part.items * c.kv_heads * j.row_blocks));
       auto join = [&](auto rows, auto groups) {
         constexpr int ROWS = decltype(rows)::value, SP = decltype(groups)::value;
