@@ -85,7 +85,7 @@ int nkt_attn_bind_cache(void* handle, void* const* ptrs, char* err, size_t err_l
  *   (y1, y2) -> (y1 cos - y2 sin, y2 cos + y1 sin) on the two halves of a head,
  *   cos | sin = row positions[t] of rope fp32 [rope_rows, D];
  * in fp32 with one rounding, to bf16 for q_out [T, num_heads, D] (which may be
- * q itself) and to the cache's format for the keys; values are stored as they
+ * q itself if its tokens are dense) and to the cache's format for the keys; values are stored as they
  * are.  slots int64 [T]: where each token's key and value go; a negative slot
  * stores nothing (padding).  The slots of one call are distinct: what a slot
  * given twice holds is undefined. */
@@ -119,9 +119,9 @@ int nkt_attn_workspace_bytes(void* handle, int num_tokens, int num_seqs, int max
 
 /* Causal attention over the cache (scale > 0): out[i] = sum_j softmax_j(scale q_i . k_j) v_j
  * over the positions j <= seq_len - n + i of the sequence's i-th row (i < n).
- * q and out bf16 [num_tokens, num_heads, D], contiguous, 16-byte aligned.  A row
- * that sees nothing is zero; rows behind the last sequence are left as they
- * were.  A token that a row does not see does not reach it, whatever the cache
+ * q and out (which may be q itself) bf16 [num_tokens, num_heads, D], contiguous,
+ * 16-byte aligned.  A row that sees nothing, or whose scores are all -infinity,
+ * is zero; rows behind the last sequence are left as they were.  A token that a row does not see does not reach it, whatever the cache
  * holds there. */
 int nkt_attn_forward(void* handle, const void* q, const int32_t* page_table, int table_width, const int32_t* seq_lens,
                      const int32_t* query_starts, int num_tokens, int num_seqs, int max_queries, int max_seq_len,

@@ -38,11 +38,14 @@ __device__ __forceinline__ float scale_from_max(uint32_t max_bits) {
   return max_bits >= 0x7f800000u ? __builtin_nanf("") : s == 0.0f ? 1.0f : s;
 }
 // round-half-even(x / scale): the quotient by the scale's reciprocal and one
-// correction step, |x| <= 127 scale
+// correction step, |x| <= 127 scale.  Both are taken 2^64 times as large for a
+// scale whose reciprocal could pass fp32's range.
 struct Quantizer {
-  float scale, inverse;
-  __device__ __forceinline__ explicit Quantizer(float s) : scale(s), inverse(1.0f / s) {}
+  float up, scale, inverse;
+  __device__ __forceinline__ explicit Quantizer(float s)
+      : up(s < 0x1p-64f ? 0x1p64f : 1.0f), scale(s * up), inverse(1.0f / scale) {}
   __device__ __forceinline__ uint32_t code(float x) const {
+    x *= up;
     const float q = x * inverse;
     const float r = __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q, scale, x), inverse, q));
     return (uint32_t)(int)fminf(fmaxf(r, -127.0f), 127.0f) & 0xffu;

@@ -2,8 +2,9 @@
 the C ABI (include/nkt_attn.h).
 
 ``NativeAttention`` owns the cache (torch tensors in HBM) and enqueues on
-torch's current HIP stream.  No call synchronises the host.  Activations are
-bf16; the cache holds bf16 or int8 with one fp32 scale per token and head.
+torch's current HIP stream.  No call synchronises the host (``status`` and
+``check_status`` do).  Activations are bf16; the cache holds bf16 or int8 with one
+fp32 scale per token and head.  For inference: no call gives gradients.
 
 A serving program keeps, per batch, a page table [sequences, pages], the
 sequences' lengths, and where its new tokens go:
@@ -203,10 +204,18 @@ class NativeAttention:
 
     # ------------------------------------------------------------------ cache
     def slots(self, page_table: torch.Tensor, seqs: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-        """int64 slots of the tokens at ``positions`` of the sequences ``seqs`` (rows of the page table)."""
-        positions = positions.long()
-        pages = page_table[seqs.long(), torch.div(positions, self.page_size, rounding_mode="floor")].long()
-        return pages * self.page_size + positions % self.page_size
+        """int64 slots of the tokens at ``positions`` of the sequences ``seqs`` (rows of the page table): -1 for
+        a negative position (padding), a slot past the cache, which ``write`` reports, for one past the table."""
+        B, W = page_table.shape
+        seqs, positions = seqs.long(), positions.long()
+        past = self.num_pages * self.page_size
+        if B == 0 or W == 0:
+            return torch.where(positions < 0, -1, past)
+        at = torch.div(positions, self.page_size, rounding_mode="floor")
+        inside = (at < W) & (seqs >= 0) & (seqs < B)
+        pages = page_table[seqs.clamp(0, B - 1), at.clamp(0, W - 1)].long()
+        slots = torch.where(inside, pages * self.page_size + positions % self.page_size, past)
+        return slots.masked_fill(positions < 0, -1)
 
     def write(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
               rope: torch.Tensor, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
@@ -313,7 +322,8 @@ class NativeAttention:
         sequences; query_starts [sequences + 1] their rows of q (None: one row each, a decode step).
         max_queries and max_seq_len bound the rows of one sequence and the lengths: known to the caller
         without asking the device, they choose the launch (default: all of q, the whole page table).  A
-        row that sees nothing is zero; rows behind the last sequence are left as ``out`` had them."""
+        row that sees nothing is zero; rows behind the last sequence are left as ``out`` (which may be q
+        itself) had them."""
         return self._attend("nkt_attn_forward", q, (), page_table, seq_lens, query_starts, max_queries, max_seq_len,
                             out)
 

@@ -127,6 +127,22 @@ def test_write_special_rows(gpu_device, fmt):
             assert bool(torch.isnan(got[3]).all()) and bool(torch.isnan(got[4]).all())
 
 
+@pytest.mark.parametrize("largest", [127 * 2.0 ** -133, 2.0 ** -126, 1.2e-38, 3e-37, 1e-20])
+def test_write_tiny_rows_to_int8(gpu_device, largest):
+    """Rows whose scale, or its reciprocal, is outside fp32's normal range.  The scale is max / 127 to fp32's
+    denormal step, 2^-149, so codes up to 127 are off by that many of them beside the half step."""
+    announce(f"write tiny rows {largest}")
+    attn = make_attention(2, 1, 64, "int8", 64, 1)
+    rows = (torch.linspace(-1, 1, 64, dtype=torch.float64) * largest).to(torch.bfloat16).view(1, 1, 64).to(DEV)
+    slots = torch.arange(1, device=DEV)
+    attn.write(torch.zeros(1, 2, 64, dtype=torch.bfloat16, device=DEV), rows, rows, torch.zeros_like(slots), slots,
+               rope_table(1, 64, 1e4, DEV))
+    want = rows[0].double()
+    for got in dense(attn, slots):
+        step = want.abs().amax() / 127
+        assert bool(((got[0] - want).abs() <= step * (0.5 + 2.0 ** -15) + 2.0 ** -142).all())
+
+
 def test_write_reports_bad_slots_and_positions(gpu_device):
     announce("write: bad slots and positions")
     attn = make_attention(4, 2, 128, "int8", 64, 3)
@@ -174,6 +190,18 @@ def test_read(gpu_device, heads, kv_heads, dim, page, fmt, n, run):
     bad = slots.clone()
     bad[0] = 12 * page
     assert bool((attn.read(bad)[0][0] == 0).all()) and attn.status()["bad_slot"]
+
+
+def test_slots(gpu_device):
+    """Padding positions, and positions and sequences that the page table does not have."""
+    attn = make_attention(2, 1, 64, "bf16", 64, 9)
+    table = torch.tensor([[7, 2], [0, -1]], dtype=torch.int32, device=DEV)
+    seqs = torch.tensor([0, 0, 1, 1, 0, 1, 2, -1], device=DEV)
+    positions = torch.tensor([3, 64, 63, 70, 128, -1, 0, 0], dtype=torch.int32, device=DEV)
+    past = 9 * 64
+    want = [7 * 64 + 3, 2 * 64, 63, -64 + 6, past, -1, past, past]
+    assert attn.slots(table, seqs, positions).tolist() == want
+    assert attn.slots(table[:, :0], seqs, positions).tolist() == [past] * 5 + [-1, past, past]
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "int8"])
