@@ -11,7 +11,8 @@ nano_ktrans/models/mixtral.py:191-205 runs, before the MoE half:
 ``NativeAttention``: the projections are the caller's nn.Linear modules; head
 norms (architectures with ``use_qk_norm``), rotation and the cache write are
 one launch on the projection's output, attention one or two.
-``FusedDecoderLayer`` follows it with the MoE half (``FusedMoEBlock``).
+``FusedDecoderLayer`` follows it with the MoE half (``FusedMoEBlock``).  Both are
+for inference: their outputs carry no gradient.
 """
 from __future__ import annotations
 
@@ -65,6 +66,7 @@ class FusedAttentionBlock(nn.Module):
         self.q_norm = q_norm
         self.k_norm = k_norm
 
+    @torch.no_grad()
     def forward(self, hidden_states: torch.Tensor, batch: AttentionBatch) -> torch.Tensor:
         if hidden_states.dtype != torch.bfloat16:
             raise ValueError("FusedAttentionBlock needs bf16 hidden states")
@@ -78,10 +80,11 @@ class FusedAttentionBlock(nn.Module):
         q = a.write(q, k, v, batch.positions, batch.slots, self.rope, **norms)
         where = (batch.page_table, batch.seq_lens, batch.query_starts)
         bounds = {"max_queries": batch.max_queries, "max_seq_len": batch.max_seq_len}
+        # in place of the queries: rows behind the last sequence (padding) stay numbers
         if batch.tree_mask is None:
-            out = a.forward(q, *where, **bounds)
+            out = a.forward(q, *where, **bounds, out=q)
         else:
-            out = a.forward_tree(q, batch.tree_mask, *where, **bounds)
+            out = a.forward_tree(q, batch.tree_mask, *where, **bounds, out=q)
         return hidden_states + self.o_proj(out.flatten(1)).view(hidden_states.shape)
 
 

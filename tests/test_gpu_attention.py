@@ -219,6 +219,28 @@ def test_rows_behind_the_last_sequence_stay(gpu_device):
         assert bool((out[sum(counts):] == 7.0).all())
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("counts,lengths", [(None, [700, 0, 3000]), ([4, 1], [2500, 9]), ([130, 0, 45], [900, 4, 2000])])
+def test_in_place_of_the_queries(gpu_device, fmt, counts, lengths):
+    """out = q: the same bits, with and without splits, rows behind the last sequence as they were."""
+    announce(f"in place {fmt} rows {counts} of {lengths}")
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=64, fmt=fmt, page=64, seed=8)
+    behind = 0 if counts is None else 5
+    q = randn(generator(9), sum(counts or [1] * len(lengths)) + behind, 8, 64)
+    starts = None if counts is None else torch.tensor(split_rows(counts), dtype=torch.int32, device=DEV)
+    most = None if counts is None else max(counts)
+    want = p.attn.forward(q, p.table, p.lens, starts, max_queries=most, out=q.clone())
+    got = q.clone()
+    p.attn.forward(got, p.table, p.lens, starts, max_queries=most, out=got)
+    assert torch.equal(got, want)
+    if counts is not None:
+        assert torch.equal(got[sum(counts):], q[sum(counts):]) and not torch.equal(got, q)
+        mask = torch.full((q.shape[0], 3), -1, dtype=torch.int64, device=DEV)
+        want = p.attn.forward_tree(q, mask, p.table, p.lens, starts, max_queries=most, out=q.clone())
+        p.attn.forward_tree(q, mask, p.table, p.lens, starts, max_queries=most, out=q)
+        assert torch.equal(q, want)
+
+
 @pytest.mark.parametrize("counts", [None, [9, 40]])
 def test_bad_pages_and_lengths_are_reported(gpu_device, counts):
     """Pages outside the cache are not seen; lengths past the table are cut, negative ones nothing; rows past
