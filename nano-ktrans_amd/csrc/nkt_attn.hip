@@ -125,6 +125,7 @@ __device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t* lo, uint32_t
 }
 
 constexpr int kTileRows = 128, kTileKeys = 64;  // of the tile form
+constexpr int kPairRows = 64;                   // of the same where a sequence has no more
 constexpr int kRowRows = 16;                    // of the row form
 
 // How a launch is cut: items (a tile of rows of one head) x splits (of chunk
@@ -134,6 +135,7 @@ constexpr int kRowRows = 16;                    // of the row form
 struct Parts {
   int items, splits, chunk;
   int rows;   // of an item
+  bool whole;  // an item is a sequence with all its rows
   float* o;   // [items, kv_heads, splits, rows, D]
   float* ml;  // [items, kv_heads, splits, rows, 2]
   __device__ __forceinline__ int64_t row(int item, int h, int kv_heads, int split, int r) const {
@@ -224,7 +226,12 @@ __device__ __forceinline__ int chunk_key(int r) {
   return D == 128 ? r & 15 : r >> 1 & 7;
 }
 
-template <int D, bool I8, bool TREE>
+// ROWS = 64 (no sequence has more): one pair of waves takes the rows against the
+// first half of every tile's tokens, the other against the second, and their
+// results are added at the end: half the products and exponentials that 128
+// half-empty rows would cost.  64 drafts of up to 8 tokens on up to 8192, 32 / 4
+// heads, int8 116 us, as 128 rows 151; bf16 137 and 153.
+template <int D, bool I8, bool TREE, int ROWS>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int kQ = D / 16;       // Q fragments, and key products per half tile
   constexpr int kO = D / 32;       // output tiles
@@ -232,6 +239,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   constexpr int kLoads = kTileKeys * D * 2 / 4096;  // 16-byte loads per thread, keys or values
   // value fragments read ahead, in 16 tokens (int8's staging needs the registers)
   constexpr int kVAhead = I8 && D == 128 ? 1 : 2;
+  constexpr bool kPairs = ROWS == kPairRows;
   __shared__ TileLds<D, I8> lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int half = lane >> 5, col = lane & 31;
@@ -244,23 +252,24 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const int split = rest % part.splits;
   const int tile = part.items - 1 - rest / part.splits;
   const int begin = split * part.chunk;
-  const int b = sequence_of_tile(a, G, tile, lane);
+  const int b = kPairs || part.whole ? tile : sequence_of_tile(a, G, tile, lane);
   const SeqWords words = sequence_words(a, b);
   // 64 entries of the page table from pages_at on
   int pages_at = begin >> c.page_shift;
   int pages = table_entries(a, b, pages_at, lane);
-  const int block = block_of_tile(a, G, tile, b, words);
+  const int block = kPairs || part.whole ? 0 : block_of_tile(a, G, tile, b, words);
   const Seq s = sequence(c, a, b, words, h == 0 && block == 0 && split == 0 && tid == 0);
   const int rows = s.n * G;
-  const int r0 = block * kTileRows;
+  const int r0 = block * ROWS;
   if (block < 0 || r0 >= rows) return;
+  const int mine = kPairs ? __builtin_amdgcn_readfirstlane(wave) >> 1 : 0;  // the wave's half of a tile
   // This lane's row; rows past the end repeat the last one and are not stored.
   // (Worked out again where it is needed, rather than held in registers that
   // the loop has no room for.)
   auto my_row = [&] {
     int lane_col = col;
     __asm__ volatile("" : "+v"(lane_col));
-    return r0 + wave * 32 + lane_col;
+    return r0 + (kPairs ? wave & 1 : wave) * 32 + lane_col;
   };
   auto my_token = [&] {
     const int row = my_row();
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   }
 
   // the positions that the workgroup takes: its part of those that its rows see
-  const int row_end = end_of_rows<TREE>(s, G, r0, kTileRows);
+  const int row_end = end_of_rows<TREE>(s, G, r0, ROWS);
   if (split > 0 && begin >= row_end) return;
   const int end = row_end - begin > part.chunk ? begin + part.chunk : row_end;
   // positions below are seen by all rows
@@ -514,7 +523,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     if (odd) lds.flag = 1;
     lds_barrier();
     if (!lds.flag) return;
-    const uint64_t vis = visible<TREE>(a, s, my_token(), p);
+    uint64_t vis = visible<TREE>(a, s, my_token(), p);
+    if (kPairs) vis &= 0xffffffffull << 32 * mine;
     for (int t = 0; t < kTileKeys; ++t) {
       const uint16_t* src = (const uint16_t*)lds.v[buf] + (t >> 3) * D * 8 + (t & 7);
       const bool sees = vis >> t & 1;
@@ -561,12 +571,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       wait_vmem_but<kLoads>();
     }
     lds_barrier();
-    read_k(0, 0);
+    read_k(0, mine);
     scores(0, kQ);
-    less_maximum(0, 0);
-    mask_scores(0, p);
+    less_maximum(0, mine);
+    mask_scores(mine, p);
     top = maximum();
-    read_k(0, 1);
+    if (!kPairs) read_k(0, 1);
     if (I8) {
       land_v(0, raw_v);
       land_k(1, 1, raw_k1);
@@ -621,12 +631,81 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     p1 = p2;
     at1 = at2;
   };
+  Raw raw_k = {};
+  // The same for a pair: one half tile of each tile, whose keys for the next
+  // tile are read at its start.
+  auto pair_step = [&](auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
+    wait_vmem();
+    lds_barrier();
+    const int p2 = find(p1 + kTileKeys, &at2);
+    if (p1 < end) load_v(at1, buf ^ 1, raw);
+    if (p2 < end) load_k(at2, buf, raw_k);
+    if (p + kTileKeys > open) clean(buf, p);
+    rescale(top);
+    const f32x16 x = st;
+    __builtin_amdgcn_sched_barrier(0);
+    if (!I8) read_k(buf ^ 1, mine);
+    weights(x, buf, mine);
+    if (I8) read_k(buf ^ 1, mine);
+    scores(0, kQ);  // of the next tile
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(buf, mine, 0, 1);
+    products(0, kO);
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(buf, mine, 1, 2);
+    products(kO, 2 * kO);
+    less_maximum(n + 1, mine);
+    top = maximum();
+    if (mask_scores(mine, p1)) top = maximum();
+    if (I8) {
+      land_v(buf ^ 1, raw);
+      land_k(buf, n + 2, raw_k);
+    }
+    ++n;
+    p = p1;
+    p1 = p2;
+    at1 = at2;
+  };
+  auto step = [&](auto buffer) __attribute__((always_inline)) {
+    if constexpr (kPairs)
+      pair_step(buffer);
+    else
+      tile_step(buffer);
+  };
   while (p < end) {
-    tile_step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 0>{});
     if (p >= end) break;
-    tile_step(std::integral_constant<int, 1>{});
+    step(std::integral_constant<int, 1>{});
   }
   l = add_xor32(l);
+  if (kPairs) {  // the second pair's results, added to the first's (whose keys and values are read)
+    float* const s_o = (float*)lds.k + (wave & 1) * (D / 2) * 64 + lane;
+    float* const s_ml = (float*)lds.v + (wave & 1) * 128 + lane;
+    m = limit == kSlack ? m : kLowest;
+    lds_barrier();
+    if (wave >= 2) {
+#pragma unroll
+      for (int i = 0; i < kO; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s_o[(i * 16 + r) * 64] = o[i][r];
+      s_ml[0] = m;
+      s_ml[64] = l;
+    }
+    lds_barrier();
+    if (wave >= 2) return;
+    const float m2 = s_ml[0], both = fmaxf(m, m2);
+    const float f = __builtin_amdgcn_exp2f(m - both), f2 = __builtin_amdgcn_exp2f(m2 - both);
+    m = both;
+    limit = m > kLowest ? kSlack : limit;
+    l = l * f + s_ml[64] * f2;
+#pragma unroll
+    for (int i = 0; i < kO; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] = o[i][r] * f + s_o[(i * 16 + r) * 64] * f2;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
   const int out_row = my_row();
   if (out_row >= rows) return;
   if (row_end > part.chunk) {  // the join adds the parts
@@ -969,9 +1048,9 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
   const int h = (int)(blockIdx.x % (unsigned)HK);
   const int rest = (int)(blockIdx.x / (unsigned)HK);
   const int item = rest / row_blocks;
-  const int b = ROWS == kRowRows ? item : sequence_of_tile(a, G, item, lane);
+  const int b = part.whole ? item : sequence_of_tile(a, G, item, lane);
   const SeqWords words = sequence_words(a, b);
-  const int block = ROWS == kRowRows ? 0 : block_of_tile(a, G, item, b, words);
+  const int block = part.whole ? 0 : block_of_tile(a, G, item, b, words);
   const Seq s = sequence(c, a, b, words, false);
   const int rows = s.n * G, r0 = block * ROWS;
   if (block < 0 || r0 >= rows) return;
@@ -1048,8 +1127,10 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
   Plan p = {};
   const int64_t G = heads / c.kv_heads;
   p.row_form = max_queries * G <= kRowRows;
-  p.part.rows = p.row_form ? (int)(max_queries > 0 ? max_queries * G : G) : kTileRows;
-  p.part.items = (int)(p.row_form ? seqs : tokens * G / kTileRows + seqs);
+  const int tile_rows = max_queries * G <= kPairRows ? kPairRows : kTileRows;
+  p.part.rows = p.row_form ? (int)(max_queries > 0 ? max_queries * G : G) : tile_rows;
+  p.part.whole = p.row_form || max_queries * G <= tile_rows;
+  p.part.items = (int)(p.part.whole ? seqs : tokens * G / tile_rows + seqs);
   if (p.part.items < 1) p.part.items = 1;
   const int64_t wgs = (int64_t)p.part.items * c.kv_heads;
   int64_t splits = 1, least = 256, most = (int64_t)1 << 30;
@@ -1067,10 +1148,12 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
   } else if (wgs < 512) {
     // About one and a half rounds of workgroups (two run on a CU at a time);
     // in us, for 512, 768 and 1536 of them: 1000 tokens bf16 33, 31, 42; four
-    // drafts of 32 on 8000 tokens 41, 39, 52.  Parts of fewer than 256 tokens
+    // drafts of 32 on 8000 tokens 41, 39, 52.  One round where the items are
+    // counted, not bounded: 32 drafts of 8 on 4000 tokens, 32 / 4 heads, bf16 60
+    // for 512, 71 for 768.  Parts of fewer than 256 tokens
     // cost more than they give (512 tokens 20, in parts of 128 24), but for the
     // least launches (a draft of 12 on 500 tokens 13.5, in parts of 128 11.5).
-    splits = (768 + wgs / 2) / wgs;
+    splits = ((p.part.whole ? 512 : 768) + wgs / 2) / wgs;
     if (wgs <= 64) least = 128;
   } else if (wgs < 1536 && max_len >= 4096) {
     // Up to three rounds of long ones: parts even out the last round (chunks
@@ -1101,7 +1184,7 @@ struct JoinPlan {
 JoinPlan join_of(const CacheView& c, const Plan& p) {
   if (p.row_form && p.part.splits <= 8) return {4, (p.part.rows + 3) / 4};
   if (p.row_form) return {16, p.part.rows};
-  if ((int64_t)p.part.items * c.kv_heads <= 64) return {4, kTileRows / 4};
+  if ((int64_t)p.part.items * c.kv_heads <= 64) return {4, p.part.rows / 4};
   return {1, 2};
 }
 
@@ -1130,8 +1213,10 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
       constexpr bool TREE = decltype(tree)::value;
       if (p.row_form)
         hipLaunchKernelGGL((attn_row_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
+      else if (p.part.rows == kPairRows)
+        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE, kPairRows>), grid, dim3(256), 0, stream, c, a, p.part);
       else
-        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
+        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE, kTileRows>), grid, dim3(256), 0, stream, c, a, p.part);
       if (p.part.splits == 1) return;
       const JoinPlan j = join_of(c, p);
       const dim3 join_grid((unsigned)(p.part.items * c.kv_heads * j.row_blocks));
@@ -1140,16 +1225,18 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
         hipLaunchKernelGGL((join_kernel<D, TREE, ROWS, SP>), join_grid, dim3(256), 0, stream, c, a, p.part,
                            (int)j.row_blocks);
       };
-      std::integral_constant<int, kRowRows> row_form;
-      std::integral_constant<int, kTileRows> tile_form;
-      if (p.row_form && j.groups == 4)
-        join(row_form, std::integral_constant<int, 4>{});
-      else if (p.row_form)
-        join(row_form, std::integral_constant<int, 16>{});
-      else if (j.groups == 4)
-        join(tile_form, std::integral_constant<int, 4>{});
+      const std::integral_constant<int, 1> one;
+      const std::integral_constant<int, 4> four;
+      const std::integral_constant<int, 16> sixteen;
+      const std::integral_constant<int, kRowRows> row_form;
+      const std::integral_constant<int, kPairRows> narrow;
+      const std::integral_constant<int, kTileRows> tile;
+      if (p.row_form)
+        j.groups == 4 ? join(row_form, four) : join(row_form, sixteen);
+      else if (p.part.rows == kPairRows)
+        j.groups == 4 ? join(narrow, four) : join(narrow, one);
       else
-        join(tile_form, std::integral_constant<int, 1>{});
+        j.groups == 4 ? join(tile, four) : join(tile, one);
     };
     a.tree ? launch(std::true_type{}) : launch(std::false_type{});
   });

@@ -107,6 +107,26 @@ def test_trees(gpu_device, heads, kv_heads, dim, page, fmt, counts, contexts):
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lengths", [[5, 31, 33, 64, 65, 100, 129, 4], [9, 700, 64, 2049, 90, 127, 6, 40],
+                                     [6100, 5, 3000, 20]])
+def test_few_rows(gpu_device, fmt, dim, lengths):
+    """17 to 64 rows per sequence (and sequences of none, and with more rows than tokens beside them): drafts
+    and causal rows, alone and in parts."""
+    counts = [5, 16, 1, 8, 13, 0, 7, 3][:len(lengths)]
+    announce(f"few rows {fmt} dim {dim} rows {counts} of {lengths}")
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=dim, fmt=fmt, page=64, seed=sum(lengths))
+    g = generator(len(lengths))
+    q = randn(g, sum(counts), 8, dim)
+    mask = random_trees(g, counts)
+    for most in (16, None):  # 64 rows bound the launch, then the whole batch's
+        check_attention(p, counts, q, p.attn.forward(q, p.table, p.lens, starts_of(counts), max_queries=most))
+        check_attention(p, counts, q, p.attn.forward_tree(q, mask, p.table, p.lens, starts_of(counts), max_queries=most),
+                        mask)
+    assert not any(p.attn.status().values())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
 def test_tree_rows_that_see_nothing(gpu_device, fmt):
     """Masks with empty rows and no context (zeros), without the row's own bit, with bits past the draft,
     and masks shorter than the draft."""
@@ -135,7 +155,7 @@ def test_tree_rows_that_see_nothing(gpu_device, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "int8"])
-@pytest.mark.parametrize("counts", [[1, 1], [20, 5], [90, 130]])
+@pytest.mark.parametrize("counts", [[1, 1], [16, 5], [20, 5], [90, 130]])
 def test_unseen_tokens_do_not_reach_a_row(gpu_device, fmt, counts):
     """NaN and infinities in later tokens (causal) and in unseen branches (trees): the rows that do not see
     them keep their bits; the rows that do are NaN or infinite as the formula's."""
@@ -195,11 +215,15 @@ def test_large_scores(gpu_device, fmt):
         p.k[b], p.v[b] = dense(p.attn, slots)
     q = torch.cat([base.repeat_interleave(4, dim=1)] * 4).to(torch.bfloat16) * 8
     got = p.attn.forward(q, p.table, p.lens, starts_of([2, 2]))
+    # the same rows in the launch for more of them: each form within the bounds below of the same values
+    other = p.attn.forward(torch.cat([q[:1].expand(8, -1, -1), q[:2], q[2:3].expand(6, -1, -1), q[2:]]), p.table, p.lens,
+                           starts_of([10, 8]))
     # scores up to 8 * 6 * |base|^2 / sqrt(128) ~ 550 with one sign: an fp32 score is off by 2^-24 * 136 * 550
     # (2^-7.8 would come out of a sum of 128 such roundings; they add as a walk: 2^-24 * 12 * 550 * 4 < 2^-9)
     for b in range(2):
         want, A = reference(q[2 * b:2 * b + 2], p.k[b], p.v[b], causal(2, 700), p.attn.scale)
-        assert bool(((got[2 * b:2 * b + 2].double() - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -7) * A).all())
+        for x in (got[2 * b:2 * b + 2], other[[8, 9] if b == 0 else [16, 17]]):
+            assert bool(((x.double() - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -7) * A).all())
 
 
 def test_rows_behind_the_last_sequence_stay(gpu_device):
