@@ -206,9 +206,9 @@ __device__ __forceinline__ int end_of_rows(const Seq& s, int G, int r0, int coun
 //
 // Bound by the two units' shares of a SIMD's time and by power, not by memory.  A
 // prompt of 8192 tokens, 32 / 4 heads, D = 128, bf16: 521 us, 1.05 PFLOP/s (a
-// library product of 16384^3: 1.36), at a clock that falls to 1.83 of 2.4 GHz;
-// matrix cores busy 51 % of it, the vector unit 47 %, 5.3 vector instructions per
-// matrix one, waves waiting 20 %, no bank conflict.
+// library product of 16384^3: 1.36), at a clock that falls to 1.8 of 2.4 GHz (557
+// on a card that holds less); matrix cores busy 51 % of it, the vector unit 47 %,
+// 5.3 vector instructions per matrix one, waves waiting 20 %, no bank conflict.
 // int8, three chunks of 1021 tokens on up to 9000, 32 / 8 heads: 398 us and 21
 // of join, 0.71 PFLOP/s; 31 % and 50 %, 10.7 vector instructions: widening the
 // codes and the two scales are what it has more.
