@@ -56,7 +56,8 @@ extern "C" {
 
 /* bits of the status word */
 #define NKT_ATTN_STATUS_BAD_SLOT 1u     /* a slot past the cache: not stored, read as zeros */
-#define NKT_ATTN_STATUS_BAD_POSITION 2u /* a position outside the rotation table: queries zero, nothing stored */
+#define NKT_ATTN_STATUS_BAD_POSITION 2u /* a position outside the rotation table, of a token that is not padding:
+                                           queries zero, nothing stored */
 #define NKT_ATTN_STATUS_BAD_PAGE 4u     /* a page outside the cache: its tokens are not seen, not moved */
 #define NKT_ATTN_STATUS_BAD_LENGTH 8u   /* a length past max_seq_len or the table (cut), negative (0), or a sequence
                                            with more than max_queries rows (the rest left as they were) */
@@ -87,7 +88,8 @@ int nkt_attn_bind_cache(void* handle, void* const* ptrs, char* err, size_t err_l
  * in fp32 with one rounding, to bf16 for q_out [T, num_heads, D] (which may be
  * q itself if its tokens are dense) and to the cache's format for the keys; values are stored as they
  * are.  slots int64 [T]: where each token's key and value go; a negative slot
- * stores nothing (padding).  The slots of one call are distinct: what a slot
+ * stores nothing (padding, whose position may be anything: outside the table
+ * its queries are zero).  The slots of one call are distinct: what a slot
  * given twice holds is undefined. */
 int nkt_attn_write(void* handle, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                    int64_t v_stride, const int64_t* positions, const int64_t* slots, const float* rope,

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void write_kernel(CacheView c, WriteArgs 
     const int64_t pos = a.positions[t];
     const int64_t given = a.slots[t];
     const bool pos_ok = pos >= 0 && pos < a.rope_rows;
-    if (!pos_ok && l == 0) report(c.status, kBadPosition);
+    if (!pos_ok && given >= 0 && l == 0) report(c.status, kBadPosition);  // (padding may have any)
     const float* rp = a.rope + (pos_ok ? pos : 0) * D;
     const f32x4 cs = *(const f32x4*)(rp + 4 * l);
     const f32x4 sn = *(const f32x4*)(rp + D / 2 + 4 * l);

@@ -222,7 +222,7 @@ class NativeAttention:
               eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Queries and keys normalised per head (by ``q_norm`` / ``k_norm`` [head_dim], where given) and rotated
         by their positions' rows of ``rope`` (``rope_table``); keys and values stored at ``slots`` (negative:
-        not stored), the queries returned [T, num_heads, head_dim].  q, k and v may be parts of one
+        not stored, padding, at any position), the queries returned [T, num_heads, head_dim].  q, k and v may be parts of one
         projection's output.  The slots of one call have to be distinct."""
         q = self._strided(q, self.num_heads, "q")
         T = q.shape[0]
