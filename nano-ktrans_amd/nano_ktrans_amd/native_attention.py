@@ -27,6 +27,9 @@ from . import _native as N
 
 _FORMATS = {"bf16": N.CACHE_BF16, "int8": N.CACHE_INT8}
 
+# words of the status tensor: the kernels' (bits added atomically), one that says nothing, and ``slots``'s own
+_STATUS_KERNELS, _STATUS_SPARE, _STATUS_SLOTS = 0, 1, 2
+
 # the current stream's handle without building a Stream object (2 us of a 12 us call)
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -205,7 +208,9 @@ class NativeAttention:
     # ------------------------------------------------------------------ cache
     def slots(self, page_table: torch.Tensor, seqs: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """int64 slots of the tokens at ``positions`` of the sequences ``seqs`` (rows of the page table): -1 for
-        a negative position (padding), a slot past the cache, which ``write`` reports, for one past the table."""
+        a negative position (padding), a slot past the cache, which ``write`` reports, for one past the table.
+        A token whose entry of the table is no page of the cache (an unallocated one) gets a slot that nothing
+        is stored at and is reported here, as ``bad_page``: ``write`` could not tell a negative one from padding."""
         B, W = page_table.shape
         seqs, positions = seqs.long(), positions.long()
         past = self.num_pages * self.page_size
@@ -214,8 +219,12 @@ class NativeAttention:
         at = torch.div(positions, self.page_size, rounding_mode="floor")
         inside = (at < W) & (seqs >= 0) & (seqs < B)
         pages = page_table[seqs.clamp(0, B - 1), at.clamp(0, W - 1)].long()
-        slots = torch.where(inside, pages * self.page_size + positions % self.page_size, past)
-        return slots.masked_fill(positions < 0, -1)
+        padding = positions < 0
+        bad = ((pages < 0) | (pages >= self.num_pages)) & inside & ~padding
+        # (a word that only this call writes, and never reads: kernels on other streams add their bits to theirs)
+        self._status.index_fill_(0, _STATUS_SPARE + bad.any().view(1).long(), N.ATTN_STATUS["bad_page"])
+        slots = torch.where(inside, pages.clamp(-1, self.num_pages) * self.page_size + positions % self.page_size, past)
+        return slots.masked_fill(padding, -1)
 
     def write(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
               rope: torch.Tensor, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
@@ -343,7 +352,8 @@ class NativeAttention:
     def status(self) -> Dict[str, bool]:
         """What calls found out of range on the device since the status was last cleared (synchronises)."""
         torch.cuda.synchronize(self.device)
-        word = int(self._status[0].item())
+        words = self._status.tolist()
+        word = words[_STATUS_KERNELS] | words[_STATUS_SLOTS]
         return {name: bool(word & bit) for name, bit in N.ATTN_STATUS.items()}
 
     def check_status(self, clear: bool = True) -> None:

@@ -51,3 +51,45 @@ def test_padding_positions_are_no_error(gpu_device, fmt, tokens):
     slots[1] = 5
     attn.write(q, k, v, positions, slots, rope)
     assert attn.status() == {name: name == "bad_position" for name in N.ATTN_STATUS}
+
+
+def test_slots_report_pages_that_no_sequence_has(gpu_device):
+    """A token whose page-table entry is not a page of the cache gets no slot of it (``write`` stores nothing) and
+    is reported; padding, and entries that no token needs, are not.  In a captured graph as well."""
+    announce("slots of unallocated pages")
+    attn = make_attention(2, 1, 64, "bf16", 64, 9)
+    poison(attn)
+    table = torch.tensor([[7, 2, -1], [0, -1, 9]], dtype=torch.int32, device=DEV)
+    seqs = torch.tensor([0, 0, 1, 1, 0], device=DEV)
+    fine = torch.tensor([3, 64, 63, -1, -130], device=DEV)
+    attn.slots(table, seqs, fine)
+    attn.check_status()
+    g = generator(2)
+    q, k, v = randn(g, 5, 2, 64), randn(g, 5, 1, 64), randn(g, 5, 1, 64)
+    rope = rope_table(256, 64, 1e4, DEV)
+    positions = fine.clone()
+    positions[3] = 70
+    slots = attn.slots(table, seqs, positions)
+    attn.write(q, k, v, positions, slots, rope)
+    assert attn.status() == {name: name == "bad_page" for name in N.ATTN_STATUS}
+    with pytest.raises(N.NativeError, match="bad_page"):
+        attn.check_status()
+    attn.check_status()
+    every = torch.arange(9 * 64, device=DEV)
+    stored = ~torch.isnan(dense(attn, every)[0]).flatten(1).any(dim=1)
+    assert every[stored].tolist() == [63, 2 * 64, 7 * 64 + 3]
+    for at in (130, -2):
+        positions[3] = at  # a page past the cache; padding
+        attn.slots(table, seqs, positions)
+        assert attn.status()["bad_page"] == (at > 0)
+        attn._status.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = attn.slots(table, seqs, positions)
+    for at, bad in ((70, True), (5, False), (-1, False), (69, True)):
+        positions[3] = at
+        graph.replay()
+        assert attn.status()["bad_page"] == bad, at
+        attn._status.zero_()
+        assert torch.equal(held, attn.slots(table, seqs, positions))
+        attn._status.zero_()
