@@ -157,7 +157,8 @@ class NativeAttention:
         if t.dtype != dtype:
             if t.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"{name} must be an integer tensor, got {t.dtype}")
-            t = t.to(dtype)
+            # (what 32 bits do not hold stays out of range, rather than what its lower half says)
+            t = t.to(dtype) if dtype == torch.int64 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(dtype)
         if t.shape != shape:
             raise ValueError(f"{name} is {tuple(t.shape)}, expected {shape}")
         return t if t.is_contiguous() else t.contiguous()

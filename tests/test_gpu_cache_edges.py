@@ -4,7 +4,7 @@ import sys
 import pytest
 import torch
 
-from attn_cases import DEV, U, dense, generator, make_attention, poison, randn, rotated
+from attn_cases import DEV, U, dense, generator, make_attention, make_problem, poison, randn, rotated
 from nano_ktrans_amd import rope_table
 from nano_ktrans_amd import _native as N
 from test_gpu_cache import check_stored
@@ -93,3 +93,26 @@ def test_slots_report_pages_that_no_sequence_has(gpu_device):
         attn._status.zero_()
         assert torch.equal(held, attn.slots(table, seqs, positions))
         attn._status.zero_()
+
+
+def test_keep_takes_64_bit_indexes_for_what_they_are(gpu_device):
+    """Kept indexes, counts, contexts and pages that 32 bits do not hold are out of range and reported, not what
+    their lower half says."""
+    announce("keep: 64-bit indexes")
+    for which, bit in (("table", "bad_page"), ("context", "bad_kept"), ("kept", "bad_kept"), ("counts", "bad_kept")):
+        p = make_problem([100, 100], heads=4, kv_heads=2, dim=64, fmt="int8", page=64, seed=1, width=2)
+        args = {"table": p.table.long(), "context": torch.tensor([20, 20], device=DEV),
+                "kept": torch.tensor([[1, 3], [2, 5]], device=DEV), "counts": torch.tensor([2, 2], device=DEV)}
+        args[which][(0,) * args[which].dim()] += 1 << 32
+        p.attn.keep(args["table"], args["context"], args["kept"], args["counts"])
+        st = p.attn.status()
+        assert st == {name: name == bit for name in N.ATTN_STATUS}, which
+        # the second sequence is not affected; of the first, what is out of range is not moved
+        moved = [{} if which in ("table", "context") else {1: 3} if which == "kept" else {0: 1, 1: 3}, {0: 2, 1: 5}]
+        for b, m in enumerate(moved):
+            at = torch.arange(100, device=DEV)
+            index = at.clone()
+            for to, src in m.items():
+                index[20 + to] = 20 + src
+            k, v = dense(p.attn, p.attn.slots(p.table, torch.full_like(at, b), at))
+            assert torch.equal(k, p.k[b][index]) and torch.equal(v, p.v[b][index]), (which, b)
