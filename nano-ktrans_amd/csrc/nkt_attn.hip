@@ -491,9 +491,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   };
   // Values that some row must not see (or that lie past the sequence's end)
   // would still meet a weight of zero in the matrix products: 0 x NaN.  In
-  // tiles with masked tokens, values past the end become zero, and if a
-  // value is not finite, it is added by hand to the rows that see it (int8:
+  // tiles with masked tokens, values past the end become zero, as do those that
+  // are not finite, which add_odd adds to the rows that see them (int8:
   // values' scales instead, and such rows are NaN).
+  int odd_from = end;  // the first tile with such values
   auto clean = [&](int buf, int p) __attribute__((always_inline)) {
     if (I8) {
       const float f = lds.vs[buf][lane];
@@ -524,20 +525,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     if (odd) lds.flag = 1;
     lds_barrier();
     if (!lds.flag) return;
-    uint64_t vis = visible<TREE>(a, s, my_token(), p);
-    if (kPairs) vis &= 0xffffffffull << 32 * mine;
-    for (int t = 0; t < kTileKeys; ++t) {
-      const uint16_t* src = (const uint16_t*)lds.v[buf] + (t >> 3) * D * 8 + (t & 7);
-      const bool sees = vis >> t & 1;
-#pragma unroll
-      for (int i = 0; i < kO; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const uint32_t x = src[(i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * 8];
-          o[i][r] += sees && (x & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(x) : 0.f;
-        }
-    }
-    lds_barrier();
+    odd_from = p < odd_from ? p : odd_from;
     for (int i = tid; i < kTileKeys * kChunks; i += 256) {
       u32x4 w = *(const u32x4*)(lds.v[buf] + i * 16);
 #pragma unroll
@@ -548,6 +536,28 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       *(u32x4*)(lds.v[buf] + i * 16) = w;
     }
     lds_barrier();
+  };
+
+  // The values that clean took out, from the cache, to the sums of the rows that
+  // see them: once nothing rescales these any more (infinity x 0).
+  auto add_odd = [&] {
+    for (int p = odd_from; p < end; p += kTileKeys) {
+      const int64_t page = a.table[(int64_t)b * a.width + (p >> c.page_shift)];
+      if (page < 0 || page >= c.num_pages) continue;
+      const int64_t at = ((page * HK + h) << c.page_shift) + (p & mask);
+      const uint64_t vis = visible<TREE>(a, s, my_token(), p);
+      for (int t = 0; t < kTileKeys; ++t) {
+        const uint16_t* src = (const uint16_t*)c.v + at * D + (t >> 3) * D * 8 + (t & 7);
+        const bool sees = vis >> t & 1;
+#pragma unroll
+        for (int i = 0; i < kO; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const uint32_t x = src[(i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * 8];
+            o[i][r] += sees && (x & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(x) : 0.f;
+          }
+      }
+    }
   };
 
   // tile t: at position p, in key and value buffer buf; tile t + 1: p1, its
@@ -707,6 +717,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+  if (!I8 && odd_from < end) add_odd();
   const int out_row = my_row();
   if (out_row >= rows) return;
   if (row_end > part.chunk) {  // the join adds the parts
@@ -873,8 +884,10 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     const int valid = x.ok ? s.len - p : 0;  // tokens of the step that exist
     const bool masks = p + KS > open || valid < KS;
     uint32_t vis = ~0u;
+    uint64_t bits = 0;
+    bool odd = false;
     if (masks) {
-      uint64_t bits = visible<TREE>(a, s, token, p);
+      bits = visible<TREE>(a, s, token, p);
       if (valid < KS) bits &= (1ull << valid) - 1;
       vis = (uint32_t)(bits >> (g * (KS / 4)));
       if (!x.ok && lane == 0) report(c.status, kBadPage);
@@ -883,10 +896,9 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[t][r] = vis >> (t * 4 + r) & 1 ? st[t][r] : -__builtin_huge_valf();
       if (!I8) {
-        // values past the end become zero; one that is not finite, which some
-        // row may not see, is added by hand to the rows that do (0 x NaN)
+        // values past the end become zero; so do those that are not finite, which
+        // some row may not see (0 x NaN): the rows that do get them below
         const int inside = valid - g * 8;
-        bool odd = false;
 #pragma unroll
         for (int i = 0; i < kO; ++i)
 #pragma unroll
@@ -895,18 +907,8 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
             x.v[i][j] &= keep;
             odd |= non_finite_pair(x.v[i][j]);
           }
-        if (__any(odd)) {
-          for (int t = 0; t < KS && t < valid; ++t) {
-            const uint16_t* src = (const uint16_t*)c.v + x.at * D + (t >> 3) * D * 8 + (t & 7);
-            const bool sees = bits >> t & 1;
-#pragma unroll
-            for (int i = 0; i < kO; ++i)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const uint32_t e = src[(i * 16 + g * 4 + r) * 8];
-                o[i][r] += sees && (e & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(e) : 0.f;
-              }
-          }
+        odd = __any(odd);
+        if (odd) {
 #pragma unroll
           for (int i = 0; i < kO; ++i)
 #pragma unroll
@@ -932,6 +934,19 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
       l *= fix;
 #pragma unroll
       for (int i = 0; i < kO; ++i) o[i] *= fix;
+    }
+    if (odd) {  // (past the rescale: infinity x 0)
+      for (int t = 0; t < KS && t < valid; ++t) {
+        const uint16_t* src = (const uint16_t*)c.v + x.at * D + (t >> 3) * D * 8 + (t & 7);
+        const bool sees = bits >> t & 1;
+#pragma unroll
+        for (int i = 0; i < kO; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t e = src[(i * 16 + g * 4 + r) * 8];
+            o[i][r] += sees && (e & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(e) : 0.f;
+          }
+      }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)

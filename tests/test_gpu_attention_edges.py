@@ -5,9 +5,12 @@ import sys
 import pytest
 import torch
 
-from attn_cases import DEV, generator, make_problem, randn, split_rows
+from attn_cases import DEV, check_attention, dense, generator, make_problem, put, randn, split_rows
 
 pytestmark = pytest.mark.gpu
+
+# rows per sequence of 8 / 2 heads: the row form, the 64-row form and the tile form
+FORMS = [[1, 1], [3, 4], [5, 16], [40, 70]]
 
 
 def announce(msg):
@@ -17,6 +20,44 @@ def announce(msg):
 
 def starts_of(counts):
     return torch.tensor(split_rows(counts), dtype=torch.int32, device=DEV)
+
+
+def signs(g, *shape):
+    return 1.0 - 2.0 * torch.randint(0, 2, shape, generator=g, device=DEV).float()
+
+
+def store(p, b, k, v):
+    """Keys and values [len, HK, D] (fp32) as sequence b's, and what the cache then holds of them."""
+    at = torch.arange(p.lengths[b], device=DEV)
+    slots = p.attn.slots(p.table, torch.full_like(at, b), at)
+    put(p.attn, slots, k, v)
+    p.k[b], p.v[b] = dense(p.attn, slots)
+
+
+def attend(p, counts, q):
+    return p.attn.forward(q, p.table, p.lens, starts_of(counts), max_queries=max(counts))
+
+
+@pytest.mark.parametrize("counts", FORMS)
+@pytest.mark.parametrize("lengths", [[80, 75], [700, 3000]])
+def test_infinite_values_reach_the_rows_that_see_them(gpu_device, counts, lengths):
+    """An infinity in a value, beside later tokens: the rows that see it are infinite there and nowhere else
+    (not NaN), also where its own score lies far above all before it.  Such rows' weights are 0 and 1 (the
+    next score is 2^-250 of it), so their scores' size adds no error."""
+    announce(f"infinite values, rows {counts} of {lengths}")
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=128, fmt="bf16", page=64, seed=3)
+    g = generator(5)
+    base = signs(g, 2, 128)
+    for b, (n, length) in enumerate(zip(counts, lengths)):
+        for far in (False, True):
+            k, v = 0.01 * randn(g, length, 2, 128).float(), randn(g, length, 2, 128).float()
+            at = length - 1 - n // 2
+            if far:
+                k[at] = base
+            v[at, 0, 3], v[at, 1, 70], v[at, 1, 71] = float("inf"), float("-inf"), float("inf")
+            store(p, b, k, v)
+            q = (16 * base).repeat_interleave(4, dim=0).to(torch.bfloat16).expand(sum(counts), -1, -1).contiguous()
+            check_attention(p, counts, q, attend(p, counts, q))
 
 
 @pytest.mark.parametrize("counts", [None, [9, 40]])
