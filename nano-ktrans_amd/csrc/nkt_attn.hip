@@ -112,6 +112,14 @@ constexpr float kLowest = -1.0e38f;  // the running maximum before any score
 // bf16 weight's relative precision notice, and most tiles skip the rescale.
 constexpr float kSlack = 8.0f;
 
+// A product that is rounded before the maximum is taken off it.  Contracted with
+// the subtraction it would keep bits that the maximum has lost: from 2^31 on, a
+// score less the maximum that it is itself could reach 2^7, its weight infinity.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 __device__ __forceinline__ bool non_finite_pair(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
@@ -878,8 +886,13 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
       for (int t = 0; t < NT; ++t) {
         const f32x4 f = *(const f32x4*)&s_scale[wave][0][g * 16 + t * 4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st[t][r] *= f[r];
+        for (int r = 0; r < 4; ++r) st[t][r] = rounded_product(st[t][r], f[r]);
       }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[t][r] = rounded_product(st[t][r], scale2);
     }
     const int valid = x.ok ? s.len - p : 0;  // tokens of the step that exist
     const bool masks = p + KS > open || valid < KS;
@@ -925,7 +938,6 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, st[t][r]);
     top = max_xor32(max_xor16(top));
-    if (!I8) top *= scale2;
     const bool moves = top > m + kSlack;
     if (__any(moves)) {
       const float to = moves ? top : m;
@@ -952,7 +964,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        st[t][r] = __builtin_amdgcn_exp2f(I8 ? st[t][r] - m : st[t][r] * scale2 - m);
+        st[t][r] = __builtin_amdgcn_exp2f(st[t][r] - m);
         l += st[t][r];
       }
     if (I8) {

@@ -60,6 +60,28 @@ def test_infinite_values_reach_the_rows_that_see_them(gpu_device, counts, length
             check_attention(p, counts, q, attend(p, counts, q))
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("counts", FORMS)
+@pytest.mark.parametrize("lengths", [[80, 75], [700, 3000]])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_past_24_bits(gpu_device, fmt, counts, lengths, sign):
+    """Finite scores of 2^35 to 2^125, one token's above all others' by a part of itself: its value, whatever a
+    product of such a score keeps of its lower bits.  (fp32 scores are off by 2^-16 of their terms' sum at most,
+    the gaps are 2^-7 of the largest and more, so all weights but that token's are 0.)"""
+    announce(f"large scores {fmt} rows {counts} of {lengths} sign {sign}")
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=128, fmt=fmt, page=64, seed=4)
+    g = generator(6)
+    base = signs(g, 2, 128)
+    for power in (15, 33, 55):
+        for b, (n, length) in enumerate(zip(counts, lengths)):
+            c = torch.randint(2, 127, (length,), generator=g, device=DEV).float()
+            c[length - n - b] = 128 if sign > 0 else 1  # (every row sees it)
+            store(p, b, c.view(-1, 1, 1) * base * 2.0 ** power, randn(g, length, 2, 128).float())
+        q = (sign * 2.0 ** power * base).repeat_interleave(4, dim=0).to(torch.bfloat16)
+        q = q.expand(sum(counts), -1, -1).contiguous()
+        check_attention(p, counts, q, attend(p, counts, q))
+
+
 @pytest.mark.parametrize("counts", [None, [9, 40]])
 def test_64_bit_indexes_do_not_wrap(gpu_device, counts):
     """Integers of 64 bits that 32 bits do not hold are out of range, not what their lower half says."""
