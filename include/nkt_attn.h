@@ -123,8 +123,10 @@ int nkt_attn_workspace_bytes(void* handle, int num_tokens, int num_seqs, int max
  * over the positions j <= seq_len - n + i of the sequence's i-th row (i < n).
  * q and out (which may be q itself) bf16 [num_tokens, num_heads, D], contiguous,
  * 16-byte aligned.  A row that sees nothing, or whose scores are all -infinity,
- * is zero; rows behind the last sequence are left as they were.  A token that a row does not see does not reach it, whatever the cache
- * holds there. */
+ * is zero; rows behind the last sequence are left as they were.  A token that a
+ * row does not see does not reach it, whatever the cache holds there.  Scores
+ * (and scale q . k log2(e)) are fp32: those past its range, and a row's that lie
+ * more than 2^127 apart, count as infinite. */
 int nkt_attn_forward(void* handle, const void* q, const int32_t* page_table, int table_width, const int32_t* seq_lens,
                      const int32_t* query_starts, int num_tokens, int num_seqs, int max_queries, int max_seq_len,
                      float scale, void* out, void* workspace, size_t workspace_bytes, void* stream, char* err,

@@ -106,11 +106,17 @@ __device__ __forceinline__ float max_xor16(float v) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLowest = -1.0e38f;  // the running maximum before any score
+constexpr float kUnseen = -__builtin_huge_valf();  // the running maximum before any score
 // The running maximum moves only when a score passes it by this much (in
 // log2): weights then reach 2^8 at most, which neither the fp32 sums nor a
 // bf16 weight's relative precision notice, and most tiles skip the rescale.
 constexpr float kSlack = 8.0f;
+
+// 2^(m - top): the factor that brings sums under maximum m to maximum top >= m
+// (0 for sums of no score, also where there is no other either).
+__device__ __forceinline__ float factor(float m, float top) {
+  return __builtin_amdgcn_exp2f(m - fmaxf(top, -__FLT_MAX__));
+}
 
 // A product that is rounded before the maximum is taken off it.  Contracted with
 // the subtraction it would keep bits that the maximum has lost: from 2^31 on, a
@@ -574,7 +580,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   int p = find(begin, &at);
   int p1 = find(p + kTileKeys, &at1);
   int n = 0;  // the tile's number; its buffers are n & 1
-  float top = kLowest;
+  float top = kUnseen;
   Raw raw = {};
   if (p < end) {
     // the first keys, values and second keys, all asked for at once
@@ -701,7 +707,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   if (kPairs) {  // the second pair's results, added to the first's (whose keys and values are read)
     float* const s_o = (float*)lds.k + (wave & 1) * (D / 2) * 64 + lane;
     float* const s_ml = (float*)lds.v + (wave & 1) * 128 + lane;
-    m = limit == kSlack ? m : kLowest;
+    m = limit == kSlack ? m : kUnseen;
     lds_barrier();
     if (wave >= 2) {
 #pragma unroll
@@ -714,9 +720,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     lds_barrier();
     if (wave >= 2) return;
     const float m2 = s_ml[0], both = fmaxf(m, m2);
-    const float f = __builtin_amdgcn_exp2f(m - both), f2 = __builtin_amdgcn_exp2f(m2 - both);
+    const float f = factor(m, both), f2 = factor(m2, both);
     m = both;
-    limit = m > kLowest ? kSlack : limit;
+    limit = m > kUnseen ? kSlack : limit;
     l = l * f + s_ml[64] * f2;
 #pragma unroll
     for (int i = 0; i < kO; ++i) {
@@ -737,7 +743,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
         *(f32x4*)(part.o + to * D + i * 32 + 8 * (r >> 2) + 4 * half) =
             f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
     if (half == 0) {
-      part.ml[2 * to] = limit == kSlack ? m : kLowest;
+      part.ml[2 * to] = limit == kSlack ? m : kUnseen;
       part.ml[2 * to + 1] = l;
     }
     return;
@@ -814,7 +820,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   f32x4 o[kO];
 #pragma unroll
   for (int i = 0; i < kO; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = kLowest, l = 0.f;
+  float m = kUnseen, l = 0.f;
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
   const int krow = (col >> 2) * (KS / 4) + (col & 3);
@@ -940,9 +946,8 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     top = max_xor32(max_xor16(top));
     const bool moves = top > m + kSlack;
     if (__any(moves)) {
-      const float to = moves ? top : m;
-      const float fix = __builtin_amdgcn_exp2f(m - to);
-      m = to;
+      const float fix = moves ? __builtin_amdgcn_exp2f(m - top) : 1.f;
+      m = moves ? top : m;
       l *= fix;
 #pragma unroll
       for (int i = 0; i < kO; ++i) o[i] *= fix;
@@ -960,11 +965,12 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
           }
       }
     }
+    const float less = fmaxf(m, -__FLT_MAX__);  // (a number: scores of -infinity have a weight of 0)
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        st[t][r] = __builtin_amdgcn_exp2f(st[t][r] - m);
+        st[t][r] = __builtin_amdgcn_exp2f(st[t][r] - less);
         l += st[t][r];
       }
     if (I8) {
@@ -1037,7 +1043,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   for (int d = 0; d < D / 16; ++d) out[d] = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float f = __builtin_amdgcn_exp2f(s_m[w][r] - top);
+    const float f = factor(s_m[w][r], top);
     sum += s_l[w][r] * f;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) out[d] += s_o[w][r][d0 + d] * f;
@@ -1090,14 +1096,14 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
   const int sp = group % SP;
   for (int base = rest % row_blocks * kRows; base < used; base += row_blocks * kRows) {
     const int r = base + group / SP;
-    float m = kLowest, l = 0.f, out[kN];
+    float m = kUnseen, l = 0.f, out[kN];
 #pragma unroll
     for (int d = 0; d < kN; ++d) out[d] = 0.f;
     for (int i = sp; i < splits && r < used; i += SP) {
       const int64_t at = part.row(item, h, HK, i, r);
       const float mi = part.ml[2 * at], li = part.ml[2 * at + 1];
       const float to = fmaxf(m, mi);
-      const float f = __builtin_amdgcn_exp2f(m - to), fi = __builtin_amdgcn_exp2f(mi - to);
+      const float f = factor(m, to), fi = factor(mi, to);
       m = to;
       l = l * f + li * fi;
 #pragma unroll
@@ -1125,7 +1131,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
         for (int d = 0; d < kN; ++d) out[d] = 0.f;
 #pragma unroll
         for (int i = 0; i < SP; ++i) {
-          const float f = __builtin_amdgcn_exp2f(s_m[group + i] - m);
+          const float f = factor(s_m[group + i], m);
           l += s_l[group + i] * f;
 #pragma unroll
           for (int d = 0; d < kN; ++d) out[d] += s_o[group + i][SP > 1 ? d0 + d : 0] * f;

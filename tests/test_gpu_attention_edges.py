@@ -82,6 +82,25 @@ def test_scores_past_24_bits(gpu_device, fmt, counts, lengths, sign):
         check_attention(p, counts, q, attend(p, counts, q))
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("counts", FORMS)
+@pytest.mark.parametrize("lengths", [[80, 75], [700, 3000]])
+def test_finite_scores_near_the_lowest_number(gpu_device, fmt, counts, lengths):
+    """Every score of a row is finite and below -1.2e38 (times log2(e)): such a row is not one that sees
+    nothing.  One token's score is a fifth above all others', so the row is its value."""
+    announce(f"lowest scores {fmt} rows {counts} of {lengths}")
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=128, fmt=fmt, page=64, seed=4)
+    p.attn.scale = 1.0
+    g = generator(7)
+    base = signs(g, 2, 128)
+    for b, (n, length) in enumerate(zip(counts, lengths)):
+        c = 1.25 + 0.125 * torch.randint(0, 11, (length,), generator=g, device=DEV).float()
+        c[length - n - b] = 1  # (every row sees it)
+        store(p, b, c.view(-1, 1, 1) * base * 2.0 ** 59, randn(g, length, 2, 128).float())
+    q = (-2.0 ** 60 * base).repeat_interleave(4, dim=0).to(torch.bfloat16).expand(sum(counts), -1, -1).contiguous()
+    check_attention(p, counts, q, attend(p, counts, q))
+
+
 @pytest.mark.parametrize("counts", [None, [9, 40]])
 def test_64_bit_indexes_do_not_wrap(gpu_device, counts):
     """Integers of 64 bits that 32 bits do not hold are out of range, not what their lower half says."""
