@@ -107,10 +107,17 @@ __device__ __forceinline__ float max_xor16(float v) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUnseen = -__builtin_huge_valf();  // the running maximum before any score
-// The running maximum moves only when a score passes it by this much (in
-// log2): weights then reach 2^8 at most, which neither the fp32 sums nor a
-// bf16 weight's relative precision notice, and most tiles skip the rescale.
+// Weights may differ by this much (in log2) from what the row's largest score so
+// far gives, so that most tiles skip the rescale; neither the fp32 sums nor a bf16
+// weight's relative precision notice.  A score that passes the running maximum m
+// moves it to `above` over itself, and m moves again once a score passes it by
+// kSlack - above.  bf16: above = kSlack, no weight is over 1, and a sum passes
+// fp32's range only if the values' own sum may.  int8 rounds weight x scale to bf16,
+// where weights of 2^-8 would cost the smallest scales their bits: above = 0
+// until a value's scale passes kLargeScale, then as bf16 (2^20 tokens x a weight
+// of 2^8 x 127 x kLargeScale are within the range).
 constexpr float kSlack = 8.0f;
+constexpr float kLargeScale = 0x1p90f;
 
 // 2^(m - top): the factor that brings sums under maximum m to maximum top >= m
 // (0 for sums of no score, also where there is no other either).
@@ -312,9 +319,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  // Running maximum (log2), sum, and what a score must pass m by for m to move:
-  // -infinity until the row has seen a token, then kSlack.
+  // Running maximum (log2), sum, and what a score less m must pass for m to move:
+  // -infinity until the row has seen a token, then kSlack - above.
   float m = 0.f, l = 0.f, limit = -__builtin_huge_valf();
+  float above = I8 ? 0.f : kSlack;
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
 
@@ -463,13 +471,19 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     for (int r = 3; r < 15; r += 2) top = fmaxf(fmaxf(top, st[r]), st[r + 1]);
     return max_xor32(fmaxf(top, st[15]));
   };
-  auto rescale = [&](float top) {
+  float top = kUnseen;  // of the next half tile's scores, less m
+  // (scale: of the lane's token, int8, once per tile)
+  auto rescale = [&](float scale) {
     const bool moves = top > limit;
-    if (__any(moves)) {
-      const float by = moves ? top : 0.f;
-      const float fix = limit == kSlack ? __builtin_amdgcn_exp2f(-by) : 1.f;  // (nothing to rescale before)
+    const bool large = I8 && above == 0.f && scale > kLargeScale;
+    if (__any(moves || large)) {
+      const float up = I8 && __any(large) ? kSlack : 0.f;
+      above += up;
+      const bool seen = limit >= 0.f;  // (nothing to rescale before)
+      const float by = moves ? top + above : seen ? up : 0.f;
+      const float fix = seen ? __builtin_amdgcn_exp2f(-by) : 1.f;
       m += by;
-      limit = moves ? kSlack : limit;
+      limit = moves || seen ? kSlack - above : limit;
       l *= fix;
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[r] -= by;
@@ -580,7 +594,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   int p = find(begin, &at);
   int p1 = find(p + kTileKeys, &at1);
   int n = 0;  // the tile's number; its buffers are n & 1
-  float top = kUnseen;
   Raw raw = {};
   if (p < end) {
     // the first keys, values and second keys, all asked for at once
@@ -611,6 +624,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     constexpr int buf = decltype(buffer)::value;
     wait_vmem();
     lds_barrier();
+    const float scale = I8 ? lds.vs[buf][lane] : 0.f;
+    __builtin_amdgcn_sched_barrier(0);
     const int p2 = find(p1 + kTileKeys, &at2);
     if (p1 < end) load_v(at1, buf ^ 1, raw);
     if (p + kTileKeys > open) clean(buf, p);
@@ -619,7 +634,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     // scheduler must not move it.
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
-      rescale(top);
+      rescale(sub ? 0.f : scale);
       const f32x16 x = st;
       scores(0, 1);  // of half tile 1 here, or 0 of the next tile
       __builtin_amdgcn_sched_barrier(0);
@@ -663,11 +678,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     constexpr int buf = decltype(buffer)::value;
     wait_vmem();
     lds_barrier();
+    const float scale = I8 ? lds.vs[buf][lane] : 0.f;
+    __builtin_amdgcn_sched_barrier(0);
     const int p2 = find(p1 + kTileKeys, &at2);
     if (p1 < end) load_v(at1, buf ^ 1, raw);
     if (p2 < end) load_k(at2, buf, raw_k);
     if (p + kTileKeys > open) clean(buf, p);
-    rescale(top);
+    rescale(scale);
     const f32x16 x = st;
     __builtin_amdgcn_sched_barrier(0);
     if (!I8) read_k(buf ^ 1, mine);
@@ -707,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   if (kPairs) {  // the second pair's results, added to the first's (whose keys and values are read)
     float* const s_o = (float*)lds.k + (wave & 1) * (D / 2) * 64 + lane;
     float* const s_ml = (float*)lds.v + (wave & 1) * 128 + lane;
-    m = limit == kSlack ? m : kUnseen;
+    m = limit >= 0.f ? m : kUnseen;
     lds_barrier();
     if (wave >= 2) {
 #pragma unroll
@@ -722,7 +739,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     const float m2 = s_ml[0], both = fmaxf(m, m2);
     const float f = factor(m, both), f2 = factor(m2, both);
     m = both;
-    limit = m > kUnseen ? kSlack : limit;
+    limit = m > kUnseen ? 0.f : limit;
     l = l * f + s_ml[64] * f2;
 #pragma unroll
     for (int i = 0; i < kO; ++i) {
@@ -743,7 +760,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
         *(f32x4*)(part.o + to * D + i * 32 + 8 * (r >> 2) + 4 * half) =
             f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
     if (half == 0) {
-      part.ml[2 * to] = limit == kSlack ? m : kUnseen;
+      part.ml[2 * to] = limit >= 0.f ? m : kUnseen;
       part.ml[2 * to + 1] = l;
     }
     return;
@@ -820,7 +837,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   f32x4 o[kO];
 #pragma unroll
   for (int i = 0; i < kO; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = kUnseen, l = 0.f;
+  float m = kUnseen, l = 0.f, above = I8 ? 0.f : kSlack;
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
   const int krow = (col >> 2) * (KS / 4) + (col & 3);
@@ -944,10 +961,14 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, st[t][r]);
     top = max_xor32(max_xor16(top));
-    const bool moves = top > m + kSlack;
-    if (__any(moves)) {
-      const float fix = moves ? __builtin_amdgcn_exp2f(m - top) : 1.f;
-      m = moves ? top : m;
+    const bool moves = top > m + (kSlack - above);
+    const bool large = I8 && above == 0.f && x.vs > kLargeScale;
+    if (__any(moves || large)) {
+      const float up = I8 && __any(large) ? kSlack : 0.f;
+      above += up;
+      const float to = moves ? top + above : m + up;
+      const float fix = to > kUnseen ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+      m = to;
       l *= fix;
 #pragma unroll
       for (int i = 0; i < kO; ++i) o[i] *= fix;

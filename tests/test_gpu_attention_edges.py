@@ -101,6 +101,36 @@ def test_finite_scores_near_the_lowest_number(gpu_device, fmt, counts, lengths):
     check_attention(p, counts, q, attend(p, counts, q))
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("counts", FORMS)
+@pytest.mark.parametrize("power", [120, -120])
+def test_values_near_the_largest_and_smallest_numbers(gpu_device, fmt, counts, power):
+    """Values up to 2^120, whose weighted sum passes fp32's range if a weight is 2^7.5 and does not if weights
+    are 1 at most (74 x 2^120): the scores rise by 2^7.5 behind the first 64 tokens, or 256 (each wave of the
+    row form has then seen some).  And as small ones, which weights below 1 must not lose: 2^-120 leaves 2^-29
+    of it to fp32's smallest step, 2^-21 under a weight of 2^-8, far below the weight's rounding."""
+    announce(f"values of 2^{power} {fmt} rows {counts}")
+    g = generator(8)
+    base = signs(g, 2, 128)
+    for low in (64, 256):
+        length = low + 74
+        p = make_problem([length, length], heads=8, kv_heads=2, dim=128, fmt=fmt, page=64, seed=4)
+        for b in range(2):
+            k = torch.zeros(length, 2, 128, device=DEV)
+            k[low:] = 0.4609375 * base  # a score of 5.2 = 7.5 ln 2
+            v = torch.rand(length, 2, 128, generator=g, device=DEV)
+            v[:, :, ::2] *= signs(g, length, 2, 64)
+            store(p, b, k, v * 2.0 ** power)
+        q = base.repeat_interleave(4, dim=0).to(torch.bfloat16).expand(sum(counts), -1, -1).contiguous()
+        got = attend(p, counts, q)
+        if power < 0:
+            # held against values 2^120 times as large (a power of two: exact), so that the bound's share for
+            # values in the denormal range does not cover them
+            p.v = [v * 2.0 ** 120 for v in p.v]
+            got = got.double() * 2.0 ** 120
+        check_attention(p, counts, q, got)
+
+
 @pytest.mark.parametrize("counts", [None, [9, 40]])
 def test_64_bit_indexes_do_not_wrap(gpu_device, counts):
     """Integers of 64 bits that 32 bits do not hold are out of range, not what their lower half says."""
