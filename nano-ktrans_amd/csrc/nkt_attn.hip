@@ -114,8 +114,8 @@ constexpr float kUnseen = -__builtin_huge_valf();  // the running maximum before
 // kSlack - above.  bf16: above = kSlack, no weight is over 1, and a sum passes
 // fp32's range only if the values' own sum may.  int8 rounds weight x scale to bf16,
 // where weights of 2^-8 would cost the smallest scales their bits: above = 0
-// until a value's scale passes kLargeScale, then as bf16 (2^20 tokens x a weight
-// of 2^8 x 127 x kLargeScale are within the range).
+// until the row sees a value's scale past kLargeScale, then as bf16 (2^20 tokens x
+// a weight of 2^8 x 127 x kLargeScale are within the range).
 constexpr float kSlack = 8.0f;
 constexpr float kLargeScale = 0x1p90f;
 
@@ -322,7 +322,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   // Running maximum (log2), sum, and what a score less m must pass for m to move:
   // -infinity until the row has seen a token, then kSlack - above.
   float m = 0.f, l = 0.f, limit = -__builtin_huge_valf();
-  float above = I8 ? 0.f : kSlack;
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
 
@@ -472,14 +471,20 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     return max_xor32(fmaxf(top, st[15]));
   };
   float top = kUnseen;  // of the next half tile's scores, less m
-  // (scale: of the lane's token, int8, once per tile)
-  auto rescale = [&](float scale) {
+  // (int8: p is the tile's position, scale the value scale of the lane's token of it)
+  auto rescale = [&](int p, float scale) {
     const bool moves = top > limit;
-    const bool large = I8 && above == 0.f && scale > kLargeScale;
-    if (__any(moves || large)) {
-      const float up = I8 && __any(large) ? kSlack : 0.f;
-      above += up;
+    if (__any(moves || (I8 && scale > kLargeScale))) {
       const bool seen = limit >= 0.f;  // (nothing to rescale before)
+      float above = seen ? kSlack - limit : I8 ? 0.f : kSlack, up = 0.f;
+      if (I8) {
+        const uint64_t large = __ballot(scale > kLargeScale);
+        if (large) {
+          const uint64_t vis = p + kTileKeys > open ? visible<TREE>(a, s, my_token(), p) : ~0ull;
+          up = above == 0.f && (vis & large) ? kSlack : 0.f;
+          above += up;
+        }
+      }
       const float by = moves ? top + above : seen ? up : 0.f;
       const float fix = seen ? __builtin_amdgcn_exp2f(-by) : 1.f;
       m += by;
@@ -634,7 +639,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     // scheduler must not move it.
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
-      rescale(sub ? 0.f : scale);
+      rescale(p, scale);
       const f32x16 x = st;
       scores(0, 1);  // of half tile 1 here, or 0 of the next tile
       __builtin_amdgcn_sched_barrier(0);
@@ -684,7 +689,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     if (p1 < end) load_v(at1, buf ^ 1, raw);
     if (p2 < end) load_k(at2, buf, raw_k);
     if (p + kTileKeys > open) clean(buf, p);
-    rescale(scale);
+    rescale(p, scale);
     const f32x16 x = st;
     __builtin_amdgcn_sched_barrier(0);
     if (!I8) read_k(buf ^ 1, mine);
@@ -962,10 +967,13 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
       for (int r = 0; r < 4; ++r) top = fmaxf(top, st[t][r]);
     top = max_xor32(max_xor16(top));
     const bool moves = top > m + (kSlack - above);
-    const bool large = I8 && above == 0.f && x.vs > kLargeScale;
-    if (__any(moves || large)) {
-      const float up = I8 && __any(large) ? kSlack : 0.f;
-      above += up;
+    if (__any(moves || (I8 && x.vs > kLargeScale))) {
+      float up = 0.f;
+      if (I8) {
+        const uint64_t large = __ballot(x.vs > kLargeScale);
+        up = above == 0.f && ((masks ? bits : ~0ull) & large) ? kSlack : 0.f;
+        above += up;
+      }
       const float to = moves ? top + above : m + up;
       const float fix = to > kUnseen ? __builtin_amdgcn_exp2f(m - to) : 1.f;
       m = to;

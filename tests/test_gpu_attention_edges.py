@@ -131,6 +131,30 @@ def test_values_near_the_largest_and_smallest_numbers(gpu_device, fmt, counts, p
         check_attention(p, counts, q, got)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("counts", FORMS[1:])
+@pytest.mark.parametrize("lengths", [[80, 75], [700, 3000]])
+def test_large_values_reach_only_the_rows_that_see_them(gpu_device, fmt, counts, lengths):
+    """A finite value of 2^121 in a sequence's last token: the rows before the last keep their bits."""
+    announce(f"large unseen values {fmt} rows {counts} of {lengths}")
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=128, fmt=fmt, page=64, seed=9)
+    g = generator(10)
+    q = randn(g, sum(counts), 8, 128)
+    before = attend(p, counts, q)
+    for b, length in enumerate(lengths):
+        # (the last token alone: an int8 row that is stored once more may get another scale)
+        at = torch.arange(length, device=DEV)
+        slots = p.attn.slots(p.table, torch.full_like(at, b), at)
+        put(p.attn, slots[-1:], p.k[b][-1:].float(), 2.0 ** 121 * randn(g, 1, 2, 128).float())
+        p.k[b], p.v[b] = dense(p.attn, slots)
+    got = attend(p, counts, q)
+    check_attention(p, counts, q, got)
+    last = torch.tensor(split_rows(counts)[1:], device=DEV) - 1
+    others = torch.ones(sum(counts), dtype=torch.bool, device=DEV)
+    others[last] = False
+    assert torch.equal(got[others], before[others]) and not torch.equal(got[last], before[last])
+
+
 @pytest.mark.parametrize("counts", [None, [9, 40]])
 def test_64_bit_indexes_do_not_wrap(gpu_device, counts):
     """Integers of 64 bits that 32 bits do not hold are out of range, not what their lower half says."""
