@@ -4,10 +4,10 @@ import sys
 import pytest
 import torch
 
-from attn_cases import DEV, U, dense, generator, make_attention, make_problem, poison, randn, rotated
+from attn_cases import DEV, U, dense, generator, make_attention, make_problem, poison, put, randn, rotated
 from nano_ktrans_amd import rope_table
 from nano_ktrans_amd import _native as N
-from test_gpu_cache import check_stored
+from test_gpu_cache import check_stored, random_slots
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +116,77 @@ def test_keep_takes_64_bit_indexes_for_what_they_are(gpu_device):
                 index[20 + to] = 20 + src
             k, v = dense(p.attn, p.attn.slots(p.table, torch.full_like(at, b), at))
             assert torch.equal(k, p.k[b][index]) and torch.equal(v, p.v[b][index]), (which, b)
+
+
+SHAPES = [(32, 4, 128, 64), (16, 16, 128, 256), (14, 2, 64, 64), (5, 1, 64, 128), (1, 1, 128, 64), (6, 3, 128, 128),
+          (2, 1, 64, 64)]
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", SHAPES)
+@pytest.mark.parametrize("tokens,run,norm", [(1024, True, False), (1025, True, True), (1100, False, False), (1337, True, False)])
+def test_write_of_many_tokens(gpu_device, heads, kv_heads, dim, page, fmt, tokens, run, norm):
+    """On both sides of the size from which a launch takes wide windows and four heads at a time (whose number
+    need not be a multiple of four): runs of slots from an odd offset, broken by padding and by swapped tokens, and
+    scattered slots; a last window of any size."""
+    announce(f"write {heads}/{kv_heads}/{dim} page {page} {fmt} T={tokens} run={run} norm={norm}")
+    g = generator(tokens + heads)
+    attn = make_attention(heads, kv_heads, dim, fmt, page, 1536 // page + 1)
+    poison(attn)
+    qkv = randn(g, tokens, (heads + 2 * kv_heads) * dim)
+    q, k, v = (x.unflatten(1, (-1, dim)) for x in qkv.split([heads * dim, kv_heads * dim, kv_heads * dim], dim=1))
+    slots = (page - 5) + torch.arange(tokens, device=DEV) if run else random_slots(g, attn, tokens)
+    slots[[100, 101, 700]] = slots[[101, 100, 640]]
+    slots[[3, 640, tokens - 1]] = -1
+    slots[tokens - 2] = -7
+    rope = rope_table(131072, dim, 1e6, DEV)
+    positions = torch.randint(0, 131072, (tokens,), generator=g, device=DEV)
+    weights = {"q_norm": 1 + 0.1 * randn(g, dim), "k_norm": 1 + 0.1 * randn(g, dim)} if norm else {}
+    before = [x.clone() for x in (attn.k_cache, attn.v_cache)]
+    out = attn.write(q, k, v, positions, slots, rope, **weights)
+    assert not any(attn.status().values())
+    rows = rope[positions]
+    want, spread = rotated(q, weights.get("q_norm"), 1e-6, rows)
+    assert bool(((out.double() - want).abs() <= U * want.abs() + 2.0 ** -20 * spread * (1 + U)).all())
+    want, spread = rotated(k, weights.get("k_norm"), 1e-6, rows)
+    on = slots >= 0
+    check_stored(attn, slots[on], want[on], spread[on], v.double()[on])
+    every = torch.arange(attn.num_pages * page, device=DEV)
+    other = every[~torch.isin(every, slots[on])]
+    at, r, unit = torch.div(other, page, rounding_mode="floor"), other % page, attn.v_cache.shape[4]
+    as_int = torch.int16 if fmt == "bf16" else torch.int8
+    assert torch.equal(attn.k_cache[at, :, r].view(as_int), before[0][at, :, r].view(as_int))
+    vi = torch.div(r, unit, rounding_mode="floor"), r % unit
+    assert torch.equal(attn.v_cache[at, :, vi[0], :, vi[1]].view(as_int), before[1][at, :, vi[0], :, vi[1]].view(as_int))
+    # in place: the same bits; and in calls of a few tokens each: the same cache
+    held = [x.clone() for x in (attn.k_cache, attn.v_cache)]
+    q2 = q.contiguous()
+    assert torch.equal(attn.write(q2, k.contiguous(), v.contiguous(), positions, slots, rope, out=q2, **weights), out)
+    poison(attn)
+    for i in range(0, tokens, 333):
+        part = slice(i, i + 333)
+        few = attn.write(q[part], k[part], v[part], positions[part], slots[part], rope, **weights)
+        assert torch.equal(few, out[part])
+    for x, y in zip((attn.k_cache, attn.v_cache), held):
+        assert torch.equal(x.view(as_int), y.view(as_int))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", SHAPES)
+@pytest.mark.parametrize("n,run", [(1024, True), (1025, True), (1100, False), (1337, True)])
+def test_read_of_many_slots(gpu_device, heads, kv_heads, dim, page, fmt, n, run):
+    """On both sides of the size from which a launch takes wide windows: runs and scattered slots, repeated ones,
+    and negative ones (zeros)."""
+    announce(f"read {kv_heads}/{dim} page {page} {fmt} n={n} run={run}")
+    g = generator(n)
+    attn = make_attention(heads, kv_heads, dim, fmt, page, 1536 // page + 1)
+    total = attn.num_pages * page
+    put(attn, torch.arange(total, device=DEV), randn(g, total, kv_heads, dim).float(), randn(g, total, kv_heads, dim).float())
+    slots = (3 + torch.arange(n, device=DEV)) if run else random_slots(g, attn, n)
+    slots[[5, 700, n - 1]] = -1
+    slots[[9, 800]] = slots[[2, 12]]
+    want = dense(attn, slots.clamp(min=0))
+    for a, b in zip(attn.read(slots), want):
+        b = torch.where((slots >= 0).view(-1, 1, 1), b, 0.0)
+        assert torch.equal(a, b.to(torch.float32).to(torch.bfloat16))  # (as in the small calls' test)
+    assert not any(attn.status().values())
