@@ -230,8 +230,8 @@ __device__ __forceinline__ int end_of_rows(const Seq& s, int G, int r0, int coun
 // library product of 16384^3: 1.36), at a clock that falls to 1.8 of 2.4 GHz (557
 // on a card that holds less); matrix cores busy 51 % of it, the vector unit 47 %,
 // 5.3 vector instructions per matrix one, waves waiting 20 %, no bank conflict.
-// int8, three chunks of 1021 tokens on up to 9000, 32 / 8 heads: 398 us and 21
-// of join, 0.71 PFLOP/s; 31 % and 50 %, 10.7 vector instructions: widening the
+// int8, three chunks of up to 1021 tokens on up to 9000, 32 / 8 heads: 405 us and
+// 21 of join, 0.70 PFLOP/s; 31 % and 51 %, 10.9 vector instructions: widening the
 // codes and the two scales are what it has more.
 // ---------------------------------------------------------------------------
 template <int D, bool I8>
@@ -252,7 +252,7 @@ __device__ __forceinline__ int chunk_key(int r) {
 // first half of every tile's tokens, the other against the second, and their
 // results are added at the end: half the products and exponentials that 128
 // half-empty rows would cost.  64 drafts of up to 8 tokens on up to 8192, 32 / 4
-// heads, int8 116 us, as 128 rows 151; bf16 137 and 153.
+// heads, int8 117 us, as 128 rows 151; bf16 137 and 153.
 template <int D, bool I8, bool TREE, int ROWS>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int kQ = D / 16;       // Q fragments, and key products per half tile
@@ -799,7 +799,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 // Bound by HBM for batches: 16 x 16384 tokens, 32 / 8 heads, bf16 192 us, 5.6
 // TB/s; 64 sequences of up to 8192, 32 / 4 heads, int8 75 us, 4.7 TB/s (the
 // vector unit busy 28 %, the rest lost to sequences of unequal length).  One
-// sequence of 517 tokens takes 9 us: four workgroups, at about 57 GB/s each.
+// sequence of 517 tokens takes 9.1 us in four workgroups: 4.7 of launch, first
+// loads and the waves' sum, the rest reading at 61 GB/s each (the slope from 517
+// to 2000 tokens in one workgroup per key head; int8 46).
 // ---------------------------------------------------------------------------
 template <int D, bool I8, bool TREE>
 __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs a, Parts part) {
@@ -1100,7 +1102,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
 // each by SP x 16 threads: thread group i the splits i, i + SP, ... in order,
 // then the groups in order (the same sums whatever the batch).  A launch of its
 // own, so that no counter has to outlive a call: 4 us for few rows (latency), 21
-// for the chunks above (3063 tokens x 32 heads in three parts).
+// for the chunks above (2500 tokens x 32 heads in three parts).
 template <int D, bool TREE, int ROWS, int SP>
 __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Parts part, int row_blocks) {
   constexpr int kRows = 16 / SP, kN = D / 16;
@@ -1198,11 +1200,13 @@ Plan plan_of(const CacheView& c, int heads, int tokens, int seqs, int max_querie
   const int64_t wgs = (int64_t)p.part.items * c.kv_heads;
   int64_t splits = 1, least = 256, most = (int64_t)1 << 30;
   if (p.row_form) {
-    // One workgroup reads about 57 GB/s, 100 of them what HBM gives: fewer
-    // share the contexts (one request, bf16, D = 128, in us: 1000 tokens 8.9
-    // against 13.6, 2000 9.2 against 22), but under 640 tokens a second launch
-    // costs what the split gains (517 tokens: 8.3 for both launches, 9.0 for
-    // one).  More only split what would run on after the others: chunks of
+    // One workgroup reads about 61 GB/s, 100 of them what HBM gives: fewer
+    // share the contexts (one request, bf16, D = 128, in us: 800 tokens 8.5
+    // against 10.4, 1000 9.2 against 12.8, 2000 9.5 against 21.6).  Up to 640
+    // tokens they do not: both launches take 0.5 less there than the one (517
+    // tokens 8.6 against 9.1, 640 8.4 against 9.0; 257 8.3 against 6.9), but the
+    // second costs the host 4 in a call outside of a graph (14.8 against 10.7).
+    // More only split what would run on after the others: chunks of
     // 2048 against 4096 tokens, 32 x 4000 tokens 52 against 60; over two
     // rounds of workgroups chunks of 4096, the most that a wave holds page
     // numbers for.
@@ -1239,7 +1243,12 @@ size_t plan_rows(const CacheView& c, const Plan& p) {
 
 // Workgroups per item and head of the join, and its thread groups per row:
 // several for a row's splits while workgroups are few; most of many would find
-// nothing to do (a workgroup that does costs about 2 us).
+// nothing to do (a workgroup that does costs about 2 us).  Whole calls in us, the
+// row form with 4 and 16 groups: 4 splits (1000 tokens) 9.2 and 9.4 (of 16
+// sequences of 4000 28.3 and 29.0), 8 (2000) 9.9 and 9.7, 16 (4000) 10.2 and 9.5,
+// 32 (8000) 12.0 and 10.2.  The tile form with 4 and 1: 4 items x heads (a draft
+// of 12 on 2000) 13.7 and 23.9, 32 (8 of 8 on 4000) 24.6 and 32.4, 96 (24 of 8)
+// 43.0 and 43.2, 132 (a prompt of 512) 22.4 and 19.3, 252 (of 1000) 39.8 and 31.9.
 struct JoinPlan {
   int groups;
   int64_t row_blocks;
