@@ -61,7 +61,8 @@ extern "C" {
 #define NKT_ATTN_STATUS_BAD_PAGE 4u     /* a page outside the cache: its tokens are not seen, not moved */
 #define NKT_ATTN_STATUS_BAD_LENGTH 8u   /* a length past max_seq_len or the table (cut), negative (0), or a sequence
                                            with more than max_queries rows (the rest left as they were) */
-#define NKT_ATTN_STATUS_BAD_KEPT 16u    /* a kept index smaller than its place or past the table: not moved */
+#define NKT_ATTN_STATUS_BAD_KEPT 16u    /* a kept index smaller than its place or past the table, a
+                                           count past kept_width, a negative context: not moved */
 
 /* A handle for one layer shape: num_heads a multiple of num_kv_heads (query
  * head i reads key / value head i / (num_heads / num_kv_heads)), head_dim 64 or
@@ -106,7 +107,7 @@ int nkt_attn_read(void* handle, const int64_t* slots, int num_slots, void* k_out
  * position context[b] + kept[b, i] move to position context[b] + i, for i <
  * counts[b].  context int32 [num_seqs]: the tokens before the draft; kept int32
  * [num_seqs, kept_width], ascending in each row up to its count; counts int32
- * [num_seqs].  No two sequences may share a page that a draft reaches into. */
+ * [num_seqs] (0: padding, whose context may be anything).  No two sequences may share a page that a draft reaches into. */
 int nkt_attn_keep(void* handle, const int32_t* page_table, int table_width, const int32_t* context,
                   const int32_t* kept, int kept_width, const int32_t* counts, int num_seqs, void* stream, char* err,
                   size_t err_len);

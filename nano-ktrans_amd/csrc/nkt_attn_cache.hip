@@ -422,7 +422,7 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(CacheView c, const int32
   const int64_t most = (int64_t)width << c.page_shift;
   const int64_t base = context[b];
   int count = counts[b];
-  if (count > kept_width || base < 0) {
+  if (count > kept_width || (base < 0 && count > 0)) {  // (a sequence that keeps nothing may be padding)
     if (threadIdx.x == 0) report(c.status, kBadKept);
     count = base < 0 ? 0 : kept_width;
   }

@@ -190,3 +190,23 @@ def test_read_of_many_slots(gpu_device, heads, kv_heads, dim, page, fmt, n, run)
         b = torch.where((slots >= 0).view(-1, 1, 1), b, 0.0)
         assert torch.equal(a, b.to(torch.float32).to(torch.bfloat16))  # (as in the small calls' test)
     assert not any(attn.status().values())
+
+
+def test_keep_of_padding_sequences_is_no_error(gpu_device):
+    """A sequence that keeps nothing may have any context (a padded batch's length less its rows is negative); one
+    that keeps something of a negative context is reported and not moved."""
+    announce("keep: padding sequences")
+    p = make_problem([100, 100], heads=4, kv_heads=2, dim=64, fmt="bf16", page=64, seed=1, width=2)
+    kept = torch.tensor([[1, 3], [2, 5]], dtype=torch.int32, device=DEV)
+    for counts, bad in (([0, 2], False), ([1, 2], True)):
+        p.attn.keep(p.table, torch.tensor([-4, 20], device=DEV), kept, torch.tensor(counts, device=DEV))
+        assert p.attn.status() == {name: bad and name == "bad_kept" for name in N.ATTN_STATUS}
+        for b, m in enumerate(({}, {0: 2, 1: 5})):
+            at = torch.arange(100, device=DEV)
+            index = at.clone()
+            for to, src in m.items():
+                index[20 + to] = 20 + src
+            slots = p.attn.slots(p.table, torch.full_like(at, b), at)
+            k, v = dense(p.attn, slots)
+            assert torch.equal(k, p.k[b][index]) and torch.equal(v, p.v[b][index]), b
+            put(p.attn, slots, p.k[b].float(), p.v[b].float())
