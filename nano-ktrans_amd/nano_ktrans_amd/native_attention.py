@@ -27,8 +27,9 @@ from . import _native as N
 
 _FORMATS = {"bf16": N.CACHE_BF16, "int8": N.CACHE_INT8}
 
-# words of the status tensor: the kernels' (bits added atomically), one that says nothing, and ``slots``'s own
-_STATUS_KERNELS, _STATUS_SPARE, _STATUS_SLOTS = 0, 1, 2
+# words of the status tensor: the kernels' (bits added atomically), and two that ``slots`` writes: the first says
+# nothing, the second that a token's page was bad
+_STATUS_KERNELS, _STATUS_SLOTS = 0, 2
 
 # the current stream's handle without building a Stream object (2 us of a 12 us call)
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
@@ -122,6 +123,7 @@ class NativeAttention:
             self.k_scales = torch.zeros(num_pages, num_kv_heads, page_size, device=self.device)
             self.v_scales = torch.zeros_like(self.k_scales)
         self._status = torch.zeros(4, dtype=torch.int32, device=self.device)
+        self._slots_status = self._status[_STATUS_SLOTS - 1:_STATUS_SLOTS + 1]
         ptrs = (ctypes.c_void_p * N.ATTN_NUM_BUFS)()
         for i, t in enumerate((self.k_cache, self.v_cache, self.k_scales, self.v_scales, self._status)):
             ptrs[i] = t.data_ptr() if t is not None else None
@@ -217,15 +219,18 @@ class NativeAttention:
         past = self.num_pages * self.page_size
         if B == 0 or W == 0:
             return torch.where(positions < 0, -1, past)
+        # (each of these is a launch: ranges are told by what a clamp changes)
         at = torch.div(positions, self.page_size, rounding_mode="floor")
-        inside = (at < W) & (seqs >= 0) & (seqs < B)
-        pages = page_table[seqs.clamp(0, B - 1), at.clamp(0, W - 1)].long()
-        padding = positions < 0
-        bad = ((pages < 0) | (pages >= self.num_pages)) & inside & ~padding
+        seq, entry = seqs.clamp(0, B - 1), at.clamp(0, W - 1)
+        inside = (seq == seqs) & (entry == at)
+        pages = page_table[seq, entry]
+        if pages.dtype == torch.int64:
+            pages = pages.clamp(-1, self.num_pages)
+        slots = torch.add(positions % self.page_size, pages, alpha=self.page_size)
+        bad = inside & (slots != slots.clamp(0, past - 1))
         # (a word that only this call writes, and never reads: kernels on other streams add their bits to theirs)
-        self._status.index_fill_(0, _STATUS_SPARE + bad.any().view(1).long(), N.ATTN_STATUS["bad_page"])
-        slots = torch.where(inside, pages.clamp(-1, self.num_pages) * self.page_size + positions % self.page_size, past)
-        return slots.masked_fill(padding, -1)
+        self._slots_status.index_fill_(0, bad.view(-1).long(), N.ATTN_STATUS["bad_page"])
+        return torch.where(inside, slots, past).masked_fill(positions < 0, -1)
 
     def write(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
               rope: torch.Tensor, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
