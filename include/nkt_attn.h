@@ -87,8 +87,8 @@ int nkt_attn_bind_cache(void* handle, void* const* ptrs, char* err, size_t err_l
  *   (y1, y2) -> (y1 cos - y2 sin, y2 cos + y1 sin) on the two halves of a head,
  *   cos | sin = row positions[t] of rope fp32 [rope_rows, D];
  * in fp32 with one rounding, to bf16 for q_out [T, num_heads, D] (which may be
- * q itself if its tokens are dense) and to the cache's format for the keys; values are stored as they
- * are.  slots int64 [T]: where each token's key and value go; a negative slot
+ * q itself if its tokens are dense) and to the cache's format for the keys;
+ * values are stored as they are.  slots int64 [T]: where each token's key and value go; a negative slot
  * stores nothing (padding, whose position may be anything: outside the table
  * its queries are zero).  The slots of one call are distinct: what a slot
  * given twice holds is undefined. */
@@ -107,7 +107,8 @@ int nkt_attn_read(void* handle, const int64_t* slots, int num_slots, void* k_out
  * position context[b] + kept[b, i] move to position context[b] + i, for i <
  * counts[b].  context int32 [num_seqs]: the tokens before the draft; kept int32
  * [num_seqs, kept_width], ascending in each row up to its count; counts int32
- * [num_seqs] (0: padding, whose context may be anything).  No two sequences may share a page that a draft reaches into. */
+ * [num_seqs] (0: padding, whose context may be anything).  No two sequences may
+ * share a page that a draft reaches into. */
 int nkt_attn_keep(void* handle, const int32_t* page_table, int table_width, const int32_t* context,
                   const int32_t* kept, int kept_width, const int32_t* counts, int num_seqs, void* stream, char* err,
                   size_t err_len);

@@ -237,8 +237,9 @@ class NativeAttention:
               eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Queries and keys normalised per head (by ``q_norm`` / ``k_norm`` [head_dim], where given) and rotated
         by their positions' rows of ``rope`` (``rope_table``); keys and values stored at ``slots`` (negative:
-        not stored, padding, at any position), the queries returned [T, num_heads, head_dim].  q, k and v may be parts of one
-        projection's output.  The slots of one call have to be distinct."""
+        not stored, padding, at any position), the queries returned [T, num_heads, head_dim].  q, k and v may be
+        parts of one projection's output.  Norm weights of another type are rounded to bf16, the activations'.
+        The slots of one call have to be distinct."""
         q = self._strided(q, self.num_heads, "q")
         T = q.shape[0]
         k, v = self._strided(k, self.num_kv_heads, "k"), self._strided(v, self.num_kv_heads, "v")
