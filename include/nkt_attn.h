@@ -54,6 +54,9 @@ extern "C" {
 #define NKT_ATTN_BUF_STATUS 4 /* one uint32, zeroed by the caller */
 #define NKT_ATTN_NUM_BUFS 5
 
+/* most axes of positions (nkt_attn_write_axes) */
+#define NKT_ATTN_MAX_AXES 4
+
 /* bits of the status word */
 #define NKT_ATTN_STATUS_BAD_SLOT 1u     /* a slot past the cache: not stored, read as zeros */
 #define NKT_ATTN_STATUS_BAD_POSITION 2u /* a position outside the rotation table, of a token that is not padding:
@@ -96,6 +99,17 @@ int nkt_attn_write(void* handle, const void* q, int64_t q_stride, const void* k,
                    int64_t v_stride, const int64_t* positions, const int64_t* slots, const float* rope,
                    int64_t rope_rows, const void* q_norm, const void* k_norm, float eps, int num_tokens, void* q_out,
                    void* stream, char* err, size_t err_len);
+
+/* The same with positions on num_axes axes (time, height and width of images and
+ * video): positions int64 [num_axes, T], and frequency i of a head turns by the
+ * position on axis axis_of[i] (host memory, head_dim / 2 entries below num_axes):
+ * cosine i and sine i come from row positions[axis_of[i], t] of rope.  A token
+ * with a position outside the table on any axis counts as one whose position is. */
+int nkt_attn_write_axes(void* handle, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                        int64_t v_stride, const int64_t* positions, int num_axes, const uint8_t* axis_of,
+                        const int64_t* slots, const float* rope, int64_t rope_rows, const void* q_norm,
+                        const void* k_norm, float eps, int num_tokens, void* q_out, void* stream, char* err,
+                        size_t err_len);
 
 /* The cache read back: keys and values of num_slots slots (int64, in any order,
  * repeated ones too) to k_out and v_out, bf16 [num_slots, num_kv_heads, D].  A
@@ -143,6 +157,57 @@ int nkt_attn_forward_tree(void* handle, const void* q, const int64_t* tree_mask,
                           const int32_t* query_starts, int num_tokens, int num_seqs, int max_queries, int max_seq_len,
                           float scale, void* out, void* workspace, size_t workspace_bytes, void* stream, char* err,
                           size_t err_len);
+
+/* Workspace of nkt_attn_forward_weights. */
+int nkt_attn_weights_workspace_bytes(void* handle, int num_tokens, int num_seqs, int max_queries, int max_seq_len,
+                                     int last, size_t* bytes, char* err, size_t err_len);
+
+/* nkt_attn_forward, and what each cached token got of the attention: with p_rj the
+ * softmax that row r gives position j,
+ *   weights[b, h, j] += sum p_rj
+ * over the rows r of the last `last` (at least 1) of sequence b's rows and of the
+ * query heads that read key / value head h, in fp32 and in the same order at every
+ * call of the same sizes.  weights fp32 [num_seqs, num_kv_heads, weights_width],
+ * rows *_stride elements apart that do not overlap, weights_width >= max_seq_len:
+ * row b belongs to row b of the page table, position by position, also where
+ * sequences share pages.  Positions that no counted row sees keep what they had;
+ * a row that sees nothing adds nothing; one whose softmax is NaN (a NaN or infinite
+ * score) makes what it sees NaN.  out is nkt_attn_forward's up to the rounding of
+ * its rows' sums. */
+int nkt_attn_forward_weights(void* handle, const void* q, float* weights, int64_t seq_stride, int64_t head_stride,
+                             int weights_width, int last, const int32_t* page_table, int table_width,
+                             const int32_t* seq_lens, const int32_t* query_starts, int num_tokens, int num_seqs,
+                             int max_queries, int max_seq_len, float scale, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream, char* err, size_t err_len);
+
+/* Workspace of nkt_attn_evict. */
+int nkt_attn_evict_workspace_bytes(void* handle, int num_seqs, int max_seq_len, size_t* bytes, char* err,
+                                   size_t err_len);
+
+/* Eviction: of each sequence's len = seq_lens[b] tokens, keep = min(budgets[b],
+ * len) stay, per key / value head: the last min(recent, keep) ones, and of those
+ * before them the ones with the largest weights (of equal weights the earlier
+ * position; a NaN is below every number).  With front = keep - min(recent, keep):
+ *   a kept token before position front stays where it is;
+ *   the others before the recent ones go to the places before front that became
+ *   free, in order;
+ *   the recent ones go to positions front .. keep - 1, in order
+ * so the order of older tokens changes, which attention does not ask for: a key
+ * carries its rotation.  Each head's tokens move by themselves, in both caches and
+ * with their scales.  weights_out [num_seqs, num_kv_heads, weights_width] gets the
+ * kept tokens' weights at their new places and zeros behind them; it may be
+ * weights itself, with its strides.  lens_out int32 [num_seqs] (another array than
+ * seq_lens) gets keep.  max_seq_len bounds the lengths.  A sequence whose length
+ * is negative or past max_seq_len, the table or weights_width
+ * (NKT_ATTN_STATUS_BAD_LENGTH), or whose budget is negative
+ * (NKT_ATTN_STATUS_BAD_KEPT), is left as it is, its length and weights copied; a
+ * token on a page outside the cache is not moved.  No two sequences may share a
+ * page. */
+int nkt_attn_evict(void* handle, const int32_t* page_table, int table_width, const int32_t* seq_lens,
+                   const float* weights, int64_t seq_stride, int64_t head_stride, int weights_width,
+                   const int32_t* budgets, int recent, int num_seqs, int max_seq_len, float* weights_out,
+                   int64_t out_seq_stride, int64_t out_head_stride, int32_t* lens_out, void* workspace,
+                   size_t workspace_bytes, void* stream, char* err, size_t err_len);
 
 #ifdef __cplusplus
 }

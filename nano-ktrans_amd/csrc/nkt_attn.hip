@@ -5,57 +5,6 @@ namespace nkt {
 
 namespace {
 
-// ---------------------------------------------------------------------------
-// A sequence's rows are its n tokens x the G query heads that share a key /
-// value head, token by token (row r: token r / G, head r % G), so keys and
-// values are read once for all of them.
-// ---------------------------------------------------------------------------
-struct Seq {
-  int first;    // row of q of its first token
-  int n;        // tokens of it in this call
-  int len;      // positions of it in the cache
-  int context;  // position of its first token here (negative: more rows than tokens)
-};
-
-// What the sequence is made from, asked for together (b is the same in all
-// lanes): one round trip, and the caller's own loads may go beside it.
-struct SeqWords {
-  int start, next, len;
-};
-__device__ __forceinline__ SeqWords sequence_words(const AttnArgs& a, int b) {
-  const int32_t* at = a.starts ? a.starts + b : a.lens + b;
-  return {at[0], at[a.starts ? 1 : 0], a.lens[b]};
-}
-
-// (the result is held in scalar registers)
-__device__ __forceinline__ Seq sequence(const CacheView& c, const AttnArgs& a, int b, const SeqWords& w, bool reports) {
-  Seq s;
-  s.first = b;
-  s.n = 1;
-  bool bad = false;
-  if (a.starts) {
-    const int s0 = __builtin_amdgcn_readfirstlane(w.start);
-    const int s1 = __builtin_amdgcn_readfirstlane(w.next);
-    s.first = s0 < 0 ? 0 : s0 > a.tokens ? a.tokens : s0;
-    const int end = s1 > a.tokens ? a.tokens : s1;
-    s.n = end > s.first ? end - s.first : 0;
-    bad = s.n > a.max_queries;
-  }
-  const int len = __builtin_amdgcn_readfirstlane(w.len);
-  s.context = (len < 0 ? 0 : len) - s.n;
-  if (s.n > a.max_queries) s.n = a.max_queries;
-  const int64_t table = (int64_t)a.width << c.page_shift;
-  const int most = table < a.max_len ? (int)table : a.max_len;
-  s.len = len < 0 ? 0 : len > most ? most : len;
-  if (reports && (bad || len < 0 || len > most)) report(c.status, kBadLength);
-  return s;
-}
-
-// 64 entries of sequence b's page table from entry i on, one per lane
-__device__ __forceinline__ int table_entries(const AttnArgs& a, int b, int i, int lane) {
-  return i + lane < a.width ? a.table[(int64_t)b * a.width + i + lane] : -1;
-}
-
 // Positions p0 .. p0 + 63 that a token of the sequence sees, as bits.
 template <bool TREE>
 __device__ __forceinline__ uint64_t visible(const AttnArgs& a, const Seq& s, int token, int p0) {
@@ -86,15 +35,6 @@ __device__ __forceinline__ float add_pair(uint32_t w, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), ones, c, false);
 }
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-// 32x32x16 bf16: lane l supplies A[l%32][8*(l/32) .. +7] and B[8*(l/32) ..
-// +7][l%32]; D[(v&3) + 8*(v>>2) + 4*(l/32)][l%32] lands in register v.
-__device__ __forceinline__ f32x16 mfma32_bf16(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                 0);
-}
-
 __device__ __forceinline__ float max_xor32(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -105,7 +45,6 @@ __device__ __forceinline__ float max_xor16(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUnseen = -__builtin_huge_valf();  // the running maximum before any score
 // Weights may differ by this much (in log2) from what the row's largest score so
 // far gives, so that most tiles skip the rescale; neither the fp32 sums nor a bf16
@@ -125,24 +64,15 @@ __device__ __forceinline__ float factor(float m, float top) {
   return __builtin_amdgcn_exp2f(m - fmaxf(top, -__FLT_MAX__));
 }
 
-// A product that is rounded before the maximum is taken off it.  Contracted with
-// the subtraction it would keep bits that the maximum has lost: from 2^31 on, a
-// score less the maximum that it is itself could reach 2^7, its weight infinity.
-__device__ __forceinline__ float rounded_product(float a, float b) {
-#pragma clang fp contract(off)
-  return a * b;
+// What a row's weights are told from afterwards: exp2(score - maximum) / sum.
+__device__ __forceinline__ void keep_stats(const AttnArgs& a, int token, int head, float m, float l) {
+  float* to = a.stats + 2 * ((int64_t)token * a.heads + head);
+  to[0] = m;
+  to[1] = l;
 }
 
 __device__ __forceinline__ bool non_finite_pair(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-}
-
-// int8 codes of one 32-bit word -> two words of bf16 (exact)
-__device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t* lo, uint32_t* hi) {
-  const float f0 = (float)(int8_t)w, f1 = (float)(int8_t)(w >> 8), f2 = (float)(int8_t)(w >> 16),
-              f3 = (float)(int8_t)(w >> 24);
-  *lo = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u);
-  *hi = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u);
 }
 
 constexpr int kTileRows = 128, kTileKeys = 64;  // of the tile form
@@ -253,14 +183,17 @@ __device__ __forceinline__ int chunk_key(int r) {
 // results are added at the end: half the products and exponentials that 128
 // half-empty rows would cost.  64 drafts of up to 8 tokens on up to 8192, 32 / 4
 // heads, int8 117 us, as 128 rows 151; bf16 137 and 153.
-template <int D, bool I8, bool TREE, int ROWS>
+//
+// STATS: each row's maximum and sum go out as well (keep_stats), the sum of the weights
+// before they are rounded to bf16.
+template <int D, bool I8, bool TREE, int ROWS, bool STATS>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int kQ = D / 16;       // Q fragments, and key products per half tile
   constexpr int kO = D / 32;       // output tiles
   constexpr int kChunks = D / 8;   // 16-byte chunks of a key row
   constexpr int kLoads = kTileKeys * D * 2 / 4096;  // 16-byte loads per thread, keys or values
-  // value fragments read ahead, in 16 tokens (int8's staging needs the registers)
-  constexpr int kVAhead = I8 && D == 128 ? 1 : 2;
+  // value fragments read ahead, in 16 tokens (the registers go to int8's staging, to the unrounded sum)
+  constexpr int kVAhead = (I8 || (STATS && ROWS == kTileRows)) && D == 128 ? 1 : 2;
   constexpr bool kPairs = ROWS == kPairRows;
   __shared__ TileLds<D, I8> lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -506,7 +439,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         w[j] = __builtin_amdgcn_exp2f(x[q4 * 4 + j]);
-        if (I8) l += w[j];
+        if (I8 || STATS) l += w[j];
       }
       if (I8) {
         const f32x4 f = *(const f32x4*)(lds.vs[buf] + sub * 32 + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
@@ -515,7 +448,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       }
       pf[q4 >> 1][2 * (q4 & 1)] = pack_pair(w[0], w[1]);
       pf[q4 >> 1][2 * (q4 & 1) + 1] = pack_pair(w[2], w[3]);
-      if (!I8) l = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], l));
+      if (!I8 && !STATS) l = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], l));
     }
   };
   auto products = [&](int from, int to) {
@@ -534,7 +467,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       const bool odd = !(__builtin_fabsf(f) < __builtin_huge_valf());
       const uint64_t odds = __ballot(odd);
       if (odds == 0) return;
-      if (visible<TREE>(a, s, my_token(), p) & odds) l = __builtin_nanf("");
+      if (visible<TREE>(a, s, my_token(), p) & odds) {
+        if (!STATS) {
+          l = __builtin_nanf("");
+        } else {  // (the row's weights are numbers all the same)
+#pragma unroll
+          for (int i = 0; i < kO; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] = __builtin_nanf("");
+        }
+      }
       lds_barrier();  // every wave has read the scales
       if (wave == 0 && odd) lds.vs[buf][lane] = 0.f;
       lds_barrier();
@@ -772,6 +714,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   const int out_token = out_row / G;
+  if (STATS && half == 0)
+    keep_stats(a, s.first + out_token, h * G + out_row - out_token * G, limit >= 0.f ? m : kUnseen, l);
   uint16_t* out = a.out + ((int64_t)(s.first + out_token) * a.heads + h * G + (out_row - out_token * G)) * D;
 #pragma unroll
   for (int i = 0; i < kO; ++i)
@@ -803,7 +747,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
 // loads and the waves' sum, the rest reading at 61 GB/s each (the slope from 517
 // to 2000 tokens in one workgroup per key head; int8 46).
 // ---------------------------------------------------------------------------
-template <int D, bool I8, bool TREE>
+template <int D, bool I8, bool TREE, bool STATS>
 __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int KS = I8 ? 64 : 32;  // tokens per step
   constexpr int NT = KS / 16;       // key tiles per step
@@ -1092,6 +1036,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int tok = r / G;
+  if (STATS && d0 == 0) keep_stats(a, s.first + tok, h * G + r - tok * G, top, sum);
   uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r - tok * G)) * D + d0;
 #pragma unroll
   for (int d = 0; d < D / 16; d += 4)
@@ -1172,6 +1117,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
     if (sp == 0 && r < used) {
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       const int tok = (r0 + r) / G;
+      if (a.stats && d0 == 0) keep_stats(a, s.first + tok, h * G + r0 + r - tok * G, m, l);
       uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r0 + r - tok * G)) * D + d0;
 #pragma unroll
       for (int d = 0; d < kN; d += 4)
@@ -1281,14 +1227,14 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
   by_layout(c, [&](auto dim, auto int8) {
     constexpr int D = decltype(dim)::value;
     constexpr bool I8 = decltype(int8)::value;
-    auto launch = [&](auto tree) {
-      constexpr bool TREE = decltype(tree)::value;
+    auto launch = [&](auto tree, auto keeps) {
+      constexpr bool TREE = decltype(tree)::value, STATS = decltype(keeps)::value;
       if (p.row_form)
-        hipLaunchKernelGGL((attn_row_kernel<D, I8, TREE>), grid, dim3(256), 0, stream, c, a, p.part);
+        hipLaunchKernelGGL((attn_row_kernel<D, I8, TREE, STATS>), grid, dim3(256), 0, stream, c, a, p.part);
       else if (p.part.rows == kPairRows)
-        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE, kPairRows>), grid, dim3(256), 0, stream, c, a, p.part);
+        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE, kPairRows, STATS>), grid, dim3(256), 0, stream, c, a, p.part);
       else
-        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE, kTileRows>), grid, dim3(256), 0, stream, c, a, p.part);
+        hipLaunchKernelGGL((attn_tile_kernel<D, I8, TREE, kTileRows, STATS>), grid, dim3(256), 0, stream, c, a, p.part);
       if (p.part.splits == 1) return;
       const JoinPlan j = join_of(c, p);
       const dim3 join_grid((unsigned)(p.part.items * c.kv_heads * j.row_blocks));
@@ -1310,7 +1256,12 @@ hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, h
       else
         j.groups == 4 ? join(tile, four) : join(tile, one);
     };
-    a.tree ? launch(std::true_type{}) : launch(std::false_type{});
+    if (a.stats)  // (causal calls only)
+      launch(std::false_type{}, std::true_type{});
+    else if (a.tree)
+      launch(std::true_type{}, std::false_type{});
+    else
+      launch(std::false_type{}, std::false_type{});
   });
   return hipGetLastError();
 }

@@ -86,6 +86,17 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
          (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
 
+// Whether the rotation table has token t's position (on every axis).
+template <bool AXES>
+__device__ __forceinline__ bool inside(const WriteArgs& a, int t) {
+  bool ok = true;
+  for (int i = 0; i < (AXES ? a.num_axes : 1); ++i) {
+    const int64_t pos = a.positions[(int64_t)i * a.tokens + t];
+    ok = ok && pos >= 0 && pos < a.rope_rows;
+  }
+  return ok;
+}
+
 // ---------------------------------------------------------------------------
 // Write.  The first rope_blocks workgroups take the query and key rows: D / 8
 // lanes per row, four values from each half of the head, so that a rotation's
@@ -97,7 +108,11 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // Bound by HBM: 16384 tokens of 16 + 16 heads, D = 128, bf16 403 MB in 77 us, 5.2
 // TB/s; one token of 16 sequences, 32 / 4 heads, int8: 4.5 us, a launch's latency.
 // ---------------------------------------------------------------------------
-template <int D, bool I8, int HEADS, int W>
+//
+// AXES: the frequency of a pair of values has its position on one of several axes.
+// A lane's four frequencies take their cosines and sines from up to four rows of
+// the table.
+template <int D, bool I8, int HEADS, int W, bool AXES>
 __global__ __launch_bounds__(kThreads) void write_kernel(CacheView c, WriteArgs a, int rope_blocks) {
   constexpr int LR = D / 8;
   constexpr int kRows = kThreads / LR;
@@ -122,13 +137,24 @@ __global__ __launch_bounds__(kThreads) void write_kernel(CacheView c, WriteArgs 
       w1[j] = *(const u32x2*)(src + 4 * l);
       w2[j] = *(const u32x2*)(src + D / 2 + 4 * l);
     }
-    const int64_t pos = a.positions[t];
     const int64_t given = a.slots[t];
-    const bool pos_ok = pos >= 0 && pos < a.rope_rows;
+    const bool pos_ok = inside<AXES>(a, t);
     if (!pos_ok && given >= 0 && l == 0) report(c.status, kBadPosition);  // (padding may have any)
-    const float* rp = a.rope + (pos_ok ? pos : 0) * D;
-    const f32x4 cs = *(const f32x4*)(rp + 4 * l);
-    const f32x4 sn = *(const f32x4*)(rp + D / 2 + 4 * l);
+    f32x4 cs, sn;
+    if (!AXES) {
+      const float* rp = a.rope + (pos_ok ? a.positions[t] : 0) * D;
+      cs = *(const f32x4*)(rp + 4 * l);
+      sn = *(const f32x4*)(rp + D / 2 + 4 * l);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = 4 * l + i;
+        const int axis = (int)(a.axis_of[f >> 4] >> (2 * (f & 15))) & 3;
+        const float* rp = a.rope + (pos_ok ? a.positions[(int64_t)axis * a.tokens + t] : 0) * D + f;
+        cs[i] = rp[0];
+        sn[i] = rp[D / 2];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < HEADS; ++j) {
       const int h = h0 + j;
@@ -198,10 +224,7 @@ __global__ __launch_bounds__(kThreads) void write_kernel(CacheView c, WriteArgs 
   const int t0 = item / HK * W;
   if (tid < kLanes) {
     int64_t slot = -1;
-    if (tid < W && t0 + tid < a.tokens) {
-      const int64_t pos = a.positions[t0 + tid];
-      if (pos >= 0 && pos < a.rope_rows) slot = checked_slot(c, a.slots[t0 + tid]);
-    }
+    if (tid < W && t0 + tid < a.tokens && inside<AXES>(a, t0 + tid)) slot = checked_slot(c, a.slots[t0 + tid]);
     s_slot[tid] = slot;
   }
   __syncthreads();
@@ -502,21 +525,25 @@ hipError_t launch_cache_write(const CacheView& c, const WriteArgs& a, hipStream_
   by_layout(c, [&](auto dim, auto int8) {
     constexpr int D = decltype(dim)::value;
     constexpr bool I8 = decltype(int8)::value;
-    auto launch = [&](auto heads, auto window) {
+    auto launch = [&](auto heads, auto window, auto axes) {
       constexpr int HEADS = decltype(heads)::value, W = decltype(window)::value;
+      constexpr bool AXES = decltype(axes)::value;
       constexpr int kRows = kThreads / (D / 8);
       const int value_blocks = (a.tokens + W - 1) / W * c.kv_heads;
       const int sets = (a.heads + c.kv_heads + HEADS - 1) / HEADS;
       const int rope_blocks = (a.tokens * sets + kRows - 1) / kRows;
-      hipLaunchKernelGGL((write_kernel<D, I8, HEADS, W>), dim3(rope_blocks + value_blocks), dim3(kThreads), 0, stream,
-                         c, a, rope_blocks);
+      hipLaunchKernelGGL((write_kernel<D, I8, HEADS, W, AXES>), dim3(rope_blocks + value_blocks), dim3(kThreads), 0,
+                         stream, c, a, rope_blocks);
     };
     // Four heads per group where there are enough rows for it (16384 tokens,
     // 16 + 16 heads: 77 us bf16, 69 int8; one head per group 85 and 89).
+    auto by_axes = [&](auto heads, auto window) {
+      a.num_axes > 0 ? launch(heads, window, std::true_type{}) : launch(heads, window, std::false_type{});
+    };
     if (window_of(a.tokens) == 64)
-      launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 64>{});
+      by_axes(std::integral_constant<int, 4>{}, std::integral_constant<int, 64>{});
     else
-      launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+      by_axes(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
   });
   return hipGetLastError();
 }

@@ -75,10 +75,58 @@ bool check_sizes(const AttnHandle* h, int num_tokens, int num_seqs, int max_quer
   return true;
 }
 
+bool check_weigh_sizes(const AttnHandle* h, int num_seqs, int max_queries, int max_seq_len, int last, char* err,
+                       size_t len) {
+  if (last < 1) {
+    set_err(err, len, "last=%d: at least one token wanted", last);
+    return false;
+  }
+  if (weigh_workgroups(h->cache, h->heads, num_seqs, max_queries, max_seq_len, last) > kMaxGroups) {
+    set_err(err, len, "num_seqs=%d of up to max_seq_len=%d tokens: over 2^24 workgroups", num_seqs, max_seq_len);
+    return false;
+  }
+  return true;
+}
+
+// Rows of a [num_seqs, kv_heads, width] array that do not overlap, whichever of the first two is the inner one.
+bool check_rows(const char* name, int64_t seq_stride, int64_t head_stride, int64_t seqs, int64_t heads, int64_t width,
+                char* err, size_t len) {
+  const int64_t most = (int64_t)1 << 40;
+  const bool in_range = seq_stride >= 0 && head_stride >= 0 && seq_stride <= most && head_stride <= most;
+  const bool head_inner = (heads <= 1 || head_stride >= width) &&
+                          (seqs <= 1 || seq_stride >= (heads - 1) * head_stride + width);
+  const bool seq_inner = (seqs <= 1 || seq_stride >= width) &&
+                         (heads <= 1 || head_stride >= (seqs - 1) * seq_stride + width);
+  if (in_range && (head_inner || seq_inner)) return true;
+  set_err(err, len, "%s: strides %lld and %lld of %lld sequences and %lld heads, rows of %lld, overlap", name,
+          (long long)seq_stride, (long long)head_stride, (long long)seqs, (long long)heads, (long long)width);
+  return false;
+}
+
+bool check_evict_sizes(const AttnHandle* h, int num_seqs, int max_seq_len, char* err, size_t len) {
+  // (fill_kernel has up to 2048 workgroups more than sequences x heads)
+  if (num_seqs < 0 || (int64_t)num_seqs * h->cache.kv_heads > kMaxGroups / 4) {
+    set_err(err, len, "num_seqs=%d: negative, or over 2^22 of %d heads", num_seqs, h->cache.kv_heads);
+    return false;
+  }
+  if (max_seq_len < 0 || max_seq_len > kMaxTokens) {
+    set_err(err, len, "max_seq_len=%d: outside [0, 2^30]", max_seq_len);
+    return false;
+  }
+  return true;
+}
+
+// What a forward call adds to the weights of (nullptr: nothing).
+struct WeightsOut {
+  float* weights;
+  int64_t seq_stride, head_stride;
+  int last;
+};
+
 int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_words, const int32_t* page_table,
             int table_width, const int32_t* seq_lens, const int32_t* query_starts, int num_tokens, int num_seqs,
             int max_queries, int max_seq_len, float scale, void* out, void* workspace, size_t workspace_bytes,
-            void* stream, char* err, size_t len) {
+            void* stream, char* err, size_t len, const WeightsOut* weights = nullptr) {
   AttnHandle* h = bound_handle(handle, err, len);
   if (!query_starts) max_queries = 1;
   if (!h || !check_sizes(h, num_tokens, num_seqs, max_queries, max_seq_len, err, len)) return NKT_ATTN_ERR;
@@ -103,7 +151,13 @@ int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_word
     set_err(err, len, "q and out must be 16-byte aligned");
     return NKT_ATTN_ERR;
   }
-  const size_t need = attn_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len);
+  const size_t own = attn_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len);
+  size_t need = own;
+  if (weights) {
+    if (!check_weigh_sizes(h, num_seqs, max_queries, max_seq_len, weights->last, err, len)) return NKT_ATTN_ERR;
+    need += weigh_workspace_floats(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len, weights->last) *
+            sizeof(float);
+  }
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) {
     set_err(err, len, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_bytes);
     return NKT_ATTN_ERR;
@@ -123,7 +177,18 @@ int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_word
   a.max_queries = max_queries;
   a.max_len = max_seq_len;
   a.scale = scale;
+  float* more = (float*)((uint8_t*)workspace + own);
+  if (weights) a.stats = more;
   if (!check_hip(launch_attn(h->cache, a, workspace, (hipStream_t)stream), "attention kernel", err, len))
+    return NKT_ATTN_ERR;
+  if (!weights) return NKT_ATTN_OK;
+  WeighArgs w = {};
+  w.attn = a;
+  w.weights = weights->weights;
+  w.seq_stride = weights->seq_stride;
+  w.head_stride = weights->head_stride;
+  w.last = weights->last;
+  if (!check_hip(launch_weigh(h->cache, w, more, (hipStream_t)stream), "attention weights kernel", err, len))
     return NKT_ATTN_ERR;
   return NKT_ATTN_OK;
 }
@@ -214,10 +279,14 @@ int nkt_attn_bind_cache(void* handle, void* const* ptrs, char* err, size_t err_l
   return NKT_ATTN_OK;
 }
 
-int nkt_attn_write(void* handle, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
-                   int64_t v_stride, const int64_t* positions, const int64_t* slots, const float* rope,
-                   int64_t rope_rows, const void* q_norm, const void* k_norm, float eps, int num_tokens, void* q_out,
-                   void* stream, char* err, size_t err_len) {
+}  // extern "C"
+
+namespace {
+
+int write(void* handle, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+          int64_t v_stride, const int64_t* positions, int num_axes, const uint8_t* axis_of, const int64_t* slots,
+          const float* rope, int64_t rope_rows, const void* q_norm, const void* k_norm, float eps, int num_tokens,
+          void* q_out, void* stream, char* err, size_t err_len) {
   AttnHandle* h = bound_handle(handle, err, err_len);
   if (!h) return NKT_ATTN_ERR;
   if (num_tokens < 0 || (int64_t)num_tokens * (h->heads + 2 * h->cache.kv_heads) > kMaxRows) {
@@ -255,9 +324,48 @@ int nkt_attn_write(void* handle, const void* q, int64_t q_stride, const void* k,
   a.tokens = num_tokens;
   a.heads = h->heads;
   a.q_out = (uint16_t*)q_out;
+  a.num_axes = num_axes;
+  for (int i = 0; num_axes > 0 && i < h->cache.dim / 2; ++i) a.axis_of[i >> 4] |= (uint32_t)axis_of[i] << (2 * (i & 15));
   if (!check_hip(launch_cache_write(h->cache, a, (hipStream_t)stream), "cache write kernel", err, err_len))
     return NKT_ATTN_ERR;
   return NKT_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nkt_attn_write(void* handle, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                   int64_t v_stride, const int64_t* positions, const int64_t* slots, const float* rope,
+                   int64_t rope_rows, const void* q_norm, const void* k_norm, float eps, int num_tokens, void* q_out,
+                   void* stream, char* err, size_t err_len) {
+  return write(handle, q, q_stride, k, k_stride, v, v_stride, positions, 0, nullptr, slots, rope, rope_rows, q_norm,
+               k_norm, eps, num_tokens, q_out, stream, err, err_len);
+}
+
+int nkt_attn_write_axes(void* handle, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                        int64_t v_stride, const int64_t* positions, int num_axes, const uint8_t* axis_of,
+                        const int64_t* slots, const float* rope, int64_t rope_rows, const void* q_norm,
+                        const void* k_norm, float eps, int num_tokens, void* q_out, void* stream, char* err,
+                        size_t err_len) {
+  const AttnHandle* h = bound_handle(handle, err, err_len);
+  if (!h) return NKT_ATTN_ERR;
+  if (num_axes < 1 || num_axes > NKT_ATTN_MAX_AXES) {
+    set_err(err, err_len, "num_axes=%d outside [1, %d]", num_axes, NKT_ATTN_MAX_AXES);
+    return NKT_ATTN_ERR;
+  }
+  if (!axis_of) {
+    set_err(err, err_len, "null axis_of");
+    return NKT_ATTN_ERR;
+  }
+  for (int i = 0; i < h->cache.dim / 2; ++i) {
+    if (axis_of[i] >= num_axes) {
+      set_err(err, err_len, "axis_of[%d]=%d outside [0, %d)", i, axis_of[i], num_axes);
+      return NKT_ATTN_ERR;
+    }
+  }
+  return write(handle, q, q_stride, k, k_stride, v, v_stride, positions, num_axes, axis_of, slots, rope, rope_rows,
+               q_norm, k_norm, eps, num_tokens, q_out, stream, err, err_len);
 }
 
 int nkt_attn_read(void* handle, const int64_t* slots, int num_slots, void* k_out, void* v_out, void* stream, char* err,
@@ -336,6 +444,119 @@ int nkt_attn_forward_tree(void* handle, const void* q, const int64_t* tree_mask,
   }
   return forward(handle, q, tree_mask, mask_words, page_table, table_width, seq_lens, query_starts, num_tokens,
                  num_seqs, max_queries, max_seq_len, scale, out, workspace, workspace_bytes, stream, err, err_len);
+}
+
+int nkt_attn_weights_workspace_bytes(void* handle, int num_tokens, int num_seqs, int max_queries, int max_seq_len,
+                                     int last, size_t* bytes, char* err, size_t err_len) {
+  AttnHandle* h = (AttnHandle*)handle;
+  if (!h || !bytes) {
+    set_err(err, err_len, "null handle or output pointer");
+    return NKT_ATTN_ERR;
+  }
+  if (!check_sizes(h, num_tokens, num_seqs, max_queries, max_seq_len, err, err_len) ||
+      !check_weigh_sizes(h, num_seqs, max_queries, max_seq_len, last, err, err_len))
+    return NKT_ATTN_ERR;
+  *bytes = attn_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len) +
+           weigh_workspace_floats(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len, last) *
+               sizeof(float);
+  return NKT_ATTN_OK;
+}
+
+int nkt_attn_forward_weights(void* handle, const void* q, float* weights, int64_t seq_stride, int64_t head_stride,
+                             int weights_width, int last, const int32_t* page_table, int table_width,
+                             const int32_t* seq_lens, const int32_t* query_starts, int num_tokens, int num_seqs,
+                             int max_queries, int max_seq_len, float scale, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream, char* err, size_t err_len) {
+  const AttnHandle* h = bound_handle(handle, err, err_len);
+  if (!h) return NKT_ATTN_ERR;
+  if (!weights || !aligned(weights, 4)) {
+    set_err(err, err_len, "null weights, or not 4-byte aligned");
+    return NKT_ATTN_ERR;
+  }
+  if (max_seq_len > weights_width) {
+    set_err(err, err_len, "max_seq_len=%d past weights_width=%d", max_seq_len, weights_width);
+    return NKT_ATTN_ERR;
+  }
+  if (!check_rows("weights", seq_stride, head_stride, num_seqs, h->cache.kv_heads, weights_width, err, err_len))
+    return NKT_ATTN_ERR;
+  const WeightsOut w = {weights, seq_stride, head_stride, last};
+  return forward(handle, q, nullptr, 0, page_table, table_width, seq_lens, query_starts, num_tokens, num_seqs,
+                 max_queries, max_seq_len, scale, out, workspace, workspace_bytes, stream, err, err_len, &w);
+}
+
+int nkt_attn_evict_workspace_bytes(void* handle, int num_seqs, int max_seq_len, size_t* bytes, char* err,
+                                   size_t err_len) {
+  AttnHandle* h = (AttnHandle*)handle;
+  if (!h || !bytes) {
+    set_err(err, err_len, "null handle or output pointer");
+    return NKT_ATTN_ERR;
+  }
+  if (!check_evict_sizes(h, num_seqs, max_seq_len, err, err_len)) return NKT_ATTN_ERR;
+  *bytes = evict_workspace_bytes(h->cache, num_seqs, max_seq_len);
+  return NKT_ATTN_OK;
+}
+
+int nkt_attn_evict(void* handle, const int32_t* page_table, int table_width, const int32_t* seq_lens,
+                   const float* weights, int64_t seq_stride, int64_t head_stride, int weights_width,
+                   const int32_t* budgets, int recent, int num_seqs, int max_seq_len, float* weights_out,
+                   int64_t out_seq_stride, int64_t out_head_stride, int32_t* lens_out, void* workspace,
+                   size_t workspace_bytes, void* stream, char* err, size_t err_len) {
+  AttnHandle* h = bound_handle(handle, err, err_len);
+  if (!h || !check_evict_sizes(h, num_seqs, max_seq_len, err, err_len)) return NKT_ATTN_ERR;
+  if (table_width < 0 || ((int64_t)table_width << h->cache.page_shift) > kMaxTokens) {
+    set_err(err, err_len, "table_width=%d: outside [0, 2^30 tokens]", table_width);
+    return NKT_ATTN_ERR;
+  }
+  if (recent < 0 || weights_width < 0 || weights_width > kMaxTokens) {
+    set_err(err, err_len, "recent=%d, weights_width=%d: negative, or over 2^30", recent, weights_width);
+    return NKT_ATTN_ERR;
+  }
+  if (num_seqs == 0) return NKT_ATTN_OK;
+  if (!seq_lens || !weights || !budgets || !weights_out || !lens_out || (!page_table && table_width > 0)) {
+    set_err(err, err_len, "null page_table, seq_lens, weights, budgets, weights_out or lens_out");
+    return NKT_ATTN_ERR;
+  }
+  if (lens_out == seq_lens || lens_out == budgets) {
+    set_err(err, err_len, "lens_out must not be seq_lens or budgets");
+    return NKT_ATTN_ERR;
+  }
+  const int64_t heads = h->cache.kv_heads;
+  if (!check_rows("weights", seq_stride, head_stride, num_seqs, heads, weights_width, err, err_len) ||
+      !check_rows("weights_out", out_seq_stride, out_head_stride, num_seqs, heads, weights_width, err, err_len))
+    return NKT_ATTN_ERR;
+  // the rows of one are those of the other, or none of them lies in the other's span
+  auto span = [&](int64_t ss, int64_t hs) { return (num_seqs - 1) * ss + (heads - 1) * hs + weights_width; };
+  const bool same = weights == weights_out && seq_stride == out_seq_stride && head_stride == out_head_stride;
+  if (!same && weights < weights_out + span(out_seq_stride, out_head_stride) &&
+      weights_out < weights + span(seq_stride, head_stride)) {
+    set_err(err, err_len, "weights_out overlaps weights: pass the same array, or another one");
+    return NKT_ATTN_ERR;
+  }
+  const size_t need = evict_workspace_bytes(h->cache, num_seqs, max_seq_len);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) {
+    set_err(err, err_len, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_bytes);
+    return NKT_ATTN_ERR;
+  }
+  EvictArgs e = {};
+  e.table = page_table;
+  e.width = table_width;
+  e.seqs = num_seqs;
+  e.max_len = max_seq_len;
+  e.recent = recent;
+  e.lens = seq_lens;
+  e.budgets = budgets;
+  e.weights = weights;
+  e.out = weights_out;
+  e.seq_stride = seq_stride;
+  e.head_stride = head_stride;
+  e.out_seq_stride = out_seq_stride;
+  e.out_head_stride = out_head_stride;
+  e.weights_width = weights_width;
+  e.lens_out = lens_out;
+  e.moves = (int32_t*)workspace;
+  if (!check_hip(launch_evict(h->cache, e, (hipStream_t)stream), "cache evict kernel", err, err_len))
+    return NKT_ATTN_ERR;
+  return NKT_ATTN_OK;
 }
 
 }  // extern "C"

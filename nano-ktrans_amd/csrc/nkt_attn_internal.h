@@ -38,6 +38,9 @@ struct WriteArgs {
   float eps;
   int tokens, heads;
   uint16_t* q_out;
+  // several axes of positions: [num_axes, tokens], two bits for each frequency's axis
+  int num_axes;
+  uint32_t axis_of[4];
 };
 
 hipError_t launch_cache_write(const CacheView& c, const WriteArgs& a, hipStream_t stream);
@@ -59,11 +62,44 @@ struct AttnArgs {
   int tokens, seqs, heads;
   int max_queries, max_len;
   float scale;
+  float* stats;  // [tokens, heads, 2]: each row's maximum (log2) and sum of weights, or nullptr
 };
 
 // Workgroups of the call's largest launch.
 int64_t attn_workgroups(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len);
 size_t attn_workspace_bytes(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len);
 hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, hipStream_t stream);
+
+// What cached tokens got of a forward call's weights (which kept attn.stats, the
+// first tokens x heads x 2 floats of the workspace).
+struct WeighArgs {
+  AttnArgs attn;
+  float* weights;  // of sequence b, head h, position p at b seq_stride + h head_stride + p
+  int64_t seq_stride, head_stride;
+  int last;  // rows of a sequence's last so many tokens count
+  // set by the launch
+  int blocks, chunks, chunk_rows;
+  float* parts;  // [chunks, seqs, kv_heads, blocks of tokens]
+};
+int64_t weigh_workgroups(const CacheView& c, int heads, int seqs, int max_queries, int max_len, int last);
+size_t weigh_workspace_floats(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len,
+                              int last);
+hipError_t launch_weigh(const CacheView& c, WeighArgs w, float* workspace, hipStream_t stream);
+
+// Eviction: every pointer as in nkt_attn_evict.
+struct EvictArgs {
+  const int32_t* table;
+  int width, seqs, max_len, recent;
+  const int32_t* lens;
+  const int32_t* budgets;
+  const float* weights;
+  float* out;  // may be weights, with its strides
+  int64_t seq_stride, head_stride, out_seq_stride, out_head_stride;
+  int weights_width;
+  int32_t* lens_out;
+  int32_t* moves;  // workspace
+};
+size_t evict_workspace_bytes(const CacheView& c, int seqs, int max_len);
+hipError_t launch_evict(const CacheView& c, const EvictArgs& e, hipStream_t stream);
 
 }  // namespace nkt

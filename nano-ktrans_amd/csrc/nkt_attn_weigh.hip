@@ -1,0 +1,324 @@
+// What each cached token got of the attention's weights: the second pass over
+// the keys behind a forward call that kept its rows' maxima and sums.
+#include "nkt_attn_device.h"
+
+namespace nkt {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaveTokens = 64;
+constexpr int kBlockTokens = 4 * kWaveTokens;
+constexpr int kStepRows = 32;
+
+// Past this a row's maximum (log2) is told again (recount_kernel).  The attention
+// kernels move their running maximum by rounded steps, each off by 2^-24 of it at
+// most: up to 512 that is 2^-15, a factor of 2^-15 on the row's weights, which a
+// score of that size has from its own fp32 sum as well.  From 2^24 on it would be
+// whole powers of two.
+constexpr float kRecountFrom = 512.0f;
+
+__device__ __forceinline__ bool recounts(float m, float l) {
+  return !(__builtin_fabsf(m) < kRecountFrom) && !(l == 0.f);  // (NaN, infinity: told again, with the same end)
+}
+
+// A wave's operands.  The order of the dimensions within a product is free, so a
+// lane's fragments are the 16-byte pieces that it loads: bf16 fragment i holds
+// dimensions 16 i + 8 half on, int8 fragments 2 j and 2 j + 1 the piece at
+// 32 j + 16 half.
+template <int D, bool I8>
+__device__ __forceinline__ void load_query(const uint16_t* q, int half, u32x4* f) {
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+    f[i] = *(const u32x4*)(q + (I8 ? (i >> 1) * 32 + half * 16 + (i & 1) * 8 : i * 16 + half * 8));
+}
+// keys of 32 tokens, the lane's one `col`; at: place of the first one in the cache
+template <int D, bool I8>
+__device__ __forceinline__ void load_keys(const CacheView& c, int64_t at, int col, int half, u32x4* f) {
+  if (!I8) {
+    const uint16_t* src = (const uint16_t*)c.k + (at + col) * D + half * 8;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) f[i] = *(const u32x4*)(src + i * 16);
+  } else {
+    const uint8_t* src = c.k + (at + col) * D + half * 16;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const u32x4 w = *(const u32x4*)(src + j * 32);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        uint32_t lo, hi;
+        bf16_of_codes(w[x], &lo, &hi);
+        f[2 * j + (x >> 1)][2 * (x & 1)] = lo;
+        f[2 * j + (x >> 1)][2 * (x & 1) + 1] = hi;
+      }
+    }
+  }
+}
+// of token (v & 3) + 8 (v >> 2) + 4 half in register v: what its product is
+// multiplied by to give a score in log2
+template <bool I8>
+__device__ __forceinline__ f32x16 score_factors(const CacheView& c, int64_t at, int half, float scale2) {
+  f32x16 f;
+#pragma unroll
+  for (int v = 0; v < 16; v += 4) {
+    f32x4 x = {scale2, scale2, scale2, scale2};
+    if (I8) x = *(const f32x4*)(c.k_scales + at + 8 * (v >> 2) + 4 * half) * scale2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[v + j] = x[j];
+  }
+  return f;
+}
+template <int D>
+__device__ __forceinline__ f32x16 products(const u32x4* k, const u32x4* q) {
+  f32x16 st;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) st[v] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) st = mfma32_bf16(k[i], q[i], st);
+  return st;
+}
+
+// The page of position p as a place in the cache (tokens of all heads' blocks), -1: none.
+__device__ __forceinline__ int64_t place_of(const CacheView& c, const AttnArgs& a, int b, int h, int p) {
+  const int entry = p >> c.page_shift;
+  const int page = entry < a.width ? __builtin_amdgcn_readfirstlane(a.table[(int64_t)b * a.width + entry]) : -1;
+  if (page < 0 || page >= c.num_pages) return -1;
+  return (((int64_t)page * c.kv_heads + h) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
+}
+
+// ---------------------------------------------------------------------------
+// Maxima and sums of the rows whose maximum is past kRecountFrom, from rounded
+// scores as weigh_kernel takes them: one workgroup per 32 rows of a head, its
+// waves taking 32 tokens in turn.  Without such rows (all but broken or extreme
+// inputs) it ends after reading the statistics.
+// ---------------------------------------------------------------------------
+template <int D, bool I8>
+__global__ __launch_bounds__(kThreads) void recount_kernel(CacheView c, WeighArgs w, int row_blocks) {
+  const AttnArgs& a = w.attn;
+  __shared__ float s_m[4][2][32], s_l[4][2][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int half = lane >> 5, col = lane & 31;
+  const int HK = c.kv_heads, G = a.heads / HK;
+  const int h = (int)(blockIdx.x % (unsigned)HK);
+  const int rest = (int)(blockIdx.x / (unsigned)HK);
+  const int b = rest / row_blocks;
+  const Seq s = sequence(c, a, b, sequence_words(a, b), false);
+  const int first = s.n > w.last ? s.n - w.last : 0;
+  const int rows = (s.n - first) * G;
+  const int r0 = rest % row_blocks * kStepRows;
+  if (r0 >= rows) return;
+  const int row = r0 + col < rows ? r0 + col : rows - 1;
+  const int token = first + row / G;
+  const int64_t at_row = (int64_t)(s.first + token) * a.heads + h * G + row % G;
+  float* stats = a.stats + 2 * at_row;
+  const bool again = recounts(stats[0], stats[1]);
+  if (!__any(again)) return;  // (the same in all waves)
+  u32x4 q[D / 16];
+  load_query<D, I8>(a.q + at_row * D, half, q);
+  const float scale2 = a.scale * kLog2e;
+  const int past = s.context + token;  // the last position that the row sees
+  const int last_row = r0 + kStepRows - 1 < rows ? r0 + kStepRows - 1 : rows - 1;
+  const int row_end = s.context + first + last_row / G + 1;
+  const int end = row_end < s.len ? row_end : s.len;
+  float m = -__builtin_huge_valf(), l = 0.f;
+  for (int p = wave * 32; p < end; p += 128) {
+    const int64_t at = place_of(c, a, b, h, p);
+    if (at < 0) continue;
+    u32x4 k[D / 16];
+    load_keys<D, I8>(c, at, col, half, k);
+    const f32x16 f = score_factors<I8>(c, at, half, scale2);
+    f32x16 st = products<D>(k, q);
+    float top = m;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int pos = p + (v & 3) + 8 * (v >> 2) + 4 * half;
+      st[v] = pos <= past && pos < s.len ? rounded_product(st[v], f[v]) : -__builtin_huge_valf();
+      top = fmaxf(top, st[v]);
+    }
+    const float less = fmaxf(top, -__FLT_MAX__);
+    l *= __builtin_amdgcn_exp2f(m - less);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) l += __builtin_amdgcn_exp2f(st[v] - less);
+    m = top;
+  }
+  s_m[wave][half][col] = m;
+  s_l[wave][half][col] = l;
+  __syncthreads();
+  if (tid >= 32 || r0 + col >= rows || !again) return;
+  m = s_m[0][0][col];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, s_m[i >> 1][i & 1][col]);
+  l = 0.f;
+  const float less = fmaxf(m, -__FLT_MAX__);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) l += s_l[i >> 1][i & 1][col] * __builtin_amdgcn_exp2f(s_m[i >> 1][i & 1][col] - less);
+  stats[0] = m;
+  stats[1] = l;
+}
+
+// ---------------------------------------------------------------------------
+// Weights of 64 tokens per wave, 256 per workgroup, summed over a part of the
+// rows that see them.  S = K . Q^T on 32x32x16 matrix instructions with the keys
+// held in registers: a lane's column is a row and its registers are tokens, so
+// that the sum over rows stays in the lane until the end, and the row's maximum
+// and sum are one value per lane.
+// ---------------------------------------------------------------------------
+template <int D, bool I8>
+__global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighArgs w) {
+  const AttnArgs& a = w.attn;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int half = lane >> 5, col = lane & 31;
+  const int HK = c.kv_heads, G = a.heads / HK;
+  const int h = (int)(blockIdx.x % (unsigned)HK);
+  int rest = (int)(blockIdx.x / (unsigned)HK);
+  const int block = rest % w.blocks;
+  rest /= w.blocks;
+  const int chunk = rest % w.chunks;
+  const int b = rest / w.chunks;
+  const Seq s = sequence(c, a, b, sequence_words(a, b), false);
+  const int p = block * kBlockTokens + wave * kWaveTokens;
+  if (p >= s.len) return;
+  const int64_t at = place_of(c, a, b, h, p);
+  // rows: the last tokens' ones, from the first that sees position p
+  const int first = s.n > w.last ? s.n - w.last : 0;
+  const int rows = (s.n - first) * G;
+  const int end = rows < (chunk + 1) * w.chunk_rows ? rows : (chunk + 1) * w.chunk_rows;
+  const int sees = p - s.context - first;  // the first token (of those counted) that sees p
+  int r = chunk * w.chunk_rows;
+  if (sees > 0 && (int64_t)sees * G > r) r = (int64_t)sees * G < end ? sees * G : end;
+
+  f32x16 acc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[i][v] = 0.f;
+  if (at >= 0 && r < end) {
+    u32x4 k[2][D / 16];
+    f32x16 f[2];
+    const float scale2 = a.scale * kLog2e;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load_keys<D, I8>(c, at + 32 * i, col, half, k[i]);
+      f[i] = score_factors<I8>(c, at + 32 * i, half, scale2);
+    }
+    for (; r < end; r += kStepRows) {
+      const int row = r + col < end ? r + col : end - 1;
+      const int token = first + row / G;
+      const int64_t at_row = (int64_t)(s.first + token) * a.heads + h * G + row % G;
+      u32x4 q[D / 16];
+      load_query<D, I8>(a.q + at_row * D, half, q);
+      const float m = a.stats[2 * at_row], l = a.stats[2 * at_row + 1];
+      const bool counts = r + col < end && l != 0.f;  // (a row that saw nothing has a sum of 0)
+      const int past = counts ? s.context + token : -1;
+      const float inv = 1.0f / l;
+      const bool masks = __any(past < p + kWaveTokens - 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x16 st = products<D>(k[i], q);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float x = __builtin_amdgcn_exp2f(rounded_product(st[v], f[i][v]) - m);
+          const bool seen = !masks || p + 32 * i + (v & 3) + 8 * (v >> 2) + 4 * half <= past;
+          acc[i][v] = seen ? __builtin_fmaf(x, inv, acc[i][v]) : acc[i][v];
+        }
+      }
+    }
+  }
+  // the sum over the 32 columns, register by register of the lane's number: lanes
+  // that differ in one bit of it exchange the half that they do not keep
+  float x[32];
+#pragma unroll
+  for (int v = 0; v < 32; ++v) x[v] = acc[v >> 4][v & 15];
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    const bool high = col & off;
+#pragma unroll
+    for (int v = 0; v < off; ++v) {
+      const float give = high ? x[v] : x[v + off], keep = high ? x[v + off] : x[v];
+      x[v] = keep + __shfl_xor(give, off);
+    }
+  }
+  const int pos = p + (col >> 4) * 32 + (col & 3) + 8 * ((col & 15) >> 2) + 4 * half;
+  if (pos >= s.len) return;
+  if (w.chunks > 1) {
+    w.parts[(((int64_t)chunk * a.seqs + b) * HK + h) * ((int64_t)w.blocks * kBlockTokens) + pos] = x[0];
+  } else if (at >= 0) {
+    w.weights[b * w.seq_stride + h * w.head_stride + pos] += x[0];
+  }
+}
+
+// Adds the parts of the rows to the weights, in order.
+__global__ __launch_bounds__(kThreads) void weigh_join_kernel(CacheView c, WeighArgs w) {
+  const AttnArgs& a = w.attn;
+  const int HK = c.kv_heads;
+  const int h = (int)(blockIdx.x % (unsigned)HK);
+  const int rest = (int)(blockIdx.x / (unsigned)HK);
+  const int b = rest / w.blocks;
+  const int pos = rest % w.blocks * kBlockTokens + (int)threadIdx.x;
+  const Seq s = sequence(c, a, b, sequence_words(a, b), false);
+  if (pos >= s.len) return;
+  const int64_t row = (int64_t)w.blocks * kBlockTokens;
+  float sum = 0.f;
+  for (int i = 0; i < w.chunks; ++i) sum += w.parts[(((int64_t)i * a.seqs + b) * HK + h) * row + pos];
+  w.weights[b * w.seq_stride + h * w.head_stride + pos] += sum;
+}
+
+struct WeighPlan {
+  int blocks, chunks, chunk_rows, row_blocks;
+};
+
+WeighPlan weigh_plan(const CacheView& c, int heads, int seqs, int max_queries, int max_len, int last) {
+  WeighPlan p = {};
+  const int64_t rows = (int64_t)(last < max_queries ? last : max_queries) * (heads / c.kv_heads);
+  p.blocks = (max_len + kBlockTokens - 1) / kBlockTokens;
+  p.row_blocks = (int)((rows + kStepRows - 1) / kStepRows);
+  const int64_t wgs = (int64_t)seqs * c.kv_heads * p.blocks;
+  int64_t chunks = wgs > 0 ? (2048 + wgs - 1) / wgs : 1;
+  const int64_t most = (rows + 255) / 256;
+  if (chunks > most) chunks = most;
+  if (chunks < 1) chunks = 1;
+  const int64_t chunk_rows = ((rows + chunks - 1) / chunks + kStepRows - 1) / kStepRows * kStepRows;
+  p.chunk_rows = (int)(chunk_rows > 0 ? chunk_rows : kStepRows);
+  p.chunks = rows > 0 ? (int)((rows + p.chunk_rows - 1) / p.chunk_rows) : 1;
+  return p;
+}
+
+size_t parts_of(const CacheView& c, const WeighPlan& p, int seqs) {
+  return p.chunks > 1 ? (size_t)p.chunks * seqs * c.kv_heads * p.blocks * kBlockTokens : 0;
+}
+
+}  // namespace
+
+int64_t weigh_workgroups(const CacheView& c, int heads, int seqs, int max_queries, int max_len, int last) {
+  const WeighPlan p = weigh_plan(c, heads, seqs, max_queries, max_len, last);
+  const int64_t weigh = (int64_t)p.blocks * p.chunks;
+  return (int64_t)seqs * c.kv_heads * (weigh > p.row_blocks ? weigh : p.row_blocks);
+}
+
+size_t weigh_workspace_floats(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len,
+                              int last) {
+  return (size_t)tokens * heads * 2 +
+         parts_of(c, weigh_plan(c, heads, seqs, max_queries, max_len, last), seqs);
+}
+
+hipError_t launch_weigh(const CacheView& c, WeighArgs w, float* workspace, hipStream_t stream) {
+  const AttnArgs& a = w.attn;
+  const WeighPlan p = weigh_plan(c, a.heads, a.seqs, a.max_queries, a.max_len, w.last);
+  if (p.blocks == 0 || p.row_blocks == 0) return hipSuccess;
+  w.blocks = p.blocks;
+  w.chunks = p.chunks;
+  w.chunk_rows = p.chunk_rows;
+  w.parts = workspace + (size_t)a.tokens * a.heads * 2;
+  const unsigned pairs = (unsigned)a.seqs * c.kv_heads;
+  by_layout(c, [&](auto dim, auto int8) {
+    constexpr int D = decltype(dim)::value;
+    constexpr bool I8 = decltype(int8)::value;
+    hipLaunchKernelGGL((recount_kernel<D, I8>), dim3(pairs * p.row_blocks), dim3(kThreads), 0, stream, c, w,
+                       p.row_blocks);
+    hipLaunchKernelGGL((weigh_kernel<D, I8>), dim3(pairs * p.blocks * p.chunks), dim3(kThreads), 0, stream, c, w);
+  });
+  if (p.chunks > 1) hipLaunchKernelGGL(weigh_join_kernel, dim3(pairs * p.blocks), dim3(kThreads), 0, stream, c, w);
+  return hipGetLastError();
+}
+
+}  // namespace nkt

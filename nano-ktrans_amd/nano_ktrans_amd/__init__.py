@@ -16,7 +16,7 @@ from .kernels.weight_loader import ExpertWeightLoader, GPTQLinearWeight
 from .layers.attention_block import AttentionBatch, FusedAttentionBlock, FusedDecoderLayer
 from .layers.expert_mlp import PackedSparseExpertMLP, SparseExpertMLP, build_expert_module, load_expert_weights
 from .layers.hybrid_moe import HybridMoE
-from .native_attention import NativeAttention, rope_table, tree_mask_from_parents
+from .native_attention import NativeAttention, media_positions, rope_axes, rope_table, tree_mask_from_parents
 from .native_moe import NativeMoE
 
 __all__ = [
@@ -32,10 +32,12 @@ __all__ = [
     "SparseExpertMLP",
     "build_expert_module",
     "load_expert_weights",
+    "media_positions",
     "pack_int4_matrix",
     "pack_int8_matrix",
     "quantize_symmetric_int8_per_channel",
     "quantize_symmetric_w4a32",
+    "rope_axes",
     "rope_table",
     "tree_mask_from_parents",
 ]

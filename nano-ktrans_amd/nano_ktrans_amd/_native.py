@@ -100,6 +100,8 @@ ATTN_BUF_V_SCALES = 3
 ATTN_BUF_STATUS = 4
 ATTN_NUM_BUFS = 5
 
+ATTN_MAX_AXES = 4
+
 ATTN_STATUS = {
     "bad_slot": 1,
     "bad_position": 2,
@@ -114,11 +116,16 @@ ATTN_SYMBOLS = (
     "nkt_attn_cache_bytes",
     "nkt_attn_bind_cache",
     "nkt_attn_write",
+    "nkt_attn_write_axes",
     "nkt_attn_read",
     "nkt_attn_keep",
     "nkt_attn_workspace_bytes",
     "nkt_attn_forward",
     "nkt_attn_forward_tree",
+    "nkt_attn_weights_workspace_bytes",
+    "nkt_attn_forward_weights",
+    "nkt_attn_evict_workspace_bytes",
+    "nkt_attn_evict",
 )
 
 # bytes of the static scratch behind nkt_moe_forward_noalloc (NKT_NOALLOC_SCRATCH_BYTES)
@@ -205,11 +212,16 @@ def _declare_attention(L: ctypes.CDLL) -> None:
     L.nkt_attn_cache_bytes.argtypes = [vp, i, szp, cp, sz]
     L.nkt_attn_bind_cache.argtypes = [vp, ctypes.POINTER(vp), cp, sz]
     L.nkt_attn_write.argtypes = [vp, vp, l, vp, l, vp, l, vp, vp, vp, l, vp, vp, f, i, vp, vp, cp, sz]
+    L.nkt_attn_write_axes.argtypes = [vp, vp, l, vp, l, vp, l, vp, i, cp, vp, vp, l, vp, vp, f, i, vp, vp, cp, sz]
     L.nkt_attn_read.argtypes = [vp, vp, i, vp, vp, vp, cp, sz]
     L.nkt_attn_keep.argtypes = [vp, vp, i, vp, vp, i, vp, i, vp, cp, sz]
     L.nkt_attn_workspace_bytes.argtypes = [vp, i, i, i, i, szp, cp, sz]
     L.nkt_attn_forward.argtypes = [vp, vp, vp, i, vp, vp, i, i, i, i, f, vp, vp, sz, vp, cp, sz]
     L.nkt_attn_forward_tree.argtypes = [vp, vp, vp, i, vp, i, vp, vp, i, i, i, i, f, vp, vp, sz, vp, cp, sz]
+    L.nkt_attn_weights_workspace_bytes.argtypes = [vp, i, i, i, i, i, szp, cp, sz]
+    L.nkt_attn_forward_weights.argtypes = [vp, vp, vp, l, l, i, i, vp, i, vp, vp, i, i, i, i, f, vp, vp, sz, vp, cp, sz]
+    L.nkt_attn_evict_workspace_bytes.argtypes = [vp, i, i, szp, cp, sz]
+    L.nkt_attn_evict.argtypes = [vp, vp, i, vp, vp, l, l, i, vp, i, i, i, vp, l, l, vp, vp, sz, vp, cp, sz]
     for name in ATTN_SYMBOLS[2:]:
         getattr(L, name).restype = i
 

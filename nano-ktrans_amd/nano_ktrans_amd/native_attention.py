@@ -15,11 +15,17 @@ sequences' lengths, and where its new tokens go:
     out = attn.forward(q, page_table, seq_lens, query_starts, max_queries=...)    # prompts, chunks
     out = attn.forward_tree(q, tree_mask, page_table, seq_lens, query_starts)     # drafted tokens
     attn.keep(page_table, context_lens, kept, counts)                             # the accepted ones
+
+and, for caches that keep only the tokens that attention weighs most, an fp32 tensor [sequences, kv_heads, positions]
+per layer:
+
+    out = attn.forward_weights(q, weights, page_table, seq_lens)                  # adds to weights
+    seq_lens, weights = attn.evict(page_table, seq_lens, weights, budget, recent)
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -60,6 +66,47 @@ def tree_mask_from_parents(parents: Sequence[Sequence[int]], device=None) -> tor
         rows += [[(bits >> (64 * w) & (1 << 64) - 1) for w in range(words)] for bits in sees]
     signed = [[w - (1 << 64) if w >> 63 else w for w in row] for row in rows]
     return torch.tensor(signed, dtype=torch.int64).reshape(-1, words).to(device if device is not None else "cpu")
+
+
+def rope_axes(sections: Sequence[int], interleaved: bool = False) -> List[int]:
+    """The axis of each frequency, for ``NativeAttention.write(axes=...)``: sections[a] of the head_dim / 2
+    frequencies turn by axis a (time, height, width), the highest frequencies those of axis 0, then axis 1, ...;
+    where ``interleaved``, dealt out to the axes in turn as long as they have any left."""
+    if not sections or any(n < 0 for n in sections):
+        raise ValueError(f"sections must be numbers of frequencies, got {list(sections)}")
+    if not interleaved:
+        return [axis for axis, n in enumerate(sections) for _ in range(n)]
+    left, out = list(sections), []
+    while any(left):
+        for axis, n in enumerate(left):
+            if n:
+                left[axis] -= 1
+                out.append(axis)
+    return out
+
+
+def media_positions(segments: Sequence[Union[int, Sequence[int]]], start: int = 0,
+                    device=None) -> Tuple[torch.Tensor, int]:
+    """Positions int64 [3, tokens] on the axes time, height and width of a prompt made of text (a number of tokens)
+    and media (t, h, w patches, in this order of nesting), and the next free position: text counts on, the same
+    number on all axes; a medium lies at the next number plus its patches' indexes, and what follows it goes on
+    behind the largest number it has."""
+    spans, at = [], start
+    for segment in segments:
+        if isinstance(segment, int):
+            if segment < 0:
+                raise ValueError(f"a segment of {segment} tokens")
+            spans.append((at + torch.arange(segment)).expand(3, -1))
+            at += segment
+            continue
+        t, h, w = segment
+        if min(t, h, w) < 0:
+            raise ValueError(f"a medium of {t} x {h} x {w} patches")
+        grid = torch.stack(torch.meshgrid(torch.arange(t), torch.arange(h), torch.arange(w), indexing="ij"))
+        spans.append(at + grid.reshape(3, -1))
+        at += max(t, h, w) if min(t, h, w) else 0
+    out = torch.cat(spans, dim=1) if spans else torch.zeros(3, 0, dtype=torch.int64)
+    return out.to(device if device is not None else "cpu"), at
 
 
 class NativeAttention:
@@ -110,7 +157,7 @@ class NativeAttention:
             raise N.NativeError(f"nkt_attn_create failed: {self.err.buf.value.decode()}")
         self.handle = ctypes.c_void_p(h)
         self._entry = {name: getattr(self.lib, name) for name in N.ATTN_SYMBOLS}
-        self._ws_bytes: Dict[Tuple[int, int, int, int], int] = {}
+        self._ws_bytes: Dict[tuple, int] = {}
         int8 = cache_format == "int8"
         unit = 16 if int8 else 8
         dtype = torch.int8 if int8 else torch.bfloat16
@@ -234,18 +281,30 @@ class NativeAttention:
 
     def write(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
               rope: torch.Tensor, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
-              eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              eps: float = 1e-6, out: Optional[torch.Tensor] = None,
+              axes: Optional[Sequence[int]] = None) -> torch.Tensor:
         """Queries and keys normalised per head (by ``q_norm`` / ``k_norm`` [head_dim], where given) and rotated
         by their positions' rows of ``rope`` (``rope_table``); keys and values stored at ``slots`` (negative:
         not stored, padding, at any position), the queries returned [T, num_heads, head_dim].  q, k and v may be
         parts of one projection's output.  Norm weights of another type are rounded to bf16, the activations'.
-        The slots of one call have to be distinct."""
+        The slots of one call have to be distinct.
+
+        With ``axes`` (``rope_axes``: an axis for each of the head_dim / 2 frequencies) positions are [axes, T], up
+        to four: frequency i turns by ``positions[axes[i]]``."""
         q = self._strided(q, self.num_heads, "q")
         T = q.shape[0]
         k, v = self._strided(k, self.num_kv_heads, "k"), self._strided(v, self.num_kv_heads, "v")
         if k.shape[0] != T or v.shape[0] != T:
             raise ValueError(f"q has {T} tokens, k {k.shape[0]}, v {v.shape[0]}")
-        positions = self._ints(positions, torch.int64, (T,), "positions")
+        if axes is None:
+            positions = self._ints(positions, torch.int64, (T,), "positions")
+        else:
+            if len(axes) != self.head_dim // 2 or min(axes) < 0 or max(axes) >= N.ATTN_MAX_AXES:
+                raise ValueError(f"axes must be {self.head_dim // 2} numbers in [0, {N.ATTN_MAX_AXES}), got {list(axes)}")
+            if positions.dim() != 2 or not max(axes) < positions.shape[0] <= N.ATTN_MAX_AXES:
+                raise ValueError(f"positions is {tuple(positions.shape)}, expected [axes, {T}] of {max(axes) + 1} to "
+                                 f"{N.ATTN_MAX_AXES} axes")
+            positions = self._ints(positions, torch.int64, (positions.shape[0], T), "positions")
         slots = self._ints(slots, torch.int64, (T,), "slots")
         self._on_device(rope, "rope")
         if rope.dtype != torch.float32 or rope.dim() != 2 or rope.shape[1] != self.head_dim \
@@ -254,8 +313,11 @@ class NativeAttention:
         q_norm, k_norm = self._norm_weight(q_norm, "q_norm"), self._norm_weight(k_norm, "k_norm")
         out = self._out(out, T, self.num_heads)
         if T:
-            self._call("nkt_attn_write", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
-                       v.stride(0), positions.data_ptr(), slots.data_ptr(), rope.data_ptr(), rope.shape[0],
+            name, turns = "nkt_attn_write", ()
+            if axes is not None:
+                name, turns = "nkt_attn_write_axes", (positions.shape[0], bytes(axes))
+            self._call(name, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
+                       v.stride(0), positions.data_ptr(), *turns, slots.data_ptr(), rope.data_ptr(), rope.shape[0],
                        q_norm.data_ptr() if q_norm is not None else None,
                        k_norm.data_ptr() if k_norm is not None else None, eps, T, out.data_ptr())
         return out
@@ -291,20 +353,66 @@ class NativeAttention:
         self._call("nkt_attn_keep", page_table.data_ptr(), W, context_lens.data_ptr(), kept.data_ptr(),
                    kept.shape[1], counts.data_ptr(), B)
 
+    def _weights(self, t: torch.Tensor, seqs: int, name: str) -> torch.Tensor:
+        """fp32 [seqs, kv_heads, positions], positions side by side."""
+        self._on_device(t, name)
+        if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (seqs, self.num_kv_heads) \
+                or (t.stride(2) != 1 and t.shape[2] > 1):
+            raise ValueError(f"{name} must be fp32 [{seqs}, {self.num_kv_heads}, positions], positions contiguous, got "
+                             f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+        return t
+
+    def evict(self, page_table: torch.Tensor, seq_lens: torch.Tensor, weights: torch.Tensor,
+              budgets: Union[int, torch.Tensor], recent: int, *, max_seq_len: Optional[int] = None,
+              out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Brings each sequence to at most ``budgets`` tokens (a number, or [sequences]), per key / value head: the
+        ``recent`` last ones stay, and of those before them the ones with the largest ``weights`` [sequences,
+        kv_heads, positions] (``forward_weights``; of equal weights the earlier position, NaN below all numbers).
+        Older tokens that stay fill the places of evicted ones, the recent ones follow in order: the cache's order
+        changes, its keys carry their rotation.  Returns the new lengths and the weights at the tokens' new places,
+        zeros behind, in ``out`` (which may be ``weights``) or a new tensor.  Positions of new tokens count on from
+        the sequence's own, their slots from the new length.  No two sequences may share a page."""
+        page_table = self._table(page_table)
+        B, W = page_table.shape
+        seq_lens = self._ints(seq_lens, torch.int32, (B,), "seq_lens")
+        weights = self._weights(weights, B, "weights")
+        if not isinstance(budgets, torch.Tensor):
+            budgets = torch.full((B,), min(int(budgets), 2 ** 31 - 1), dtype=torch.int32, device=self.device)
+        budgets = self._ints(budgets, torch.int32, (B,), "budgets")
+        recent = min(int(recent), 2 ** 31 - 1)
+        if recent < 0:
+            raise ValueError(f"recent must not be negative, got {recent}")
+        most = min(W * self.page_size, weights.shape[2])
+        max_seq_len = most if max_seq_len is None else min(int(max_seq_len), most)
+        if out is None:
+            out = torch.empty(weights.shape, dtype=torch.float32, device=self.device)
+        elif self._weights(out, B, "out").shape != weights.shape:
+            raise ValueError(f"out is {tuple(out.shape)}, expected {tuple(weights.shape)}")
+        lens = torch.empty(B, dtype=torch.int32, device=self.device)
+        if B == 0:
+            return lens, out
+        need = self._bytes("nkt_attn_evict_workspace_bytes", B, max_seq_len)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self._call("nkt_attn_evict", page_table.data_ptr(), W, seq_lens.data_ptr(), weights.data_ptr(),
+                   weights.stride(0), weights.stride(1), weights.shape[2], budgets.data_ptr(), recent, B, max_seq_len,
+                   out.data_ptr(), out.stride(0), out.stride(1), lens.data_ptr(), ws.data_ptr(), need)
+        return lens, out
+
     # ------------------------------------------------------------------ attention
-    def _workspace_bytes(self, *sizes: int) -> int:
-        """nkt_attn_workspace_bytes of a forward call's sizes (a serving loop has few of them)."""
-        need = self._ws_bytes.get(sizes)
+    def _bytes(self, name: str, *sizes: int) -> int:
+        """What a workspace entry point says of a call's sizes (a serving loop has few of them)."""
+        need = self._ws_bytes.get((name, *sizes))
         if need is None:
             nbytes = ctypes.c_size_t(0)
-            self.err.check(self.lib.nkt_attn_workspace_bytes(self.handle, *sizes, ctypes.byref(nbytes), self.err.buf,
-                                                             self.err.size), "nkt_attn_workspace_bytes")
+            self.err.check(self._entry[name](self.handle, *sizes, ctypes.byref(nbytes), self.err.buf, self.err.size),
+                           name)
             if len(self._ws_bytes) >= 4096:
                 self._ws_bytes.clear()
-            need = self._ws_bytes[sizes] = nbytes.value
+            need = self._ws_bytes[(name, *sizes)] = nbytes.value
         return need
 
-    def _attend(self, name: str, q, head_args, page_table, seq_lens, query_starts, max_queries, max_seq_len, out):
+    def _attend(self, name: str, q, head_args, page_table, seq_lens, query_starts, max_queries, max_seq_len, out,
+                last=None, width=None):
         q = self._dense(q, self.num_heads, "q")
         T = q.shape[0]
         page_table = self._table(page_table)
@@ -322,7 +430,12 @@ class NativeAttention:
         out = self._out(out, T, self.num_heads)
         if T == 0 or B == 0:
             return out
-        need = self._workspace_bytes(T, B, max_queries, max_seq_len)
+        if last is None:
+            need = self._bytes("nkt_attn_workspace_bytes", T, B, max_queries, max_seq_len)
+        else:
+            if max_seq_len > width:
+                raise ValueError(f"weights have {width} positions for sequences of up to {max_seq_len}: pass max_seq_len")
+            need = self._bytes("nkt_attn_weights_workspace_bytes", T, B, max_queries, max_seq_len, last)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._call(name, q.data_ptr(), *head_args, page_table.data_ptr(), W, seq_lens.data_ptr(),
                    query_starts.data_ptr() if query_starts is not None else None, T, B, max_queries, max_seq_len,
@@ -354,6 +467,23 @@ class NativeAttention:
         tree_mask = self._ints(tree_mask, torch.int64, (q.shape[0], tree_mask.shape[1]), "tree_mask")
         return self._attend("nkt_attn_forward_tree", q, (tree_mask.data_ptr(), tree_mask.shape[1]), page_table,
                             seq_lens, query_starts, max_queries, max_seq_len, out)
+
+    def forward_weights(self, q: torch.Tensor, weights: torch.Tensor, page_table: torch.Tensor,
+                        seq_lens: torch.Tensor, query_starts: Optional[torch.Tensor] = None, *,
+                        max_queries: Optional[int] = None, max_seq_len: Optional[int] = None,
+                        last: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``forward`` that adds to ``weights`` (fp32 [sequences, kv_heads, positions]: row b belongs to row b of the
+        page table) what each cached token got of the attention: its softmax weights, summed over the query heads of
+        its key / value head and over each sequence's ``last`` rows (default: all).  In the same order at every call
+        of the same sizes.  What a row does not see it does not change."""
+        weights = self._weights(weights, page_table.shape[0], "weights")
+        last = 2 ** 31 - 1 if last is None else min(int(last), 2 ** 31 - 1)
+        if last < 1:
+            raise ValueError(f"last must be at least 1, got {last}")
+        width = weights.shape[2]
+        return self._attend("nkt_attn_forward_weights", q,
+                            (weights.data_ptr(), weights.stride(0), weights.stride(1), width, last), page_table,
+                            seq_lens, query_starts, max_queries, max_seq_len, out, last=last, width=width)
 
     # ------------------------------------------------------------------ status
     def status(self) -> Dict[str, bool]:

@@ -191,3 +191,103 @@ def test_tree_mask_from_parents():
     for bad in ([[0]], [[-1, 1]], [[-2]]):
         with pytest.raises(ValueError):
             tree_mask_from_parents(bad)
+
+
+WRITE_AXES = WRITE[:7] + [3, bytes([0, 1, 2] * 21 + [0])] + WRITE[7:]
+
+
+@pytest.mark.parametrize("at,value,msg", [
+    (7, 0, b"num_axes"), (7, 5, b"num_axes"), (7, -1, b"num_axes"), (7, 2, b"axis_of"), (8, None, b"axis_of"),
+    (8, bytes([0] * 63 + [3]), b"axis_of[63]"), (0, None, b"null"), (6, None, b"null"), (9, None, b"null"),
+    (1, 641, b"aligned"), (15, -1, b"num_tokens"),
+])
+def test_write_axes_rejects(bound, at, value, msg):
+    args = list(WRITE_AXES)
+    args[at] = value
+    eb = ctypes.create_string_buffer(256)
+    assert N.lib().nkt_attn_write_axes(bound, *args, None, eb, 256) == -1
+    assert msg in eb.value
+
+
+#                  q       weights  seq  head width last
+FORWARD_WEIGHTS = [0x1000, 0x1000, 1000, 500, 300, 5] + FORWARD[1:]
+
+
+@pytest.mark.parametrize("at,value,msg", [
+    (1, None, b"weights"), (1, 0x1002, b"aligned"), (2, 400, b"overlap"), (3, 200, b"overlap"), (2, -1000, b"overlap"),
+    (3, 0, b"overlap"), (2, 1 << 62, b"overlap"), (4, 199, b"weights_width"), (5, 0, b"last"), (5, -3, b"last"),
+    (0, None, b"null"), (6, None, b"null"), (8, None, b"null"), (10, -1, b"num_tokens"), (14, 0.0, b"scale"),
+    (16, None, b"workspace"), (17, 8, b"workspace"),
+])
+def test_forward_weights_rejects(bound, at, value, msg):
+    args = list(FORWARD_WEIGHTS)
+    args[16], args[17] = 0x1000, 1 << 30
+    args[at] = value
+    eb = ctypes.create_string_buffer(256)
+    assert N.lib().nkt_attn_forward_weights(bound, *args, None, eb, 256) == -1
+    assert msg in eb.value
+
+
+def test_forward_weights_workspace(bound):
+    L, eb, sz = N.lib(), ctypes.create_string_buffer(256), ctypes.c_size_t()
+    assert L.nkt_attn_weights_workspace_bytes(bound, 4, 2, 3, 200, 5, ctypes.byref(sz), eb, 256) == 0 and sz.value > 0
+    assert L.nkt_attn_weights_workspace_bytes(bound, 4, 2, 3, 200, 0, ctypes.byref(sz), eb, 256) == -1
+    assert b"last" in eb.value
+    assert L.nkt_attn_weights_workspace_bytes(bound, 1 << 20, 1 << 20, 1, 1 << 20, 1, ctypes.byref(sz), eb, 256) == -1
+    assert b"workgroups" in eb.value
+    assert L.nkt_attn_weights_workspace_bytes(None, 4, 2, 3, 200, 5, ctypes.byref(sz), eb, 256) == -1
+
+
+#        table  width lens    weights   seq  head width budgets recent B max_len out     seq  head  lens_out ws   bytes
+EVICT = [0x1000, 4, 0x1000, 0x100000, 1000, 500, 300, 0x2000, 8, 2, 200, 0x200000, 1000, 500, 0x3000, 0x1000, 1 << 20]
+
+
+@pytest.mark.parametrize("at,value,msg", [
+    (0, None, b"null"), (1, -1, b"table_width"), (1, 1 << 25, b"table_width"), (2, None, b"null"), (3, None, b"null"),
+    (4, 600, b"overlap"), (5, 200, b"overlap"), (6, -1, b"weights_width"), (7, None, b"null"), (8, -1, b"recent"),
+    (9, -1, b"num_seqs"), (9, 1 << 24, b"num_seqs"), (10, -1, b"max_seq_len"), (10, (1 << 30) + 1, b"max_seq_len"),
+    (11, None, b"null"), (11, 0x100004, b"overlaps"), (11, 0x100000 + 4 * 1700, b"overlaps"), (12, 700, b"overlap"),
+    (13, 10, b"overlap"), (14, None, b"null"), (14, 0x1000, b"lens_out"), (14, 0x2000, b"lens_out"),
+    (15, None, b"workspace"), (16, 100, b"workspace"), (15, 0x1004, b"workspace"),
+])
+def test_evict_rejects(bound, at, value, msg):
+    args = list(EVICT)
+    args[at] = value
+    eb = ctypes.create_string_buffer(256)
+    assert N.lib().nkt_attn_evict(bound, *args, None, eb, 256) == -1
+    assert msg in eb.value
+
+
+def test_evict_of_nothing(bound):
+    L, eb, sz = N.lib(), ctypes.create_string_buffer(256), ctypes.c_size_t()
+    args = list(EVICT)
+    args[9] = 0
+    assert L.nkt_attn_evict(bound, *args, None, eb, 256) == 0
+    assert L.nkt_attn_evict_workspace_bytes(bound, 2, 200, ctypes.byref(sz), eb, 256) == 0
+    assert sz.value == 2 * 2 * (4 + 2 * 101) * 4
+    assert L.nkt_attn_evict_workspace_bytes(bound, -1, 200, ctypes.byref(sz), eb, 256) == -1
+
+
+def test_rope_axes():
+    from nano_ktrans_amd import rope_axes
+
+    assert rope_axes([2, 3, 1]) == [0, 0, 1, 1, 1, 2]
+    assert rope_axes([2, 3, 1], interleaved=True) == [0, 1, 2, 0, 1, 1]
+    assert rope_axes([4]) == [0] * 4 and rope_axes([0, 2]) == [1, 1]
+    for bad in ([], [3, -1]):
+        with pytest.raises(ValueError):
+            rope_axes(bad)
+
+
+def test_media_positions():
+    from nano_ktrans_amd import media_positions
+
+    at, following = media_positions([2, (1, 2, 3), 1, (2, 1, 1), 0, 2], start=10)
+    assert at.tolist() == [[10, 11] + [12] * 6 + [15] + [16, 17] + [18, 19],
+                           [10, 11] + [12, 12, 12, 13, 13, 13] + [15] + [16, 16] + [18, 19],
+                           [10, 11] + [12, 13, 14, 12, 13, 14] + [15] + [16, 16] + [18, 19]]
+    assert following == 20
+    assert media_positions([])[0].shape == (3, 0) and media_positions([(0, 3, 3), 1])[1] == 1
+    for bad in ([-1], [(1, -1, 1)]):
+        with pytest.raises(ValueError):
+            media_positions(bad)
