@@ -479,6 +479,11 @@ int nkt_attn_forward_weights(void* handle, const void* q, float* weights, int64_
   }
   if (!check_rows("weights", seq_stride, head_stride, num_seqs, h->cache.kv_heads, weights_width, err, err_len))
     return NKT_ATTN_ERR;
+  const int64_t bytes = (int64_t)(num_tokens > 0 ? num_tokens : 0) * h->heads * h->cache.dim * 2;
+  if (q && out && (uintptr_t)q < (uintptr_t)out + bytes && (uintptr_t)out < (uintptr_t)q + bytes) {
+    set_err(err, err_len, "out overlaps q, which is read again after it");
+    return NKT_ATTN_ERR;
+  }
   const WeightsOut w = {weights, seq_stride, head_stride, last};
   return forward(handle, q, nullptr, 0, page_table, table_width, seq_lens, query_starts, num_tokens, num_seqs,
                  max_queries, max_seq_len, scale, out, workspace, workspace_bytes, stream, err, err_len, &w);

@@ -16,6 +16,7 @@ from .kernels.weight_loader import ExpertWeightLoader, GPTQLinearWeight
 from .layers.attention_block import AttentionBatch, FusedAttentionBlock, FusedDecoderLayer
 from .layers.expert_mlp import PackedSparseExpertMLP, SparseExpertMLP, build_expert_module, load_expert_weights
 from .layers.hybrid_moe import HybridMoE
+from .native_adapters import NativeAdapters
 from .native_attention import NativeAttention, media_positions, rope_axes, rope_table, tree_mask_from_parents
 from .native_moe import NativeMoE
 
@@ -26,6 +27,7 @@ __all__ = [
     "FusedDecoderLayer",
     "GPTQLinearWeight",
     "HybridMoE",
+    "NativeAdapters",
     "NativeAttention",
     "NativeMoE",
     "PackedSparseExpertMLP",

@@ -1,4 +1,5 @@
-"""ctypes binding of the gfx950 library (C ABI: include/nkt_moe.h, include/nkt_attn.h).
+"""ctypes binding of the gfx950 library (C ABI: include/nkt_moe.h, include/nkt_attn.h,
+include/nkt_lora.h).
 
 The binding style (explicit argtypes/restype, handle + error buffer + int
 return code) follows the reference's native bridge binding in
@@ -128,6 +129,25 @@ ATTN_SYMBOLS = (
     "nkt_attn_evict",
 )
 
+# nkt_lora.h
+LORA_BUF_A = 0
+LORA_BUF_B = 1
+LORA_BUF_SCALES = 2
+LORA_BUF_RANKS = 3
+LORA_BUF_STATUS = 4
+LORA_NUM_BUFS = 5
+
+LORA_STATUS = {"bad_adapter": 1}
+
+LORA_SYMBOLS = (
+    "nkt_lora_create",
+    "nkt_lora_destroy",
+    "nkt_lora_buffer_bytes",
+    "nkt_lora_bind",
+    "nkt_lora_workspace_bytes",
+    "nkt_lora_forward",
+)
+
 # bytes of the static scratch behind nkt_moe_forward_noalloc (NKT_NOALLOC_SCRATCH_BYTES)
 NOALLOC_SCRATCH_BYTES = 64 << 20
 
@@ -198,6 +218,7 @@ def lib() -> ctypes.CDLL:
     L.nkt_moe_version.argtypes = []
     L.nkt_moe_version.restype = ctypes.c_char_p
     _declare_attention(L)
+    _declare_adapters(L)
     _lib = L
     return L
 
@@ -223,6 +244,21 @@ def _declare_attention(L: ctypes.CDLL) -> None:
     L.nkt_attn_evict_workspace_bytes.argtypes = [vp, i, i, szp, cp, sz]
     L.nkt_attn_evict.argtypes = [vp, vp, i, vp, vp, l, l, i, vp, i, i, i, vp, l, l, vp, vp, sz, vp, cp, sz]
     for name in ATTN_SYMBOLS[2:]:
+        getattr(L, name).restype = i
+
+
+def _declare_adapters(L: ctypes.CDLL) -> None:
+    vp, sz, cp, i, l = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_char_p, ctypes.c_int, ctypes.c_int64
+    szp = ctypes.POINTER(ctypes.c_size_t)
+    L.nkt_lora_create.argtypes = [i, i, ctypes.POINTER(i), i, i, cp, sz]
+    L.nkt_lora_create.restype = vp
+    L.nkt_lora_destroy.argtypes = [vp]
+    L.nkt_lora_destroy.restype = None
+    L.nkt_lora_buffer_bytes.argtypes = [vp, i, szp, cp, sz]
+    L.nkt_lora_bind.argtypes = [vp, ctypes.POINTER(vp), cp, sz]
+    L.nkt_lora_workspace_bytes.argtypes = [vp, i, szp, cp, sz]
+    L.nkt_lora_forward.argtypes = [vp, vp, l, vp, l, vp, i, vp, l, vp, sz, vp, cp, sz]
+    for name in LORA_SYMBOLS[2:]:
         getattr(L, name).restype = i
 
 

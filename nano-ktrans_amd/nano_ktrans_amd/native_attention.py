@@ -475,7 +475,7 @@ class NativeAttention:
         """``forward`` that adds to ``weights`` (fp32 [sequences, kv_heads, positions]: row b belongs to row b of the
         page table) what each cached token got of the attention: its softmax weights, summed over the query heads of
         its key / value head and over each sequence's ``last`` rows (default: all).  In the same order at every call
-        of the same sizes.  What a row does not see it does not change."""
+        of the same sizes.  What a row does not see it does not change.  ``out`` must not overlap q."""
         weights = self._weights(weights, page_table.shape[0], "weights")
         last = 2 ** 31 - 1 if last is None else min(int(last), 2 ** 31 - 1)
         if last < 1:

@@ -217,11 +217,11 @@ FORWARD_WEIGHTS = [0x1000, 0x1000, 1000, 500, 300, 5] + FORWARD[1:]
     (1, None, b"weights"), (1, 0x1002, b"aligned"), (2, 400, b"overlap"), (3, 200, b"overlap"), (2, -1000, b"overlap"),
     (3, 0, b"overlap"), (2, 1 << 62, b"overlap"), (4, 199, b"weights_width"), (5, 0, b"last"), (5, -3, b"last"),
     (0, None, b"null"), (6, None, b"null"), (8, None, b"null"), (10, -1, b"num_tokens"), (14, 0.0, b"scale"),
-    (16, None, b"workspace"), (17, 8, b"workspace"),
+    (16, None, b"workspace"), (17, 8, b"workspace"), (15, 0x1000, b"overlaps q"), (15, 0x1000 + 4 * 8 * 256 - 16, b"overlaps q"),
 ])
 def test_forward_weights_rejects(bound, at, value, msg):
     args = list(FORWARD_WEIGHTS)
-    args[16], args[17] = 0x1000, 1 << 30
+    args[15], args[16], args[17] = 0x100000, 0x1000, 1 << 30
     args[at] = value
     eb = ctypes.create_string_buffer(256)
     assert N.lib().nkt_attn_forward_weights(bound, *args, None, eb, 256) == -1

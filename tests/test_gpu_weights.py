@@ -279,5 +279,8 @@ def test_refused_weights(gpu_device, make):
         p.attn.forward_weights(randn(generator(1), 2, 8, 128), make(w), p.table, p.lens)
     with pytest.raises(ValueError):
         p.attn.forward_weights(randn(generator(1), 2, 8, 128), w, p.table, p.lens, last=0)
+    q = randn(generator(1), 2, 8, 128)
+    with pytest.raises(N.NativeError, match="overlaps q"):
+        p.attn.forward_weights(q, w, p.table, p.lens, out=q)
     torch.cuda.synchronize()
     assert not bool(w.any())
