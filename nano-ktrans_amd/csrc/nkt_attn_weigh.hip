@@ -86,16 +86,35 @@ __device__ __forceinline__ int64_t place_of(const CacheView& c, const AttnArgs& 
   return (((int64_t)page * c.kv_heads + h) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
 }
 
+// A row of a head as token (of those counted) and head of the group, moved 32 rows at
+// a time without a division.
+struct Row {
+  int token, g;
+  __device__ __forceinline__ Row() {}
+  __device__ __forceinline__ Row(int row, int G) : token(row / G), g(row - row / G * G) {}
+  __device__ __forceinline__ void next(int tokens, int heads, int G) {
+    token += tokens;
+    g += heads;
+    if (g >= G) {
+      g -= G;
+      ++token;
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------
-// Maxima and sums of the rows whose maximum is past kRecountFrom, from rounded
-// scores as weigh_kernel takes them: one workgroup per 32 rows of a head, its
-// waves taking 32 tokens in turn.  Without such rows (all but broken or extreme
-// inputs) it ends after reading the statistics.
+// The rows' statistics as weigh_kernel takes them: maximum and 1 / sum, (0, 0) for a
+// row that saw nothing.  One workgroup per 256 rows of a head.  Rows whose maximum is
+// past kRecountFrom (broken or extreme inputs) get both from rounded scores again,
+// 32 rows at a time: the waves take 32 tokens in turn.
 // ---------------------------------------------------------------------------
+constexpr int kStatRows = 256;
+
 template <int D, bool I8>
 __global__ __launch_bounds__(kThreads) void recount_kernel(CacheView c, WeighArgs w, int row_blocks) {
   const AttnArgs& a = w.attn;
   __shared__ float s_m[4][2][32], s_l[4][2][32];
+  __shared__ int s_again[kStatRows / kStepRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int half = lane >> 5, col = lane & 31;
   const int HK = c.kv_heads, G = a.heads / HK;
@@ -105,55 +124,81 @@ __global__ __launch_bounds__(kThreads) void recount_kernel(CacheView c, WeighArg
   const Seq s = sequence(c, a, b, sequence_words(a, b), false);
   const int first = s.n > w.last ? s.n - w.last : 0;
   const int rows = (s.n - first) * G;
-  const int r0 = rest % row_blocks * kStepRows;
+  const int r0 = rest % row_blocks * kStatRows;
   if (r0 >= rows) return;
-  const int row = r0 + col < rows ? r0 + col : rows - 1;
-  const int token = first + row / G;
-  const int64_t at_row = (int64_t)(s.first + token) * a.heads + h * G + row % G;
-  float* stats = a.stats + 2 * at_row;
-  const bool again = recounts(stats[0], stats[1]);
-  if (!__any(again)) return;  // (the same in all waves)
-  u32x4 q[D / 16];
-  load_query<D, I8>(a.q + at_row * D, half, q);
-  const float scale2 = a.scale * kLog2e;
-  const int past = s.context + token;  // the last position that the row sees
-  const int last_row = r0 + kStepRows - 1 < rows ? r0 + kStepRows - 1 : rows - 1;
-  const int row_end = s.context + first + last_row / G + 1;
-  const int end = row_end < s.len ? row_end : s.len;
-  float m = -__builtin_huge_valf(), l = 0.f;
-  for (int p = wave * 32; p < end; p += 128) {
-    const int64_t at = place_of(c, a, b, h, p);
-    if (at < 0) continue;
-    u32x4 k[D / 16];
-    load_keys<D, I8>(c, at, col, half, k);
-    const f32x16 f = score_factors<I8>(c, at, half, scale2);
-    f32x16 st = products<D>(k, q);
-    float top = m;
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const int pos = p + (v & 3) + 8 * (v >> 2) + 4 * half;
-      st[v] = pos <= past && pos < s.len ? rounded_product(st[v], f[v]) : -__builtin_huge_valf();
-      top = fmaxf(top, st[v]);
+  auto at_row = [&](int row) {
+    return (int64_t)(s.first + first + row / G) * a.heads + h * G + row % G;
+  };
+  auto keep = [&](float* to, float m, float l) {
+    to[0] = l == 0.f ? 0.f : m;
+    to[1] = l == 0.f ? 0.f : 1.0f / l;
+  };
+  {
+    const int row = r0 + tid;
+    bool again = false;
+    if (row < rows) {
+      float* stats = a.stats + 2 * at_row(row);
+      const float m = stats[0], l = stats[1];
+      again = recounts(m, l);
+      if (!again) keep(stats, m, l);
     }
-    const float less = fmaxf(top, -__FLT_MAX__);
-    l *= __builtin_amdgcn_exp2f(m - less);
-#pragma unroll
-    for (int v = 0; v < 16; ++v) l += __builtin_amdgcn_exp2f(st[v] - less);
-    m = top;
+    const uint64_t any = __ballot(again);
+    if (lane == 0) {
+      s_again[2 * wave] = (uint32_t)any != 0;
+      s_again[2 * wave + 1] = (uint32_t)(any >> 32) != 0;
+    }
   }
-  s_m[wave][half][col] = m;
-  s_l[wave][half][col] = l;
   __syncthreads();
-  if (tid >= 32 || r0 + col >= rows || !again) return;
-  m = s_m[0][0][col];
+  const float scale2 = a.scale * kLog2e;
+  for (int block = 0; block < kStatRows / kStepRows; ++block) {
+    if (!s_again[block]) continue;
+    const int rb = r0 + block * kStepRows;
+    const int row = rb + col < rows ? rb + col : rows - 1;
+    float* stats = a.stats + 2 * at_row(row);
+    u32x4 q[D / 16];
+    load_query<D, I8>(a.q + at_row(row) * D, half, q);
+    const int past = s.context + first + row / G;  // the last position that the row sees
+    const int last_row = rb + kStepRows - 1 < rows ? rb + kStepRows - 1 : rows - 1;
+    const int row_end = s.context + first + last_row / G + 1;
+    const int end = row_end < s.len ? row_end : s.len;
+    float m = -__builtin_huge_valf(), l = 0.f;
+    for (int p = wave * 32; p < end; p += 128) {
+      const int64_t at = place_of(c, a, b, h, p);
+      if (at < 0) continue;
+      u32x4 k[D / 16];
+      load_keys<D, I8>(c, at, col, half, k);
+      const f32x16 f = score_factors<I8>(c, at, half, scale2);
+      f32x16 st = products<D>(k, q);
+      float top = m;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, s_m[i >> 1][i & 1][col]);
-  l = 0.f;
-  const float less = fmaxf(m, -__FLT_MAX__);
+      for (int v = 0; v < 16; ++v) {
+        const int pos = p + (v & 3) + 8 * (v >> 2) + 4 * half;
+        st[v] = pos <= past && pos < s.len ? rounded_product(st[v], f[v]) : -__builtin_huge_valf();
+        top = fmaxf(top, st[v]);
+      }
+      const float less = fmaxf(top, -__FLT_MAX__);
+      l *= __builtin_amdgcn_exp2f(m - less);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) l += s_l[i >> 1][i & 1][col] * __builtin_amdgcn_exp2f(s_m[i >> 1][i & 1][col] - less);
-  stats[0] = m;
-  stats[1] = l;
+      for (int v = 0; v < 16; ++v) l += __builtin_amdgcn_exp2f(st[v] - less);
+      m = top;
+    }
+    __syncthreads();  // (of the rows before, the sums are read)
+    s_m[wave][half][col] = m;
+    s_l[wave][half][col] = l;
+    __syncthreads();
+    // (the other rows of the 32 have theirs already, changed: told again as well, they
+    // are those of rounded scores too)
+    if (tid < 32 && rb + col < rows) {
+      m = s_m[0][0][col];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) m = fmaxf(m, s_m[i >> 1][i & 1][col]);
+      l = 0.f;
+      const float less = fmaxf(m, -__FLT_MAX__);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) l += s_l[i >> 1][i & 1][col] * __builtin_amdgcn_exp2f(s_m[i >> 1][i & 1][col] - less);
+      keep(stats, m, l);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -161,10 +206,34 @@ __global__ __launch_bounds__(kThreads) void recount_kernel(CacheView c, WeighArg
 // rows that see them.  S = K . Q^T on 32x32x16 matrix instructions with the keys
 // held in registers: a lane's column is a row and its registers are tokens, so
 // that the sum over rows stays in the lane until the end, and the row's maximum
-// and sum are one value per lane.
+// and sum are one value per lane.  The waves share the rows: 32 at a time go
+// straight into LDS, two steps ahead (chunk c of row r at c ^ key(r), so that the
+// rows' same chunk lies in 16 places of the 256 bytes that LDS reads at a time).
 // ---------------------------------------------------------------------------
+template <int OFF, int CTRL>
+__device__ __forceinline__ void exchange(float* x, int col) {
+  const bool high = col & OFF;
+#pragma unroll
+  for (int v = 0; v < OFF; ++v) {
+    float low_one = x[v], high_one = x[v + OFF];
+    __asm__ volatile("" : "+v"(low_one), "+v"(high_one));  // (else the selection becomes one of an index)
+    const float keep = high ? high_one : low_one, give = high ? low_one : high_one;
+    x[v] = keep + __uint_as_float(dpp_u32<CTRL>(__float_as_uint(give)));
+  }
+}
+
+template <int D>
+__device__ __forceinline__ int query_key(int r) {
+  return D == 128 ? r & 15 : r >> 1 & 7;
+}
+
 template <int D, bool I8>
 __global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighArgs w) {
+  constexpr int kChunks = D / 8;                      // 16-byte chunks of a row
+  constexpr int kLoads = kStepRows * kChunks / 256;   // of a step, per thread
+  __shared__ __align__(16) uint8_t s_q[3][kStepRows * D * 2];
+  __shared__ __align__(16) float s_stats[3][4][2 * kStepRows];
+  __shared__ __align__(16) float s_factor[I8 ? kBlockTokens : 4];  // of the tokens
   const AttnArgs& a = w.attn;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int half = lane >> 5, col = lane & 31;
@@ -176,14 +245,14 @@ __global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighAr
   const int chunk = rest % w.chunks;
   const int b = rest / w.chunks;
   const Seq s = sequence(c, a, b, sequence_words(a, b), false);
+  if (block * kBlockTokens >= s.len) return;
   const int p = block * kBlockTokens + wave * kWaveTokens;
-  if (p >= s.len) return;
-  const int64_t at = place_of(c, a, b, h, p);
-  // rows: the last tokens' ones, from the first that sees position p
+  const int64_t at = p < s.len ? place_of(c, a, b, h, p) : -1;
+  // rows: the last tokens' ones, from the first that sees the block's first position
   const int first = s.n > w.last ? s.n - w.last : 0;
   const int rows = (s.n - first) * G;
   const int end = rows < (chunk + 1) * w.chunk_rows ? rows : (chunk + 1) * w.chunk_rows;
-  const int sees = p - s.context - first;  // the first token (of those counted) that sees p
+  const int sees = block * kBlockTokens - s.context - first;  // the first token (of those counted) that does
   int r = chunk * w.chunk_rows;
   if (sees > 0 && (int64_t)sees * G > r) r = (int64_t)sees * G < end ? sees * G : end;
 
@@ -192,52 +261,123 @@ __global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighAr
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[i][v] = 0.f;
-  if (at >= 0 && r < end) {
-    u32x4 k[2][D / 16];
-    f32x16 f[2];
+  if (r < end) {
     const float scale2 = a.scale * kLog2e;
+    u32x4 k[2][D / 16];
+    if (at >= 0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      load_keys<D, I8>(c, at + 32 * i, col, half, k[i]);
-      f[i] = score_factors<I8>(c, at + 32 * i, half, scale2);
+      for (int i = 0; i < 2; ++i) load_keys<D, I8>(c, at + 32 * i, col, half, k[i]);
+      if (I8) s_factor[wave * kWaveTokens + lane] = c.k_scales[at + lane] * scale2;  // (only this wave's)
     }
-    for (; r < end; r += kStepRows) {
-      const int row = r + col < end ? r + col : end - 1;
-      const int token = first + row / G;
-      const int64_t at_row = (int64_t)(s.first + token) * a.heads + h * G + row % G;
+    // rows of q and statistics from the sequence's first on; what lies past the rows
+    // repeats the last one and is masked
+    const uint16_t* const q0 = a.q + ((int64_t)(s.first + first) * a.heads + h * G) * D;
+    const float* const stats0 = a.stats + 2 * ((int64_t)(s.first + first) * a.heads + h * G);
+    const int last_place = (end - 1) / G * a.heads + (end - 1) % G;
+    auto place = [&](const Row& row) {
+      const int x = row.token * a.heads + row.g;
+      return (int64_t)(x < last_place ? x : last_place);
+    };
+    const int dt = kStepRows / G, dg = kStepRows % G;
+    Row load_rows[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) load_rows[j] = Row(r + ((wave * kLoads + j) * 64 + lane) / kChunks, G);
+    Row stat_row(r + (lane >> 1), G);
+    Row mine(r + col, G);
+    Row front(r, G);
+    auto load = [&](int buf) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int slot = (wave * kLoads + j) * 64 + lane;
+        const int x = slot / kChunks;
+        load16_to_lds(q0 + place(load_rows[j]) * D + ((slot % kChunks) ^ query_key<D>(x)) * 8,
+                      s_q[buf] + (wave * kLoads + j) * 1024);
+        load_rows[j].next(dt, dg, G);
+      }
+      load4_to_lds(stats0 + 2 * place(stat_row) + (lane & 1), (uint8_t*)s_stats[buf][wave]);
+      stat_row.next(dt, dg, G);
+    };
+    const int seen_from = p - s.context - first;  // the first token (of those counted) that sees the wave's first one
+    auto step = [&](int from, int buf) __attribute__((always_inline)) {
       u32x4 q[D / 16];
-      load_query<D, I8>(a.q + at_row * D, half, q);
-      const float m = a.stats[2 * at_row], l = a.stats[2 * at_row + 1];
-      const bool counts = r + col < end && l != 0.f;  // (a row that saw nothing has a sum of 0)
-      const int past = counts ? s.context + token : -1;
-      const float inv = 1.0f / l;
-      const bool masks = __any(past < p + kWaveTokens - 1);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        // (the chunk that load_query takes)
+        const int chunk_at = I8 ? (i >> 1) * 4 + half * 2 + (i & 1) : 2 * i + half;
+        q[i] = *(const u32x4*)(s_q[buf] + (col * kChunks + (chunk_at ^ query_key<D>(col))) * 16);
+      }
+      // what registers 4 v .. 4 v + 3 of half i's products are multiplied by (read where
+      // it is needed: there are no registers to hold it)
+      int factors = wave * kWaveTokens + 4 * half;
+      __asm__ volatile("" : "+v"(factors));
+      auto factor = [&](int i, int v) {
+        return I8 ? *(const f32x4*)&s_factor[factors + 32 * i + 8 * v] : f32x4{scale2, scale2, scale2, scale2};
+      };
+      const float m = s_stats[buf][wave][2 * col], inv = s_stats[buf][wave][2 * col + 1];
+      f32x16 st[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) st[i] = products<D>(k[i], q);
+      const bool all_seen = front.token >= seen_from + kWaveTokens - 1 && from + kStepRows <= end;
+      if (all_seen && !__any(!(__builtin_fabsf(m) < kRecountFrom))) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int v = 0; v < 16; v += 4) {
+            const f32x4 f = factor(i, v >> 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[i][v + j] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[i][v + j], f[j], -m)), inv,
+                                             acc[i][v + j]);
+          }
+        }
+        return;
+      }
+      // tokens of the lane's that its row sees: as many from 4 half on (eight apart in fours)
+      int sees = from + col < end ? mine.token - seen_from + 1 - 4 * half : 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const f32x16 st = products<D>(k[i], q);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const float x = __builtin_amdgcn_exp2f(rounded_product(st[v], f[i][v]) - m);
-          const bool seen = !masks || p + 32 * i + (v & 3) + 8 * (v >> 2) + 4 * half <= past;
-          acc[i][v] = seen ? __builtin_fmaf(x, inv, acc[i][v]) : acc[i][v];
+        for (int v = 0; v < 16; v += 4) {
+          const f32x4 f = factor(i, v >> 2);
+          __asm__ volatile("" : "+v"(sees));  // (all comparisons at once would not fit the scalar registers)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = __builtin_amdgcn_exp2f(rounded_product(st[i][v + j], f[j]) - m);
+            acc[i][v + j] = 32 * i + 2 * v + j < sees ? __builtin_fmaf(x, inv, acc[i][v + j]) : acc[i][v + j];
+          }
         }
       }
+    };
+    load(0);
+    if (r + kStepRows < end) load(1);
+    int buf = 0;
+    for (; r < end; r += kStepRows) {
+      if (r + kStepRows < end)
+        wait_vmem_but<kLoads + 1>();
+      else
+        wait_vmem();
+      lds_barrier();
+      const int next = buf == 2 ? 0 : buf + 1;
+      if (r + 2 * kStepRows < end) load(next == 2 ? 0 : next + 1);
+      // (a wave without tokens, or whose tokens none of these rows sees, only loads)
+      if (at >= 0 && front.token + dt + 1 >= seen_from) step(r, buf);
+      buf = next;
+      mine.next(dt, dg, G);
+      front.next(dt, dg, G);
     }
   }
-  // the sum over the 32 columns, register by register of the lane's number: lanes
-  // that differ in one bit of it exchange the half that they do not keep
+  // the sum over the 32 columns, with register `col` of the 32 left in lane col: lanes
+  // that differ in a bit of it exchange the half of the registers that they do not keep
   float x[32];
 #pragma unroll
-  for (int v = 0; v < 32; ++v) x[v] = acc[v >> 4][v & 15];
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) {
-    const bool high = col & off;
-#pragma unroll
-    for (int v = 0; v < off; ++v) {
-      const float give = high ? x[v] : x[v + off], keep = high ? x[v + off] : x[v];
-      x[v] = keep + __shfl_xor(give, off);
-    }
+  for (int v = 0; v < 16; ++v) {
+    const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[0][v]), __float_as_uint(acc[1][v]), false, false);
+    x[v] = __uint_as_float(t[0]) + __uint_as_float(t[1]);
   }
+  exchange<8, 0x128>(x, col);  // lane ^ 8
+  exchange<4, 0x141>(x, col);  // lane ^ 7
+  exchange<2, 0x4e>(x, col);   // lane ^ 2
+  exchange<1, 0xb1>(x, col);   // lane ^ 1
   const int pos = p + (col >> 4) * 32 + (col & 3) + 8 * ((col & 15) >> 2) + 4 * half;
   if (pos >= s.len) return;
   if (w.chunks > 1) {
@@ -271,7 +411,7 @@ WeighPlan weigh_plan(const CacheView& c, int heads, int seqs, int max_queries, i
   WeighPlan p = {};
   const int64_t rows = (int64_t)(last < max_queries ? last : max_queries) * (heads / c.kv_heads);
   p.blocks = (max_len + kBlockTokens - 1) / kBlockTokens;
-  p.row_blocks = (int)((rows + kStepRows - 1) / kStepRows);
+  p.row_blocks = (int)((rows + kStatRows - 1) / kStatRows);
   const int64_t wgs = (int64_t)seqs * c.kv_heads * p.blocks;
   int64_t chunks = wgs > 0 ? (2048 + wgs - 1) / wgs : 1;
   const int64_t most = (rows + 255) / 256;
