@@ -78,7 +78,8 @@ struct WeighArgs {
   int64_t seq_stride, head_stride;
   int last;  // rows of a sequence's last so many tokens count
   // set by the launch
-  int blocks, chunks, chunk_rows;
+  int blocks, chunks, chunk_rows, row_blocks;
+  int32_t* extreme;  // [seqs, kv_heads, row_blocks] of 256 rows: whether some maximum is extreme
   float* parts;  // [chunks, seqs, kv_heads, blocks of tokens]
 };
 int64_t weigh_workgroups(const CacheView& c, int heads, int seqs, int max_queries, int max_len, int last);

@@ -86,19 +86,21 @@ __device__ __forceinline__ int64_t place_of(const CacheView& c, const AttnArgs& 
   return (((int64_t)page * c.kv_heads + h) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
 }
 
-// A row of a head as token (of those counted) and head of the group, moved 32 rows at
-// a time without a division.
+// Where a row of a head lies among rows of q (token after token, all heads), and its
+// head of the group, moved 32 rows at a time without a division.
 struct Row {
-  int token, g;
+  int place, g;
   __device__ __forceinline__ Row() {}
-  __device__ __forceinline__ Row(int row, int G) : token(row / G), g(row - row / G * G) {}
-  __device__ __forceinline__ void next(int tokens, int heads, int G) {
-    token += tokens;
-    g += heads;
-    if (g >= G) {
-      g -= G;
-      ++token;
-    }
+  __device__ __forceinline__ Row(int row, int G, int heads) : place(row / G * heads + row % G), g(row % G) {}
+  // EVEN: G divides 32, the head stays
+  template <bool EVEN>
+  __device__ __forceinline__ void next(int places, int heads_on, int G, int wrap) {
+    place += places;
+    if (EVEN) return;
+    g += heads_on;
+    const bool over = g >= G;
+    g -= over ? G : 0;
+    place += over ? wrap : 0;
   }
 };
 
@@ -149,6 +151,12 @@ __global__ __launch_bounds__(kThreads) void recount_kernel(CacheView c, WeighArg
     }
   }
   __syncthreads();
+  if (tid == 0) {
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < kStatRows / kStepRows; ++i) any |= s_again[i];
+    w.extreme[((int64_t)b * HK + h) * row_blocks + rest % row_blocks] = any;
+  }
   const float scale2 = a.scale * kLog2e;
   for (int block = 0; block < kStatRows / kStepRows; ++block) {
     if (!s_again[block]) continue;
@@ -227,15 +235,19 @@ __device__ __forceinline__ int query_key(int r) {
   return D == 128 ? r & 15 : r >> 1 & 7;
 }
 
-template <int D, bool I8>
+template <int D, bool I8, bool EVEN>
 __global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighArgs w) {
   constexpr int kChunks = D / 8;                      // 16-byte chunks of a row
   constexpr int kLoads = kStepRows * kChunks / 256;   // of a step, per thread
-  __shared__ __align__(16) uint8_t s_q[3][kStepRows * D * 2];
-  __shared__ __align__(16) float s_stats[3][4][2 * kStepRows];
+  // (arrays of their own: the compiler has a read from LDS wait for every load that may
+  // go into the same one)
+  constexpr int kBytes = kStepRows * D * 2;
+  __shared__ __align__(1024) uint8_t s_q0[kBytes], s_q1[kBytes], s_q2[kBytes], s_q3[kBytes];
+  __shared__ __align__(1024) float s_stats0[8 * kStepRows], s_stats1[8 * kStepRows], s_stats2[8 * kStepRows],
+      s_stats3[8 * kStepRows];
   __shared__ __align__(16) float s_factor[I8 ? kBlockTokens : 4];  // of the tokens
   const AttnArgs& a = w.attn;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int HK = c.kv_heads, G = a.heads / HK;
   const int h = (int)(blockIdx.x % (unsigned)HK);
@@ -244,10 +256,12 @@ __global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighAr
   rest /= w.blocks;
   const int chunk = rest % w.chunks;
   const int b = rest / w.chunks;
-  const Seq s = sequence(c, a, b, sequence_words(a, b), false);
-  if (block * kBlockTokens >= s.len) return;
   const int p = block * kBlockTokens + wave * kWaveTokens;
-  const int64_t at = p < s.len ? place_of(c, a, b, h, p) : -1;
+  const SeqWords words = sequence_words(a, b);
+  const int64_t found = place_of(c, a, b, h, p);  // (asked for with the sequence's words)
+  const Seq s = sequence(c, a, b, words, false);
+  if (block * kBlockTokens >= s.len) return;
+  const int64_t at = p < s.len ? found : -1;
   // rows: the last tokens' ones, from the first that sees the block's first position
   const int first = s.n > w.last ? s.n - w.last : 0;
   const int rows = (s.n - first) * G;
@@ -261,109 +275,189 @@ __global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighAr
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[i][v] = 0.f;
+  // (parts of the rows before, which see nothing of the block, are not added either)
+  if (w.chunks > 1 && r >= end) return;
+  bool extreme = false;
+  for (int i = r / kStatRows; i * kStatRows < end; ++i)
+    extreme |= w.extreme[((int64_t)b * HK + h) * w.row_blocks + i] != 0;
   if (r < end) {
     const float scale2 = a.scale * kLog2e;
+    // (a wave without tokens reads some others')
     u32x4 k[2][D / 16];
-    if (at >= 0) {
+    const int64_t keys_at = at >= 0 ? at : 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) load_keys<D, I8>(c, at + 32 * i, col, half, k[i]);
-      if (I8) s_factor[wave * kWaveTokens + lane] = c.k_scales[at + lane] * scale2;  // (only this wave's)
-    }
+    for (int i = 0; i < 2; ++i) load_keys<D, I8>(c, keys_at + 32 * i, col, half, k[i]);
+    if (I8) s_factor[wave * kWaveTokens + lane] = c.k_scales[keys_at + lane] * scale2;  // (only this wave's)
     // rows of q and statistics from the sequence's first on; what lies past the rows
     // repeats the last one and is masked
     const uint16_t* const q0 = a.q + ((int64_t)(s.first + first) * a.heads + h * G) * D;
     const float* const stats0 = a.stats + 2 * ((int64_t)(s.first + first) * a.heads + h * G);
     const int last_place = (end - 1) / G * a.heads + (end - 1) % G;
-    auto place = [&](const Row& row) {
-      const int x = row.token * a.heads + row.g;
-      return (int64_t)(x < last_place ? x : last_place);
-    };
     const int dt = kStepRows / G, dg = kStepRows % G;
-    Row load_rows[kLoads];
+    const int places = dt * a.heads + dg, wrap = a.heads - G;
+    Row load_rows[kLoads], stat_row;
+    auto start = [&] {  // the next load is of rows r on
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) load_rows[j] = Row(r + ((wave * kLoads + j) * 64 + lane) / kChunks, G);
-    Row stat_row(r + (lane >> 1), G);
-    Row mine(r + col, G);
-    Row front(r, G);
-    auto load = [&](int buf) {
+      for (int j = 0; j < kLoads; ++j) load_rows[j] = Row(r + ((wave * kLoads + j) * 64 + lane) / kChunks, G, a.heads);
+      stat_row = Row(r + (lane >> 1), G, a.heads);
+    };
+    auto load = [&](uint8_t* to_q, float* to_stats) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int slot = (wave * kLoads + j) * 64 + lane;
-        const int x = slot / kChunks;
-        load16_to_lds(q0 + place(load_rows[j]) * D + ((slot % kChunks) ^ query_key<D>(x)) * 8,
-                      s_q[buf] + (wave * kLoads + j) * 1024);
-        load_rows[j].next(dt, dg, G);
+        const int64_t x = load_rows[j].place < last_place ? load_rows[j].place : last_place;
+        load16_to_lds(q0 + x * D + ((slot % kChunks) ^ query_key<D>(slot / kChunks)) * 8,
+                      to_q + (wave * kLoads + j) * 1024);
+        load_rows[j].template next<EVEN>(places, dg, G, wrap);
       }
-      load4_to_lds(stats0 + 2 * place(stat_row) + (lane & 1), (uint8_t*)s_stats[buf][wave]);
-      stat_row.next(dt, dg, G);
+      const int64_t x = stat_row.place < last_place ? stat_row.place : last_place;
+      load4_to_lds(stats0 + 2 * x + (lane & 1), (uint8_t*)(to_stats + wave * 2 * kStepRows));
+      stat_row.template next<EVEN>(places, dg, G, wrap);
+    };
+    u32x4 q[D / 16];
+    // (the chunk that load_query takes, 2 i + half or 4 (i / 2) + 2 half + i % 2, at its
+    // place in the row: worked out each time, there are no registers to hold them all)
+    int q_at = (col * kChunks + ((I8 ? 2 * half : half) ^ query_key<D>(col))) * 16;
+    auto read = [&](const uint8_t* from_q, int i) __attribute__((always_inline)) {
+      if (D == 128) __asm__ volatile("" : "+v"(q_at));
+      q[i] = *(const u32x4*)(from_q + (q_at ^ (I8 ? (i >> 1) * 4 + (i & 1) : 2 * i) * 16));
+    };
+    // what registers 4 v .. 4 v + 3 of half i's products are multiplied by (read where
+    // it is needed: there are no registers to hold it)
+    auto factor = [&](int i, int v) __attribute__((always_inline)) {
+      if (!I8) return f32x4{scale2, scale2, scale2, scale2};
+      int at4 = wave * kWaveTokens + 4 * half;
+      __asm__ volatile("" : "+v"(at4));
+      return *(const f32x4*)&s_factor[at4 + 32 * i + 8 * v];
+    };
+    f32x16 st[2];
+    auto product = [&](int t, int i) __attribute__((always_inline)) {
+      if (i == 0) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) st[t][v] = 0.f;
+      }
+      st[t] = mfma32_bf16(k[t][i], q[i], st[t]);
+    };
+    float m, inv;
+    auto read_stats = [&](const float* stats) __attribute__((always_inline)) {
+      m = stats[wave * 2 * kStepRows + 2 * col];
+      inv = stats[wave * 2 * kStepRows + 2 * col + 1];
     };
     const int seen_from = p - s.context - first;  // the first token (of those counted) that sees the wave's first one
-    auto step = [&](int from, int buf) __attribute__((always_inline)) {
-      u32x4 q[D / 16];
+
+    // Steps whose rows may not see all tokens, whose maxima may be extreme, or that the
+    // rows end in: one step's rows on the way into LDS at a time.
+    auto any_steps = [&](int to) __attribute__((always_inline)) {
+      auto any_step = [&](const uint8_t* now_q, const float* now_stats, uint8_t* next_q,
+                          float* next_stats) __attribute__((always_inline)) {
+        wait_vmem();
+        lds_barrier();
+        if (r + kStepRows < to) load(next_q, next_stats);
+        const int left = end - r < kStepRows ? end - r : kStepRows;
+        if (at >= 0 && (r + left - 1) / G >= seen_from) {  // (else none of these rows sees the wave's tokens)
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        // (the chunk that load_query takes)
-        const int chunk_at = I8 ? (i >> 1) * 4 + half * 2 + (i & 1) : 2 * i + half;
-        q[i] = *(const u32x4*)(s_q[buf] + (col * kChunks + (chunk_at ^ query_key<D>(col))) * 16);
-      }
-      // what registers 4 v .. 4 v + 3 of half i's products are multiplied by (read where
-      // it is needed: there are no registers to hold it)
-      int factors = wave * kWaveTokens + 4 * half;
-      __asm__ volatile("" : "+v"(factors));
-      auto factor = [&](int i, int v) {
-        return I8 ? *(const f32x4*)&s_factor[factors + 32 * i + 8 * v] : f32x4{scale2, scale2, scale2, scale2};
+          for (int i = 0; i < D / 16; ++i) read(now_q, i);
+          read_stats(now_stats);
+          // tokens of the lane's that its row sees: as many from 4 half on (eight apart in fours)
+          int sees = col < left ? (r + col) / G - seen_from + 1 - 4 * half : -64;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) product(t, i);
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {
+              const f32x4 f = factor(t, v >> 2);
+              __asm__ volatile("" : "+v"(sees));  // (all comparisons at once would not fit the scalar registers)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float e = __builtin_amdgcn_exp2f(rounded_product(st[t][v + j], f[j]) - m);
+                acc[t][v + j] = 32 * t + 2 * v + j < sees ? __builtin_fmaf(e, inv, acc[t][v + j]) : acc[t][v + j];
+              }
+            }
+          }
+        }
+        r += kStepRows;
       };
-      const float m = s_stats[buf][wave][2 * col], inv = s_stats[buf][wave][2 * col + 1];
-      f32x16 st[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) st[i] = products<D>(k[i], q);
-      const bool all_seen = front.token >= seen_from + kWaveTokens - 1 && from + kStepRows <= end;
-      if (all_seen && !__any(!(__builtin_fabsf(m) < kRecountFrom))) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int v = 0; v < 16; v += 4) {
-            const f32x4 f = factor(i, v >> 2);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[i][v + j] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[i][v + j], f[j], -m)), inv,
-                                             acc[i][v + j]);
-          }
-        }
-        return;
-      }
-      // tokens of the lane's that its row sees: as many from 4 half on (eight apart in fours)
-      int sees = from + col < end ? mine.token - seen_from + 1 - 4 * half : 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int v = 0; v < 16; v += 4) {
-          const f32x4 f = factor(i, v >> 2);
-          __asm__ volatile("" : "+v"(sees));  // (all comparisons at once would not fit the scalar registers)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = __builtin_amdgcn_exp2f(rounded_product(st[i][v + j], f[j]) - m);
-            acc[i][v + j] = 32 * i + 2 * v + j < sees ? __builtin_fmaf(x, inv, acc[i][v + j]) : acc[i][v + j];
-          }
-        }
+      if (r >= to) return;
+      start();
+      lds_barrier();  // (of the steps before, all is read)
+      load(s_q0, s_stats0);
+      while (true) {
+        any_step(s_q0, s_stats0, s_q1, s_stats1);
+        if (r >= to) break;
+        any_step(s_q1, s_stats1, s_q0, s_stats0);
+        if (r >= to) break;
       }
     };
-    load(0);
-    if (r + kStepRows < end) load(1);
-    int buf = 0;
-    for (; r < end; r += kStepRows) {
-      if (r + kStepRows < end)
+
+    // Steps whose rows all see all of the workgroup's tokens.  Rows go into LDS three
+    // steps ahead and from there into registers one step ahead; the weights of one half
+    // of the tokens are worked out beside the products of the other: half 1 with this
+    // step's rows (the next one's follow into their registers), then half 0 with those.
+    // (Behind the last step: the last row again, for products that nothing takes.)
+    auto all_steps = [&](int to) __attribute__((always_inline)) {
+      auto add = [&](auto half_of, const uint8_t* next_q) __attribute__((always_inline)) {
+        constexpr int t = decltype(half_of)::value;
+        constexpr int kEach = 16 / (D / 16);  // values beside a product
+        f32x4 f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          product(1 - t, i);
+          if (t == 0) read(next_q, i);
+#pragma unroll
+          for (int v = i * kEach; v < (i + 1) * kEach; ++v) {
+            if ((v & 3) == 0) f = factor(t, v >> 2);
+            acc[t][v] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[t][v], f[v & 3], -m)), inv, acc[t][v]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      auto all_step = [&](const float* stats, const uint8_t* next_q, uint8_t* free_q,
+                          float* free_stats) __attribute__((always_inline)) {
         wait_vmem_but<kLoads + 1>();
-      else
-        wait_vmem();
+        lds_barrier();
+        load(free_q, free_stats);
+        read_stats(stats);
+        add(std::integral_constant<int, 0>{}, next_q);
+        add(std::integral_constant<int, 1>{}, next_q);
+        r += kStepRows;
+      };
+      if (r >= to) return;
+      start();
+      lds_barrier();  // (of the steps before, all is read)
+      load(s_q0, s_stats0);
+      load(s_q1, s_stats1);
+      load(s_q2, s_stats2);
+      wait_vmem_but<2 * (kLoads + 1)>();
       lds_barrier();
-      const int next = buf == 2 ? 0 : buf + 1;
-      if (r + 2 * kStepRows < end) load(next == 2 ? 0 : next + 1);
-      // (a wave without tokens, or whose tokens none of these rows sees, only loads)
-      if (at >= 0 && front.token + dt + 1 >= seen_from) step(r, buf);
-      buf = next;
-      mine.next(dt, dg, G);
-      front.next(dt, dg, G);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) read(s_q0, i);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) product(0, i);
+      while (true) {
+        all_step(s_stats0, s_q1, s_q3, s_stats3);
+        if (r >= to) break;
+        all_step(s_stats1, s_q2, s_q0, s_stats0);
+        if (r >= to) break;
+        all_step(s_stats2, s_q3, s_q1, s_stats1);
+        if (r >= to) break;
+        all_step(s_stats3, s_q0, s_q2, s_stats2);
+        if (r >= to) break;
+      }
+      wait_vmem();  // (loads into LDS end before it is used again)
+    };
+    // whole steps from the first row that sees the workgroup's last token on
+    int plain_from = end;
+    if (!extreme) {
+      const int token = sees + kBlockTokens - 1;
+      const int64_t row = token > 0 ? (int64_t)token * G : 0;
+      if (row < end) plain_from = row > r ? r + ((int)row - r + kStepRows - 1) / kStepRows * kStepRows : r;
+    }
+    if (plain_from > end - kStepRows) plain_from = end;
+    any_steps(plain_from);
+    if (plain_from < end) {
+      all_steps(r + (end - r) / kStepRows * kStepRows);
+      any_steps(end);
     }
   }
   // the sum over the 32 columns, with register `col` of the 32 left in lane col: lanes
@@ -381,7 +475,7 @@ __global__ __launch_bounds__(kThreads, 2) void weigh_kernel(CacheView c, WeighAr
   const int pos = p + (col >> 4) * 32 + (col & 3) + 8 * ((col & 15) >> 2) + 4 * half;
   if (pos >= s.len) return;
   if (w.chunks > 1) {
-    w.parts[(((int64_t)chunk * a.seqs + b) * HK + h) * ((int64_t)w.blocks * kBlockTokens) + pos] = x[0];
+    w.parts[(((int64_t)chunk * a.seqs + b) * HK + h) * ((int64_t)w.blocks * kBlockTokens) + pos] = at >= 0 ? x[0] : 0.f;
   } else if (at >= 0) {
     w.weights[b * w.seq_stride + h * w.head_stride + pos] += x[0];
   }
@@ -398,8 +492,13 @@ __global__ __launch_bounds__(kThreads) void weigh_join_kernel(CacheView c, Weigh
   const Seq s = sequence(c, a, b, sequence_words(a, b), false);
   if (pos >= s.len) return;
   const int64_t row = (int64_t)w.blocks * kBlockTokens;
+  // the chunks with rows that see the token's block
+  const int G = a.heads / HK, first = s.n > w.last ? s.n - w.last : 0;
+  const int rows = (s.n - first) * G, sees = rest % w.blocks * kBlockTokens - s.context - first;
+  const int64_t from = sees > 0 ? (int64_t)sees * G : 0;
   float sum = 0.f;
-  for (int i = 0; i < w.chunks; ++i) sum += w.parts[(((int64_t)i * a.seqs + b) * HK + h) * row + pos];
+  for (int i = from < rows ? (int)from / w.chunk_rows : w.chunks; i < w.chunks && i * w.chunk_rows < rows; ++i)
+    sum += w.parts[(((int64_t)i * a.seqs + b) * HK + h) * row + pos];
   w.weights[b * w.seq_stride + h * w.head_stride + pos] += sum;
 }
 
@@ -413,8 +512,8 @@ WeighPlan weigh_plan(const CacheView& c, int heads, int seqs, int max_queries, i
   p.blocks = (max_len + kBlockTokens - 1) / kBlockTokens;
   p.row_blocks = (int)((rows + kStatRows - 1) / kStatRows);
   const int64_t wgs = (int64_t)seqs * c.kv_heads * p.blocks;
-  int64_t chunks = wgs > 0 ? (2048 + wgs - 1) / wgs : 1;
-  const int64_t most = (rows + 255) / 256;
+  int64_t chunks = wgs > 0 ? (8192 + wgs - 1) / wgs : 1;
+  const int64_t most = (rows + 2047) / 2048;
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
   const int64_t chunk_rows = ((rows + chunks - 1) / chunks + kStepRows - 1) / kStepRows * kStepRows;
@@ -423,6 +522,8 @@ WeighPlan weigh_plan(const CacheView& c, int heads, int seqs, int max_queries, i
   return p;
 }
 
+// floats of the workspace behind the statistics: the flags, then the parts
+size_t flags_of(const CacheView& c, const WeighPlan& p, int seqs) { return (size_t)seqs * c.kv_heads * p.row_blocks; }
 size_t parts_of(const CacheView& c, const WeighPlan& p, int seqs) {
   return p.chunks > 1 ? (size_t)p.chunks * seqs * c.kv_heads * p.blocks * kBlockTokens : 0;
 }
@@ -437,8 +538,8 @@ int64_t weigh_workgroups(const CacheView& c, int heads, int seqs, int max_querie
 
 size_t weigh_workspace_floats(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len,
                               int last) {
-  return (size_t)tokens * heads * 2 +
-         parts_of(c, weigh_plan(c, heads, seqs, max_queries, max_len, last), seqs);
+  const WeighPlan p = weigh_plan(c, heads, seqs, max_queries, max_len, last);
+  return (size_t)tokens * heads * 2 + flags_of(c, p, seqs) + parts_of(c, p, seqs);
 }
 
 hipError_t launch_weigh(const CacheView& c, WeighArgs w, float* workspace, hipStream_t stream) {
@@ -448,14 +549,20 @@ hipError_t launch_weigh(const CacheView& c, WeighArgs w, float* workspace, hipSt
   w.blocks = p.blocks;
   w.chunks = p.chunks;
   w.chunk_rows = p.chunk_rows;
-  w.parts = workspace + (size_t)a.tokens * a.heads * 2;
+  w.row_blocks = p.row_blocks;
+  w.extreme = (int32_t*)(workspace + (size_t)a.tokens * a.heads * 2);
+  w.parts = workspace + (size_t)a.tokens * a.heads * 2 + flags_of(c, p, a.seqs);
   const unsigned pairs = (unsigned)a.seqs * c.kv_heads;
   by_layout(c, [&](auto dim, auto int8) {
     constexpr int D = decltype(dim)::value;
     constexpr bool I8 = decltype(int8)::value;
     hipLaunchKernelGGL((recount_kernel<D, I8>), dim3(pairs * p.row_blocks), dim3(kThreads), 0, stream, c, w,
                        p.row_blocks);
-    hipLaunchKernelGGL((weigh_kernel<D, I8>), dim3(pairs * p.blocks * p.chunks), dim3(kThreads), 0, stream, c, w);
+    const dim3 grid(pairs * p.blocks * p.chunks);
+    if (kStepRows % (a.heads / c.kv_heads) == 0)
+      hipLaunchKernelGGL((weigh_kernel<D, I8, true>), grid, dim3(kThreads), 0, stream, c, w);
+    else
+      hipLaunchKernelGGL((weigh_kernel<D, I8, false>), grid, dim3(kThreads), 0, stream, c, w);
   });
   if (p.chunks > 1) hipLaunchKernelGGL(weigh_join_kernel, dim3(pairs * p.blocks), dim3(kThreads), 0, stream, c, w);
   return hipGetLastError();
