@@ -906,6 +906,11 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
         }
       }
     }
+    if (STATS && a.scores && col < rows) {
+      float* to = a.scores + (((int64_t)b * HK + h) * part.rows + col) * a.score_row + p + g * (KS / 4);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) *(f32x4*)(to + t * 4) = st[t];
+    }
     float top = st[0][0];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -1036,7 +1041,15 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int tok = r / G;
-  if (STATS && d0 == 0) keep_stats(a, s.first + tok, h * G + r - tok * G, top, sum);
+  if (STATS && d0 == 0) {
+    if (a.scores) {
+      const int64_t at = part.row(b, h, HK, 0, r);
+      part.ml[2 * at] = top;
+      part.ml[2 * at + 1] = sum;
+    } else {
+      keep_stats(a, s.first + tok, h * G + r - tok * G, top, sum);
+    }
+  }
   uint16_t* dst = a.out + ((int64_t)(s.first + tok) * a.heads + h * G + (r - tok * G)) * D + d0;
 #pragma unroll
   for (int d = 0; d < D / 16; d += 4)
@@ -1049,7 +1062,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
 // own, so that no counter has to outlive a call: 4 us for few rows (latency), 21
 // for the chunks above (2500 tokens x 32 heads in three parts).
 template <int D, bool TREE, int ROWS, int SP>
-__global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Parts part, int row_blocks) {
+__device__ __forceinline__ void join_rows(const CacheView& c, const AttnArgs& a, const Parts& part, int row_blocks) {
   constexpr int kRows = 16 / SP, kN = D / 16;
   __shared__ float s_m[16], s_l[16];
   __shared__ __align__(16) float s_o[16][SP > 1 ? D : 4];
@@ -1125,6 +1138,85 @@ __global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Part
             u32x2{pack_pair(out[d] * inv, out[d + 1] * inv), pack_pair(out[d + 2] * inv, out[d + 3] * inv)};
     }
   }
+}
+
+template <int D, bool TREE, int ROWS, int SP>
+__global__ __launch_bounds__(256) void join_kernel(CacheView c, AttnArgs a, Parts part, int row_blocks) {
+  join_rows<D, TREE, ROWS, SP>(c, a, part, row_blocks);
+}
+
+// ---------------------------------------------------------------------------
+// The weights of cached tokens from the scores that the row form kept, beside the
+// join of its parts where there are any: 1024 tokens per workgroup behind the
+// join's.  Scores are 4 bytes per row where the keys are 2 D or D: reading them
+// back costs a batch less than the keys once more (64 sequences of up to 8192
+// tokens, 32 / 4 heads, int8: 93 us of attention that keeps them, 78 without, and 15
+// here; the keys once more and the rows' statistics 80).
+// ---------------------------------------------------------------------------
+constexpr int kWeighTokens = 1024;
+
+template <int D, int SP>
+__global__ __launch_bounds__(256) void join_weigh_kernel(CacheView c, WeighArgs w, Parts part, int row_blocks,
+                                                         int join_groups) {
+  const AttnArgs& a = w.attn;
+  if ((int)blockIdx.x < join_groups) {
+    join_rows<D, false, kRowRows, SP>(c, a, part, row_blocks);
+    return;
+  }
+  __shared__ float s_m[kRowRows], s_inv[kRowRows];
+  const int HK = c.kv_heads, G = a.heads / HK;
+  const int tid = threadIdx.x;
+  const unsigned index = blockIdx.x - join_groups;
+  const int h = (int)(index % (unsigned)HK);
+  const int rest = (int)(index / (unsigned)HK);
+  const int b = rest / w.blocks;
+  const int p = rest % w.blocks * kWeighTokens + tid * 4;
+  const Seq s = sequence(c, a, b, sequence_words(a, b), false);
+  const int rows = s.n * G;
+  if (rows == 0 || rest % w.blocks * kWeighTokens >= s.len) return;
+  const int row_end = end_of_rows<false>(s, G, 0, kRowRows);
+  const int splits = row_end > part.chunk ? (row_end + part.chunk - 1) / part.chunk : 1;
+  const int first = s.n > w.last ? (s.n - w.last) * G : 0;
+  // a row's statistics by 16 lanes: lane i the parts i, i + 16, ...
+  const int r = tid >> 4, lane = tid & 15;
+  float m = kUnseen, l = 0.f;
+  for (int i = lane; i < splits && r < rows; i += 16) {
+    const int64_t at = part.row(b, h, HK, i, r);
+    const float mi = part.ml[2 * at], li = part.ml[2 * at + 1];
+    const float to = fmaxf(m, mi);
+    l = l * factor(m, to) + li * factor(mi, to);
+    m = to;
+  }
+#pragma unroll
+  for (int off = 8; off >= 1; off >>= 1) {
+    const float mi = __shfl_xor(m, off), li = __shfl_xor(l, off);
+    const float to = fmaxf(m, mi);
+    l = l * factor(m, to) + li * factor(mi, to);
+    m = to;
+  }
+  if (lane == 0) {
+    s_m[r] = fmaxf(m, -__FLT_MAX__);  // (a number: scores of -infinity have a weight of 0)
+    s_inv[r] = l == 0.f ? 0.f : 1.0f / l;
+  }
+  __syncthreads();
+  if (p >= s.len) return;
+  const float* scores = a.scores + ((int64_t)b * HK + h) * part.rows * a.score_row + p;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = first; i < rows; ++i) {
+    const f32x4 x = *(const f32x4*)(scores + (int64_t)i * a.score_row);
+    const float less = s_m[i], inv = s_inv[i];
+    const int past = s.context + i / G - p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // (a row of NaN reaches what it sees only)
+      const float e = __builtin_amdgcn_exp2f(x[j] - less);
+      sum[j] = j <= past ? __builtin_fmaf(e, inv, sum[j]) : sum[j];
+    }
+  }
+  float* to = w.weights + b * w.seq_stride + h * w.head_stride + p;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (p + j < s.len) to[j] += sum[j];
 }
 
 // The launch of a forward call: by what the caller knows without asking the
@@ -1217,6 +1309,62 @@ int64_t attn_workgroups(const CacheView& c, int heads, int tokens, int seqs, int
 
 size_t attn_workspace_bytes(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len) {
   return plan_rows(c, plan_of(c, heads, tokens, seqs, max_queries, max_len)) * (c.dim + 2) * sizeof(float);
+}
+
+namespace {
+
+// Floats of the workspace: the parts' outputs, maxima and sums, then the scores.
+struct ScoresPlan {
+  size_t o, ml, scores;
+  int score_row;
+};
+ScoresPlan scores_plan(const CacheView& c, const Plan& p, int max_len) {
+  ScoresPlan x = {};
+  const size_t rows = (size_t)p.part.items * c.kv_heads * p.part.splits * p.part.rows;
+  x.o = p.part.splits > 1 ? rows * c.dim : 0;
+  x.ml = (rows * 2 + 3) / 4 * 4;
+  x.score_row = (max_len + 63) / 64 * 64;
+  x.scores = (size_t)p.part.items * c.kv_heads * p.part.rows * x.score_row;
+  return x;
+}
+
+}  // namespace
+
+size_t attn_scores_workspace_bytes(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len) {
+  const Plan p = plan_of(c, heads, tokens, seqs, max_queries, max_len);
+  const ScoresPlan x = scores_plan(c, p, max_len);
+  const int64_t groups = (int64_t)p.part.items * c.kv_heads *
+                         ((max_len + kWeighTokens - 1) / kWeighTokens + (p.part.splits > 1 ? join_of(c, p).row_blocks : 0));
+  if (!p.row_form || x.scores * sizeof(float) > ((size_t)1 << 30) || groups >= (int64_t)1 << 24) return 0;
+  return (x.o + x.ml + x.scores) * sizeof(float);
+}
+
+hipError_t launch_attn_scores(const CacheView& c, WeighArgs w, void* workspace, hipStream_t stream) {
+  AttnArgs& a = w.attn;
+  Plan p = plan_of(c, a.heads, a.tokens, a.seqs, a.max_queries, a.max_len);
+  const ScoresPlan x = scores_plan(c, p, a.max_len);
+  p.part.o = (float*)workspace;
+  p.part.ml = p.part.o + x.o;
+  a.scores = p.part.ml + x.ml;
+  a.score_row = x.score_row;
+  w.blocks = (a.max_len + kWeighTokens - 1) / kWeighTokens;
+  const int64_t items = (int64_t)p.part.items * c.kv_heads;
+  const JoinPlan j = join_of(c, p);
+  const int join_groups = p.part.splits > 1 ? (int)(items * j.row_blocks) : 0;
+  const dim3 grid((unsigned)(items * p.part.splits)), after((unsigned)(join_groups + items * w.blocks));
+  by_layout(c, [&](auto dim, auto int8) {
+    constexpr int D = decltype(dim)::value;
+    constexpr bool I8 = decltype(int8)::value;
+    hipLaunchKernelGGL((attn_row_kernel<D, I8, false, true>), grid, dim3(256), 0, stream, c, a, p.part);
+    if (after.x == 0) return;
+    if (j.groups == 4)
+      hipLaunchKernelGGL((join_weigh_kernel<D, 4>), after, dim3(256), 0, stream, c, w, p.part, (int)j.row_blocks,
+                         join_groups);
+    else
+      hipLaunchKernelGGL((join_weigh_kernel<D, 16>), after, dim3(256), 0, stream, c, w, p.part, (int)j.row_blocks,
+                         join_groups);
+  });
+  return hipGetLastError();
 }
 
 hipError_t launch_attn(const CacheView& c, const AttnArgs& a, void* workspace, hipStream_t stream) {

@@ -88,6 +88,15 @@ bool check_weigh_sizes(const AttnHandle* h, int num_seqs, int max_queries, int m
   return true;
 }
 
+// Workspace of a forward call that adds to weights.
+size_t weights_bytes(const AttnHandle* h, int num_tokens, int num_seqs, int max_queries, int max_seq_len, int last) {
+  const size_t scores = attn_scores_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len);
+  if (scores > 0) return scores;
+  return attn_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len) +
+         weigh_workspace_floats(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len, last) *
+             sizeof(float);
+}
+
 // Rows of a [num_seqs, kv_heads, width] array that do not overlap, whichever of the first two is the inner one.
 bool check_rows(const char* name, int64_t seq_stride, int64_t head_stride, int64_t seqs, int64_t heads, int64_t width,
                 char* err, size_t len) {
@@ -152,12 +161,9 @@ int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_word
     return NKT_ATTN_ERR;
   }
   const size_t own = attn_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len);
-  size_t need = own;
-  if (weights) {
-    if (!check_weigh_sizes(h, num_seqs, max_queries, max_seq_len, weights->last, err, len)) return NKT_ATTN_ERR;
-    need += weigh_workspace_floats(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len, weights->last) *
-            sizeof(float);
-  }
+  if (weights && !check_weigh_sizes(h, num_seqs, max_queries, max_seq_len, weights->last, err, len)) return NKT_ATTN_ERR;
+  const size_t need =
+      weights ? weights_bytes(h, num_tokens, num_seqs, max_queries, max_seq_len, weights->last) : own;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) {
     set_err(err, len, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_bytes);
     return NKT_ATTN_ERR;
@@ -178,16 +184,24 @@ int forward(void* handle, const void* q, const int64_t* tree_mask, int mask_word
   a.max_len = max_seq_len;
   a.scale = scale;
   float* more = (float*)((uint8_t*)workspace + own);
-  if (weights) a.stats = more;
+  WeighArgs w = {};
+  if (weights) {
+    w.weights = weights->weights;
+    w.seq_stride = weights->seq_stride;
+    w.head_stride = weights->head_stride;
+    w.last = weights->last;
+    if (attn_scores_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len) > 0) {
+      w.attn = a;
+      return check_hip(launch_attn_scores(h->cache, w, workspace, (hipStream_t)stream), "attention kernel", err, len)
+                 ? NKT_ATTN_OK
+                 : NKT_ATTN_ERR;
+    }
+    a.stats = more;
+  }
   if (!check_hip(launch_attn(h->cache, a, workspace, (hipStream_t)stream), "attention kernel", err, len))
     return NKT_ATTN_ERR;
   if (!weights) return NKT_ATTN_OK;
-  WeighArgs w = {};
   w.attn = a;
-  w.weights = weights->weights;
-  w.seq_stride = weights->seq_stride;
-  w.head_stride = weights->head_stride;
-  w.last = weights->last;
   if (!check_hip(launch_weigh(h->cache, w, more, (hipStream_t)stream), "attention weights kernel", err, len))
     return NKT_ATTN_ERR;
   return NKT_ATTN_OK;
@@ -456,9 +470,7 @@ int nkt_attn_weights_workspace_bytes(void* handle, int num_tokens, int num_seqs,
   if (!check_sizes(h, num_tokens, num_seqs, max_queries, max_seq_len, err, err_len) ||
       !check_weigh_sizes(h, num_seqs, max_queries, max_seq_len, last, err, err_len))
     return NKT_ATTN_ERR;
-  *bytes = attn_workspace_bytes(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len) +
-           weigh_workspace_floats(h->cache, h->heads, num_tokens, num_seqs, max_queries, max_seq_len, last) *
-               sizeof(float);
+  *bytes = weights_bytes(h, num_tokens, num_seqs, max_queries, max_seq_len, last);
   return NKT_ATTN_OK;
 }
 

@@ -62,7 +62,12 @@ struct AttnArgs {
   int tokens, seqs, heads;
   int max_queries, max_len;
   float scale;
-  float* stats;  // [tokens, heads, 2]: each row's maximum (log2) and sum of weights, or nullptr
+  // For the weights of the cached tokens, or nullptr: each row's maximum (log2) and sum
+  // of weights, [tokens, heads, 2]; in the row form, its scores instead, [seqs,
+  // kv_heads, rows, score_row] with the sequence's rows (the statistics lie with the parts).
+  float* stats;
+  float* scores;
+  int score_row;
 };
 
 // Workgroups of the call's largest launch.
@@ -86,6 +91,11 @@ int64_t weigh_workgroups(const CacheView& c, int heads, int seqs, int max_querie
 size_t weigh_workspace_floats(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len,
                               int last);
 hipError_t launch_weigh(const CacheView& c, WeighArgs w, float* workspace, hipStream_t stream);
+
+// Both in the row form, by scores kept in the workspace: while these take no more than
+// 1 GiB.  (0 bytes: not so.)
+size_t attn_scores_workspace_bytes(const CacheView& c, int heads, int tokens, int seqs, int max_queries, int max_len);
+hipError_t launch_attn_scores(const CacheView& c, WeighArgs w, void* workspace, hipStream_t stream);
 
 // Eviction: every pointer as in nkt_attn_evict.
 struct EvictArgs {

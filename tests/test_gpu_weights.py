@@ -117,6 +117,27 @@ def test_long_prompt_and_strided_weights(gpu_device):
     assert torch.equal(whole, before)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_few_rows_of_a_wide_bound(gpu_device, fmt):
+    """A bound so wide that the scores of the rows are not kept (over 1 GiB): the keys are read again."""
+    announce(f"weights of a wide bound {fmt}")
+    lengths = [500, 3, 260] * 22
+    p = make_problem(lengths, heads=32, kv_heads=4, dim=128, fmt=fmt, page=256, seed=20, width=2)
+    table = torch.full((66, 548), -1, dtype=torch.int32, device=DEV)
+    table[:, :2] = p.table
+    g = generator(21)
+    q = randn(g, 66, 32, 128)
+    before = start_weights(g, 66, 4, 548 * 256)
+    after = before.clone()
+    got = p.attn.forward_weights(q, after, table, p.lens)
+    check_attention(p, None, q, got)
+    check_weights(p, None, q, before, after)
+    narrow = before.clone()
+    assert torch.equal(got, p.attn.forward_weights(q, narrow, table, p.lens, max_seq_len=512))
+    assert float((narrow - after).abs().max()) <= 2.0 ** -14
+    p.attn.check_status()
+
+
 def test_calls_add_up_and_repeat(gpu_device):
     """A prompt in chunks gives what the whole prompt gives; the same call gives the same bits."""
     announce("weights in chunks")
