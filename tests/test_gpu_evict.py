@@ -115,12 +115,14 @@ def test_evict(gpu_device, kv_heads, dim, page, fmt, lengths, budget, recent):
     check(attn, table, lengths, weights, budget, recent)
 
 
+@pytest.mark.parametrize("fmt,dim,page", [("bf16", 128, 64), ("int8", 128, 256), ("bf16", 64, 128), ("int8", 64, 64)])
 @pytest.mark.parametrize("length", [4100, 16500, 40000])
-def test_long_sequences(gpu_device, length):
-    """Each of the selection's ways of holding its keys."""
-    announce(f"evict {length}")
-    attn, table, weights, _ = make([length, length // 3], 2, 64, "int8", 256, seed=length)
-    check(attn, table, [length, length // 3], weights, length // 5, 200)
+@pytest.mark.parametrize("share,recent", [(0.2, 200), (0.95, 64), (0.004, 3)])
+def test_long_sequences(gpu_device, length, share, recent, fmt, dim, page):
+    """Each of the selection's ways of holding its keys, many moves and few."""
+    announce(f"evict {length} to {share} {fmt} {dim} page {page}")
+    attn, table, weights, _ = make([length, length // 3], 2, dim, fmt, page, seed=length)
+    check(attn, table, [length, length // 3], weights, int(length * share), recent)
 
 
 @pytest.mark.parametrize("kind", ["equal", "zeros", "negative", "nan", "infinite", "tiny", "close", "ascending", "descending"])
