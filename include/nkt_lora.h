@@ -18,13 +18,12 @@
  * rounded up to 16, 32, 64 or 128, M = P R rounded up to 32; the ranks that an
  * adapter does not have are zero:
  *   A       bf16 [n, M / 32, in_features / 64, 4, 2, 32, 8]: value [i, m, k, j, h, r, e]
- *           is A row 32 m + place(r), column 64 k + 32 h + 8 j + e, row p R + i being
- *           rank i of part p;
- *   B       bf16 [n, N / 32, R / 16, 2, 32, 8]: value [i, c, s, h, r, e] is column
- *           32 c + place(r), rank 16 s + 8 h + e;
- *   place(r) = 16 (r / 4 % 2) + 4 (r / 8) + r % 4
- *           (64 lanes load the operand of a matrix instruction as 1 KB in one
- *           piece, and a lane's results are 16 ranks or columns side by side);
+ *           is A row 32 m + r, column 64 k + 32 h + 8 j + e, row p R + q being rank q
+ *           of part p;
+ *   B       bf16 [n, N / 64, R / 16, 2, 2, 32, 8]: value [i, c, s, o, h, r, e] is column
+ *           64 c + 2 r + o, rank 16 s + 8 h + e
+ *           (so 64 lanes load the operand of a matrix instruction as 1 KB in one
+ *           piece, and a lane's results are pairs of columns side by side);
  *   scales  fp32 [n, P];
  *   ranks   int32 [n, P];
  *   status  one uint32, zeroed by the caller.
@@ -57,8 +56,8 @@ extern "C" {
 #define NKT_LORA_STATUS_BAD_ADAPTER 1u /* an index past the adapters: the token has none */
 
 /* A handle for a projection: in_features a multiple of 64, num_parts parts (1 to
- * NKT_LORA_MAX_PARTS) of out_features[p] columns (multiples of 32), up to
- * num_adapters adapters of ranks up to max_rank (1 to NKT_LORA_MAX_RANK).  NULL on
+ * NKT_LORA_MAX_PARTS) of out_features[p] columns (multiples of 64), up to
+ * num_adapters (4096) adapters of ranks up to max_rank (1 to NKT_LORA_MAX_RANK).  NULL on
  * failure. */
 void* nkt_lora_create(int num_adapters, int in_features, const int* out_features, int num_parts, int max_rank,
                       char* err, size_t err_len);
@@ -71,12 +70,12 @@ int nkt_lora_buffer_bytes(void* handle, int buffer, size_t* bytes, char* err, si
  * may change between calls (adapters that come and go), ordered by the stream. */
 int nkt_lora_bind(void* handle, void* const* ptrs, char* err, size_t err_len);
 
-/* Workspace of a call on num_tokens tokens. */
+/* Workspace of a call on num_tokens tokens, up to 2^22 (may be 0). */
 int nkt_lora_workspace_bytes(void* handle, int num_tokens, size_t* bytes, char* err, size_t err_len);
 
 /* The adapters' part added to a projection's output.  x bf16 [num_tokens,
- * in_features], base and out bf16 [num_tokens, N], tokens *_stride elements apart,
- * pointers and strides multiples of 16 bytes; out may be base (with its stride),
+ * in_features], base and out bf16 [num_tokens, N], tokens *_stride elements apart
+ * (up to 2^27), pointers and strides multiples of 16 bytes; out may be base (with its stride),
  * else it overlaps neither base nor x.  index int64 [num_tokens]: each token's
  * adapter, in any order; negative: none, its output is base bit for bit.  Sums are
  * taken in the same order at every call of the same number of tokens. */

@@ -27,18 +27,14 @@ void set_err(char* err, size_t len, const char* fmt, ...) {
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // Tokens of a call, columns of a projection, values of a buffer's adapter.
-constexpr int kMaxTokens = 1 << 24;
+constexpr int kMaxTokens = 1 << 22;
 constexpr int64_t kMaxColumns = 1 << 20;
 constexpr int64_t kMaxValues = (int64_t)1 << 31;
 
 bool check_tokens(int num_tokens, char* err, size_t len) {
   if (num_tokens >= 0 && num_tokens <= kMaxTokens) return true;
-  set_err(err, len, "num_tokens=%d outside [0, 2^24]", num_tokens);
+  set_err(err, len, "num_tokens=%d outside [0, 2^22]", num_tokens);
   return false;
-}
-
-size_t workspace_bytes_of(const LoraView& v, int num_tokens) {
-  return (size_t)num_tokens * v.row_blocks * 32 * sizeof(float);
 }
 
 // Whether [a, a_bytes) and [b, b_bytes) share a byte.
@@ -52,8 +48,8 @@ extern "C" {
 
 void* nkt_lora_create(int num_adapters, int in_features, const int* out_features, int num_parts, int max_rank,
                       char* err, size_t err_len) {
-  if (num_adapters < 1 || num_adapters > 65536) {
-    set_err(err, err_len, "num_adapters=%d outside [1, 65536]", num_adapters);
+  if (num_adapters < 1 || num_adapters > 4096) {
+    set_err(err, err_len, "num_adapters=%d outside [1, 4096]", num_adapters);
     return nullptr;
   }
   if (in_features < 64 || in_features % 64) {
@@ -77,13 +73,13 @@ void* nkt_lora_create(int num_adapters, int in_features, const int* out_features
   int64_t columns = 0;
   for (int p = 0; p < NKT_LORA_MAX_PARTS; ++p) {
     if (p < num_parts) {
-      if (out_features[p] < 32 || out_features[p] % 32) {
-        set_err(err, err_len, "out_features[%d]=%d: a multiple of 32 wanted", p, out_features[p]);
+      if (out_features[p] < 64 || out_features[p] % 64) {
+        set_err(err, err_len, "out_features[%d]=%d: a multiple of 64 wanted", p, out_features[p]);
         return nullptr;
       }
       columns += out_features[p];
     }
-    v.part_end[p] = p < num_parts ? (int)(columns / 32) : INT32_MAX;
+    v.part_end[p] = p < num_parts ? (int)(columns / 64) : INT32_MAX;
   }
   if (columns > kMaxColumns) {
     set_err(err, err_len, "out_features of %lld in all: over 2^20", (long long)columns);
@@ -155,7 +151,7 @@ int nkt_lora_workspace_bytes(void* handle, int num_tokens, size_t* bytes, char* 
     return NKT_LORA_ERR;
   }
   if (!check_tokens(num_tokens, err, err_len)) return NKT_LORA_ERR;
-  *bytes = workspace_bytes_of(h->view, num_tokens);
+  *bytes = lora_workspace_bytes(h->view, num_tokens);
   return NKT_LORA_OK;
 }
 
@@ -183,10 +179,10 @@ int nkt_lora_forward(void* handle, const void* x, int64_t x_stride, const void* 
     set_err(err, err_len, "x, base and out (and their strides) must be 16-byte aligned");
     return NKT_LORA_ERR;
   }
-  const int64_t most = (int64_t)1 << 36;
+  const int64_t most = (int64_t)1 << 27;
   if (num_tokens > 1 && (x_stride < 0 || x_stride > most || base_stride < 0 || base_stride > most ||
                          out_stride < v.columns || out_stride > most)) {
-    set_err(err, err_len, "strides of x=%lld, base=%lld, out=%lld: not negative wanted, out's at least %d",
+    set_err(err, err_len, "strides of x=%lld, base=%lld, out=%lld: 0 to 2^27 wanted, out's at least %d",
             (long long)x_stride, (long long)base_stride, (long long)out_stride, v.columns);
     return NKT_LORA_ERR;
   }
@@ -198,8 +194,8 @@ int nkt_lora_forward(void* handle, const void* x, int64_t x_stride, const void* 
     set_err(err, err_len, "out overlaps base or x: pass base itself, or another array");
     return NKT_LORA_ERR;
   }
-  const size_t need = workspace_bytes_of(v, num_tokens);
-  if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) {
+  const size_t need = lora_workspace_bytes(v, num_tokens);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) {
     set_err(err, err_len, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_bytes);
     return NKT_LORA_ERR;
   }
@@ -212,8 +208,7 @@ int nkt_lora_forward(void* handle, const void* x, int64_t x_stride, const void* 
   a.out_stride = out_stride;
   a.index = index;
   a.tokens = num_tokens;
-  a.low = (float*)workspace;
-  const hipError_t e = launch_lora(v, a, (hipStream_t)stream);
+  const hipError_t e = launch_lora(v, a, workspace, (hipStream_t)stream);
   if (e != hipSuccess) {
     set_err(err, err_len, "adapter kernel: %s", hipGetErrorString(e));
     return NKT_LORA_ERR;

@@ -18,7 +18,7 @@ struct LoraView {
   int adapters, parts, in, columns;
   int rank;         // padded: 16, 32, 64 or 128
   int row_blocks;   // of 32 rows of A
-  int part_end[4];  // blocks of 32 columns up to and with each part
+  int part_end[4];  // blocks of 64 columns up to and with each part
 };
 
 struct LoraArgs {
@@ -28,9 +28,13 @@ struct LoraArgs {
   int64_t x_stride, base_stride, out_stride;
   const int64_t* index;
   int tokens;
-  float* low;  // [tokens, row_blocks * 32]: scale * x A^T
+  // workspace, where tokens are grouped by adapter
+  uint16_t* low;          // scale * x A^T as operands: [tiles of 32 tokens, parts, R / 16, 2, 2, 32, 8]
+  int32_t* order;         // [tiles, 32] tokens, -1: none
+  int32_t* tile_adapter;  // [tiles]
 };
 
-hipError_t launch_lora(const LoraView& v, const LoraArgs& a, hipStream_t stream);
+size_t lora_workspace_bytes(const LoraView& v, int tokens);
+hipError_t launch_lora(const LoraView& v, LoraArgs a, void* workspace, hipStream_t stream);
 
 }  // namespace nkt

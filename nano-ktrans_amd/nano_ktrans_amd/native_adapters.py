@@ -55,14 +55,11 @@ class NativeAdapters:
         # the layouts of include/nkt_lora.h
         self.a = torch.zeros(num_adapters, self._blocks, in_features // 64, 4, 2, 32, 8, dtype=torch.bfloat16,
                              device=self.device)
-        self.b = torch.zeros(num_adapters, self.columns // 32, self._rank // 16, 2, 32, 8, dtype=torch.bfloat16,
+        self.b = torch.zeros(num_adapters, self.columns // 64, self._rank // 16, 2, 2, 32, 8, dtype=torch.bfloat16,
                              device=self.device)
         self.scales = torch.zeros(num_adapters, parts, device=self.device)
         self.ranks = torch.zeros(num_adapters, parts, dtype=torch.int32, device=self.device)
         self._status = torch.zeros(4, dtype=torch.int32, device=self.device)
-        r = torch.arange(32)
-        self._place = (16 * (r // 4 % 2) + 4 * (r // 8) + r % 4).to(self.device)  # of an operand's row
-        self._row = self._place.argsort()
         ptrs = (ctypes.c_void_p * N.LORA_NUM_BUFS)()
         for i, t in enumerate((self.a, self.b, self.scales, self.ranks, self._status)):
             ptrs[i] = t.data_ptr()
@@ -100,13 +97,13 @@ class NativeAdapters:
         rows = torch.zeros(R, self.in_features, dtype=torch.bfloat16, device=self.device)
         rows[:rank] = a.to(device=self.device, dtype=torch.bfloat16)
         at = part * R + torch.arange(R, device=self.device)
-        self.a[adapter, at // 32, :, :, :, self._row[at % 32]] = \
+        self.a[adapter, at // 32, :, :, :, at % 32] = \
             rows.view(R, -1, 2, 4, 8).transpose(2, 3)
         columns = torch.zeros(out, R, dtype=torch.bfloat16, device=self.device)
         columns[:, :rank] = b.to(device=self.device, dtype=torch.bfloat16)
-        first = sum(self.out_features[:part]) // 32
-        self.b[adapter, first:first + out // 32] = \
-            columns.view(out // 32, 32, R // 16, 2, 8)[:, self._place].permute(0, 2, 3, 1, 4)
+        first = sum(self.out_features[:part]) // 64
+        self.b[adapter, first:first + out // 64] = \
+            columns.view(out // 64, 32, 2, R // 16, 2, 8).permute(0, 3, 2, 4, 1, 5)
         self.scales[adapter, part] = float(scale)
         self.ranks[adapter, part] = rank
 
@@ -164,9 +161,9 @@ class NativeAdapters:
             if len(self._ws_bytes) >= 4096:
                 self._ws_bytes.clear()
             need = self._ws_bytes[T] = nbytes.value
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         args = (self.handle, x.data_ptr(), x.stride(0), base.data_ptr(), base.stride(0), index.data_ptr(), T,
-                out.data_ptr(), out.stride(0), ws.data_ptr(), need)
+                out.data_ptr(), out.stride(0), ws.data_ptr() if ws is not None else None, need)
         err, i = self.err, self.device.index
         if torch.cuda.current_device() == i:
             rc = self.lib.nkt_lora_forward(*args, _current_stream(i), err.buf, err.size)

@@ -57,8 +57,8 @@ class Problem:
         assert torch.equal(got[none], base[none])
 
 
-SHAPES = [(4, 2048, (4096, 512, 512), 16), (24, 4096, (4096,), 32), (6, 896, (896, 128, 128), 64), (3, 64, (32,), 128),
-          (40, 128, (64, 32, 96, 32), 5), (1, 192, (256,), 1)]
+SHAPES = [(4, 2048, (4096, 512, 512), 16), (24, 4096, (4096,), 32), (6, 896, (896, 128, 128), 64), (3, 64, (64,), 128),
+          (40, 128, (128, 64, 192, 64), 5), (1, 192, (256,), 1), (5, 320, (64, 64), 100), (4, 640, (192, 64, 64, 64), 128)]
 
 
 @pytest.mark.parametrize("n,width,outs,max_rank", SHAPES)
@@ -82,6 +82,24 @@ def test_forward(gpu_device, n, width, outs, max_rank, tokens):
         assert p.adapters.forward(x, place, index.to(torch.int32), out=place) is place
         assert torch.equal(place, got)
     p.adapters.check_status()
+
+
+@pytest.mark.parametrize("n,width,outs,max_rank,tokens", [
+    (4096, 64, (64,), 4, 5000), (3, 256, (128, 64, 64), 64, 9001), (2, 128, (64,), 64, 6000), (3, 192, (64,), 16, 20000),
+    (2, 128, (64, 64, 64, 128), 128, 4500)])
+def test_many_tokens(gpu_device, n, width, outs, max_rank, tokens):
+    """More tokens than are grouped at once, more adapters than tiles, every number of blocks of A."""
+    announce(f"adapters {n} of {max_rank}, {width} -> {outs}, T={tokens}")
+    p = Problem(n, width, outs, max_rank, seed=tokens)
+    x, base = p.inputs(tokens)
+    index = torch.randint(-1, n + 1, (tokens,), generator=p.g, device=DEV)
+    got = p.adapters.forward(x, base, index)
+    p.check(x, base, index, got)
+    with pytest.raises(N.NativeError):
+        p.adapters.check_status()
+    place = base.clone()
+    p.adapters.forward(x, place, index, out=place)
+    assert torch.equal(place, got)
 
 
 @pytest.mark.parametrize("tokens", [1, 40, 600])
@@ -131,31 +149,31 @@ def test_other_requests_stay_out_of_it(gpu_device, tokens):
 def test_infinities_keep_their_sign(gpu_device):
     """One rank, one infinite feature: the sum is an infinity of the product's sign, not NaN (the ranks that the
     adapter does not have take no part)."""
-    adapters = NativeAdapters(num_adapters=1, in_features=64, out_features=32, max_rank=32)
-    a, b = torch.ones(1, 64, device=DEV), torch.ones(32, 1, device=DEV)
-    b[16:] = -1
+    adapters = NativeAdapters(num_adapters=1, in_features=64, out_features=64, max_rank=32)
+    a, b = torch.ones(1, 64, device=DEV), torch.ones(64, 1, device=DEV)
+    b[32:] = -1
     adapters.load(0, a, b)
     x = torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV)
     x[0, 9] = float("inf")
     x[1, 9] = 3.0e38
-    out = adapters.forward(x, torch.zeros(2, 32, dtype=torch.bfloat16, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV))
-    assert bool((out[0, :16] == float("inf")).all() and (out[0, 16:] == float("-inf")).all())
-    assert torch.equal(out[1, :16], x[1, 9].expand(16)) and torch.equal(out[1, 16:], -x[1, 9].expand(16))
+    out = adapters.forward(x, torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV))
+    assert bool((out[0, :32] == float("inf")).all() and (out[0, 32:] == float("-inf")).all())
+    assert torch.equal(out[1, :32], x[1, 9].expand(32)) and torch.equal(out[1, 32:], -x[1, 9].expand(32))
 
 
 def test_reload_and_other_types(gpu_device):
     """A smaller rank replaces a larger one whole; other types are rounded to bf16."""
-    p = Problem(2, 128, (64, 32), 16, seed=6, ranks=[16, 16])
+    p = Problem(2, 128, (64, 128), 16, seed=6, ranks=[16, 16])
     x, base = p.inputs(50)
     index = torch.arange(50, device=DEV) % 2
-    a, b = torch.randn(2, 128, generator=p.g, device=DEV), torch.randn(32, 2, generator=p.g, device=DEV)
+    a, b = torch.randn(2, 128, generator=p.g, device=DEV), torch.randn(128, 2, generator=p.g, device=DEV)
     p.adapters.load(1, a.double().cpu(), b.half(), 0.5, part=1)
     p.parts[1, 1] = (a.to(torch.bfloat16), b.half().to(torch.bfloat16), 0.5)
     p.check(x, base, index, p.adapters.forward(x, base, index))
 
 
 def test_bad_indexes(gpu_device):
-    p = Problem(3, 64, (32,), 4, seed=7)
+    p = Problem(3, 64, (64,), 4, seed=7)
     x, base = p.inputs(40)
     index = torch.arange(40, device=DEV) % 3
     index[5], index[39] = 3, 2 ** 40
@@ -197,25 +215,25 @@ def test_graph_and_streams(gpu_device):
 
 
 def test_empty_and_refused(gpu_device):
-    p = Problem(2, 64, (32, 32), 4, seed=9)
+    p = Problem(2, 64, (64, 64), 4, seed=9)
     x, base = p.inputs(6)
     index = torch.zeros(6, dtype=torch.int64, device=DEV)
-    assert p.adapters.forward(x[:0], base[:0], index[:0]).shape == (0, 64)
-    wide = randn(p.g, 6, 200)
+    assert p.adapters.forward(x[:0], base[:0], index[:0]).shape == (0, 128)
+    wide = randn(p.g, 6, 320)
     for args, kw in (((x[:5], base, index), {}), ((x, base[:, :32], index), {}), ((x, base, index[:4]), {}),
                      ((x.float(), base, index), {}), ((x, base.float(), index), {}), ((x, base, index.float()), {}),
                      ((x.cpu(), base, index), {}), ((x, base, index.cpu()), {}), ((x[0], base, index), {}),
-                     ((x, base, index), {"out": wide[:, 1:65]}), ((x, base, index), {"out": base.T.contiguous().T}),
-                     ((x, wide[:, :64], index), {"out": wide[:, 8:72]}), ((x, base, index), {"out": x}),
+                     ((x, base, index), {"out": wide[:, 1:129]}), ((x, base, index), {"out": base.T.contiguous().T}),
+                     ((x, wide[:, :128], index), {"out": wide[:, 8:136]}), ((wide[:, 128:192], base, index), {"out": wide[:, 128:256]}),
                      ((x, base, index), {"out": base[:1].expand(6, -1)})):
         with pytest.raises((ValueError, N.NativeError)):
             p.adapters.forward(*args, **kw)
-    a, b = torch.zeros(4, 64, device=DEV), torch.zeros(32, 4, device=DEV)
+    a, b = torch.zeros(4, 64, device=DEV), torch.zeros(64, 4, device=DEV)
     for args, kw in (((2, a, b), {}), ((-1, a, b), {}), ((0, a, b), {"part": 2}), ((0, a[:, :63], b), {}),
-                     ((0, a, b[:31]), {}), ((0, a[:3], b), {}), ((0, torch.zeros(5, 64), torch.zeros(32, 5)), {}),
+                     ((0, a, b[:63]), {}), ((0, a[:3], b), {}), ((0, torch.zeros(5, 64), torch.zeros(64, 5)), {}),
                      ((0, a[:0], b[:, :0]), {}), ((0, a.int(), b), {})):
         with pytest.raises(ValueError):
             p.adapters.load(*args, **kw)
-    for kw in (dict(in_features=65), dict(out_features=33), dict(max_rank=129), dict(num_adapters=0)):
+    for kw in (dict(in_features=65), dict(out_features=96), dict(max_rank=129), dict(num_adapters=0)):
         with pytest.raises(N.NativeError):
-            NativeAdapters(**dict(dict(num_adapters=2, in_features=64, out_features=32, max_rank=4), **kw))
+            NativeAdapters(**dict(dict(num_adapters=2, in_features=64, out_features=64, max_rank=4), **kw))

@@ -20,17 +20,17 @@ def test_header_declarations_match_binding_and_library():
         assert hasattr(N.lib(), name), name
 
 
-def _create(n=4, width=128, outs=(64, 32), rank=24):
+def _create(n=4, width=128, outs=(64, 128), rank=24):
     err = ctypes.create_string_buffer(256)
     array = (ctypes.c_int * max(1, len(outs)))(*outs) if outs is not None else None
     return N.lib().nkt_lora_create(n, width, array, 0 if outs is None else len(outs), rank, err, 256), err.value.decode()
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(n=0), "num_adapters"), (dict(n=1 << 17), "num_adapters"), (dict(width=0), "in_features"),
+    (dict(n=0), "num_adapters"), (dict(n=4097), "num_adapters"), (dict(width=0), "in_features"),
     (dict(width=96), "in_features"), (dict(outs=None), "num_parts"), (dict(outs=()), "num_parts"),
-    (dict(outs=(32,) * 5), "num_parts"), (dict(outs=(64, 16)), "out_features[1]"), (dict(outs=(0,)), "out_features[0]"),
-    (dict(rank=0), "max_rank"), (dict(rank=129), "max_rank"), (dict(outs=(1 << 20, 32)), "2^20"),
+    (dict(outs=(64,) * 5), "num_parts"), (dict(outs=(64, 96)), "out_features[1]"), (dict(outs=(0,)), "out_features[0]"),
+    (dict(rank=0), "max_rank"), (dict(rank=129), "max_rank"), (dict(outs=(1 << 20, 64)), "2^20"),
     (dict(width=1 << 27), "2^31"),
 ])
 def test_create_rejects(kw, msg):
@@ -45,10 +45,13 @@ def test_sizes(rank, padded):
     assert h, err
     L, eb, sz = N.lib(), ctypes.create_string_buffer(256), ctypes.c_size_t()
     rows = (2 * padded + 31) // 32 * 32
-    for buf, want in enumerate((4 * rows * 128 * 2, 4 * 96 * padded * 2, 4 * 2 * 4, 4 * 2 * 4, 4)):
+    for buf, want in enumerate((4 * rows * 128 * 2, 4 * 192 * padded * 2, 4 * 2 * 4, 4 * 2 * 4, 4)):
         assert L.nkt_lora_buffer_bytes(h, buf, ctypes.byref(sz), eb, 256) == 0 and sz.value == want
     assert L.nkt_lora_buffer_bytes(h, 5, ctypes.byref(sz), eb, 256) == -1
-    assert L.nkt_lora_workspace_bytes(h, 7, ctypes.byref(sz), eb, 256) == 0 and sz.value == 7 * rows * 4
+    assert L.nkt_lora_workspace_bytes(h, 64, ctypes.byref(sz), eb, 256) == 0 and sz.value == 0
+    # grouped: 3 tiles of 32, and one more for each adapter and for those without
+    assert L.nkt_lora_workspace_bytes(h, 70, ctypes.byref(sz), eb, 256) == 0
+    assert sz.value == 8 * (2 * padded * 32 * 4 + 33 * 4)
     assert L.nkt_lora_workspace_bytes(h, -1, ctypes.byref(sz), eb, 256) == -1
     assert L.nkt_lora_forward(h, None, 0, None, 0, None, 0, None, 0, None, 0, None, eb, 256) == -1
     assert b"no buffers bound" in eb.value
@@ -59,15 +62,15 @@ def test_sizes(rank, padded):
 
 
 #          x         sx   base      sb   index   T  out       so   ws      bytes
-FORWARD = [0x100000, 128, 0x200000, 96, 0x1000, 5, 0x300000, 96, 0x2000, 1 << 20]
+FORWARD = [0x100000, 128, 0x200000, 192, 0x1000, 70, 0x300000, 192, 0x2000, 1 << 20]
 
 
 @pytest.mark.parametrize("at,value,msg", [
     (0, None, b"null"), (2, None, b"null"), (4, None, b"null"), (6, None, b"null"), (0, 0x100008, b"aligned"),
-    (1, 100, b"aligned"), (2, 0x200002, b"aligned"), (3, 100, b"aligned"), (6, 0x300004, b"aligned"), (7, 97, b"aligned"),
-    (5, -1, b"num_tokens"), (5, 1 << 25, b"num_tokens"), (1, -128, b"strides"), (3, -96, b"strides"), (7, 64, b"strides"),
-    (7, 0, b"strides"), (6, 0x200010, b"overlaps"), (6, 0x100010, b"overlaps"), (2, 0x300000 + 2 * 480 - 16, b"overlaps"),
-    (8, None, b"workspace"), (9, 5 * 64 * 4 - 1, b"workspace"), (8, 0x2008, b"workspace"),
+    (1, 100, b"aligned"), (2, 0x200002, b"aligned"), (3, 100, b"aligned"), (6, 0x300004, b"aligned"), (7, 193, b"aligned"),
+    (5, -1, b"num_tokens"), (5, 1 << 25, b"num_tokens"), (1, -128, b"strides"), (3, -192, b"strides"), (7, 128, b"strides"), (1, 1 << 28, b"strides"),
+    (7, 0, b"strides"), (6, 0x200010, b"overlaps"), (6, 0x100010, b"overlaps"), (2, 0x300000 + 2 * 70 * 192 - 16, b"overlaps"),
+    (8, None, b"workspace"), (9, 7 * 2 * 32 * 32 * 4 - 1, b"workspace"), (8, 0x2008, b"workspace"),
 ])
 def test_forward_rejects(at, value, msg):
     h, err = _create()
