@@ -185,7 +185,7 @@ __device__ __forceinline__ int chunk_key(int r) {
 // heads, int8 117 us, as 128 rows 151; bf16 137 and 153.
 //
 // STATS: each row's maximum and sum go out as well (keep_stats), the sum of the weights
-// before they are rounded to bf16.
+// before they are rounded to bf16.  The prompt above 550 - 580 us, the chunks 473.
 template <int D, bool I8, bool TREE, int ROWS, bool STATS>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int kQ = D / 16;       // Q fragments, and key products per half tile
