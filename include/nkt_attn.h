@@ -172,7 +172,7 @@ int nkt_attn_weights_workspace_bytes(void* handle, int num_tokens, int num_seqs,
  * row b belongs to row b of the page table, position by position, also where
  * sequences share pages.  Positions that no counted row sees keep what they had;
  * a row that sees nothing adds nothing; one whose softmax is NaN (a NaN or infinite
- * score) makes what it sees NaN.  out is nkt_attn_forward's up to the rounding of
+ * score) makes what it sees NaN.  out is nkt_attn_forward's up to the rounding of its weights and
  * its rows' sums, and must not overlap q, which is read again after it. */
 int nkt_attn_forward_weights(void* handle, const void* q, float* weights, int64_t seq_stride, int64_t head_stride,
                              int weights_width, int last, const int32_t* page_table, int table_width,

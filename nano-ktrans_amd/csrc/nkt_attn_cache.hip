@@ -114,7 +114,7 @@ __device__ __forceinline__ bool inside(const WriteArgs& a, int t) {
 // where they have one axis (sections), else from each axis's row, 16 bytes of each at
 // once (single values from four rows cost as many turns of the memory pipeline as 64
 // lanes have lines).  12252 tokens, 32 + 8 heads, bf16, three axes: in sections 53 us,
-// 5.8 TB/s, interleaved 60; by single values 69 either way; one axis 51.  One token of
+// 5.7 TB/s, interleaved 60; by single values 69 either way; one axis 51.  One token of
 // 16 sequences, 32 / 4 heads, int8: 4.3 us, a launch's latency (one axis 3.4).
 template <int D, bool I8, int HEADS, int W, bool AXES>
 __global__ __launch_bounds__(kThreads) void write_kernel(CacheView c, WriteArgs a, int rope_blocks) {

@@ -156,7 +156,9 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(LoraView v, LoraAr
       if (t - lane + j * kGroupThreads >= a.tokens) break;
       const int group = group_of(t + j * kGroupThreads, index[j]);
       const int place = count(group, s_place);
-      if (group != kPast && (group < v.adapters || copies)) a.order[place] = t + j * kGroupThreads;
+      // (an index that another stream changed since it was counted writes nothing outside)
+      if (group != kPast && (group < v.adapters || copies) && place < tiles * kTile)
+        a.order[place] = t + j * kGroupThreads;
     }
   }
 }

@@ -86,7 +86,7 @@ class NativeAdapters:
         """a [rank, in_features] and b [out_features[part], rank] of an adapter's part, of any rank up to max_rank;
         other types than bf16 are rounded to it.  Replaces what was there."""
         self._slot(adapter, part)
-        rank, out = a.shape[0], self.out_features[part]
+        rank, out = a.shape[0] if a.dim() else 0, self.out_features[part]
         if a.dim() != 2 or a.shape[1] != self.in_features or not 1 <= rank <= self.max_rank:
             raise ValueError(f"a is {tuple(a.shape)}, expected [1 .. {self.max_rank}, {self.in_features}]")
         if tuple(b.shape) != (out, rank):
