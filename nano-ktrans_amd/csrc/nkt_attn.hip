@@ -28,6 +28,14 @@ __device__ __forceinline__ uint64_t visible(const AttnArgs& a, const Seq& s, int
   return bits & valid;
 }
 
+// What takes the roundings' common part out of sums of weight x scale: the quotient of
+// these before and after.  (Sums that say nothing, of scales that are not finite or of both
+// signs, change nothing.)
+__device__ __forceinline__ float even_by(float exact, float rounded) {
+  const float by = exact / rounded;
+  return __builtin_fabsf(by - 1.f) < 0x1p-7f ? by : 1.f;
+}
+
 // c + lo(w) + hi(w) of a pair of bf16
 __device__ __forceinline__ float add_pair(uint32_t w, float c) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -255,6 +263,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   // Running maximum (log2), sum, and what a score less m must pass for m to move:
   // -infinity until the row has seen a token, then kSlack - above.
   float m = 0.f, l = 0.f, limit = -__builtin_huge_valf();
+  // (as in the row form; 128 rows of D = 128 have no registers left for it, and have more
+  // rows, so that less of the roundings is common to all)
+  constexpr bool kEvens = I8 && STATS && (D == 64 || kPairs);
+  float exact = 0.f, rounded = 0.f;
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
 
@@ -423,6 +435,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       m += by;
       limit = moves || seen ? kSlack - above : limit;
       l *= fix;
+      if (kEvens) exact *= fix, rounded *= fix;
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[r] -= by;
 #pragma unroll
@@ -448,6 +461,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       }
       pf[q4 >> 1][2 * (q4 & 1)] = pack_pair(w[0], w[1]);
       pf[q4 >> 1][2 * (q4 & 1) + 1] = pack_pair(w[2], w[3]);
+      if (kEvens) {
+        exact += (w[0] + w[1]) + (w[2] + w[3]);
+        rounded = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], rounded));
+      }
       if (!I8 && !STATS) l = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], l));
     }
   };
@@ -668,6 +685,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
     step(std::integral_constant<int, 1>{});
   }
   l = add_xor32(l);
+  if (kEvens) {
+    const float by = even_by(add_xor32(exact), add_xor32(rounded));
+#pragma unroll
+    for (int i = 0; i < kO; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] *= by;
+  }
   if (kPairs) {  // the second pair's results, added to the first's (whose keys and values are read)
     float* const s_o = (float*)lds.k + (wave & 1) * (D / 2) * 64 + lane;
     float* const s_ml = (float*)lds.v + (wave & 1) * 128 + lane;
@@ -1017,11 +1041,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   // the waves' results, added in order
   l = add_xor32(add_xor16(l));
   if (kEvens) {
-    exact = add_xor32(add_xor16(exact));
-    rounded = add_xor32(add_xor16(rounded));
-    // (sums that say nothing, of scales that are not finite or of both signs, change nothing)
-    const float even = exact / rounded;
-    const float by = __builtin_fabsf(even - 1.f) < 0x1p-7f ? even : 1.f;
+    const float by = even_by(add_xor32(add_xor16(exact)), add_xor32(add_xor16(rounded)));
 #pragma unroll
     for (int i = 0; i < kO; ++i) o[i] *= by;
   }

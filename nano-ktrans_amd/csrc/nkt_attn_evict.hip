@@ -509,7 +509,7 @@ hipError_t launch_evict(const CacheView& c, const EvictArgs& e, hipStream_t stre
     hipLaunchKernelGGL(select_kernel<32>, grid, threads, 0, stream, c, e);
   else
     hipLaunchKernelGGL(select_kernel<0>, grid, threads, 0, stream, c, e);
-  // about 4096 workgroups (of 3 sequences of up to 30011 tokens, 8 heads, the fill takes
+  // about 4096 workgroups (of one sequence of 30011 tokens, 8 heads, the fill takes
   // 16 us; with 2048 workgroups 20)
   int64_t groups = (most_moves(e.max_len) + kGroup - 1) / kGroup;
   const int64_t share = (4096 + pairs - 1) / pairs;
