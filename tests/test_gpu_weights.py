@@ -81,6 +81,24 @@ def test_decode(gpu_device, heads, kv_heads, dim, fmt, lengths):
     p.attn.check_status()
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,counts", [
+    (32, 4, 128, [1, 1, 1]), (5, 1, 64, [1]), (32, 4, 128, [3, 8]), (5, 1, 64, [4]), (14, 2, 64, [40])])
+def test_one_int8_token_is_its_value(gpu_device, heads, kv_heads, dim, counts):
+    """A row that sees one token: weight x scale is rounded to bf16 for the product, but all of that is common to
+    the row and taken out again.  What is left: the output's rounding, 2^-8 of it, and a few of fp32, under 2^-20."""
+    announce(f"weights of one int8 token {heads}/{kv_heads}/{dim} {counts}")
+    for seed in range(4):
+        p = make_problem(counts, heads=heads, kv_heads=kv_heads, dim=dim, fmt="int8", page=64, seed=seed)
+        q = randn(generator(seed + 9), sum(counts), heads, dim)
+        weights = torch.zeros(len(counts), kv_heads, max(counts), device=DEV)
+        starts = None if max(counts) == 1 else starts_of(counts)
+        got = p.attn.forward_weights(q, weights, p.table, p.lens, starts, max_queries=max(counts), max_seq_len=max(counts))
+        for b, first in enumerate(split_rows(counts)[:-1]):
+            want = p.v[b][0].repeat_interleave(heads // kv_heads, dim=0).double()
+            off = (got[first].double() - want).abs() - (2.0 ** -8 + 2.0 ** -20) * want.abs()
+            assert bool((off <= 0).all()), f"sequence {b}: worst {float(off.max())} over its bound"
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "int8"])
 @pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
 @pytest.mark.parametrize("counts,lengths", [([2, 1], [70, 1]), ([5, 16, 1], [40, 300, 90]), ([33, 64, 0, 7], [900, 64, 12, 8]),
