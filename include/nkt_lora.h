@@ -77,8 +77,10 @@ int nkt_lora_workspace_bytes(void* handle, int num_tokens, size_t* bytes, char* 
  * in_features], base and out bf16 [num_tokens, N], tokens *_stride elements apart
  * (up to 2^27), pointers and strides multiples of 16 bytes; out may be base (with its stride),
  * else it overlaps neither base nor x.  index int64 [num_tokens]: each token's
- * adapter, in any order; negative: none, its output is base bit for bit.  Sums are
- * taken in the same order at every call of the same number of tokens. */
+ * adapter, in any order; negative: none, its output is base bit for bit.  If another
+ * stream changes index while the call runs, which adapter a token gets is undefined, and
+ * nothing else is written.  Sums are taken in the same order at every call of the same
+ * number of tokens. */
 int nkt_lora_forward(void* handle, const void* x, int64_t x_stride, const void* base, int64_t base_stride,
                      const int64_t* index, int num_tokens, void* out, int64_t out_stride, void* workspace,
                      size_t workspace_bytes, void* stream, char* err, size_t err_len);

@@ -85,19 +85,11 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(LoraView v, LoraAr
   const int n = v.adapters + 1;  // (the last: without an adapter)
   for (int i = tid; i < n; i += kGroupThreads) s_count[i] = 0;
   __syncthreads();
-  // (indices of kEach tokens at once: one at a time their latency is all there is)
+  // (of kEach tokens at once: one at a time their latency is all there is)
   constexpr int kEach = 8;
-  int64_t index[kEach];
-  auto load = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int from = t + j * kGroupThreads;
-      index[j] = a.index[from < a.tokens ? from : a.tokens - 1];
-    }
-  };
-  auto group_of = [&](int t, int64_t i) __attribute__((always_inline)) {
-    return t >= a.tokens ? kPast : i < 0 || i >= v.adapters ? v.adapters : (int)i;
-  };
+  // A token's group, told from its index once and kept where low comes to lie: told again it
+  // could be another one, if the index changes meanwhile, and places would stay unwritten.
+  int32_t* const groups = (int32_t*)a.low;
   // (of a wave's tokens, those of the first one's adapter in one addition)
   auto count = [&](int group, int* to) __attribute__((always_inline)) {
     const int lead = __builtin_amdgcn_readfirstlane(group);
@@ -111,13 +103,23 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(LoraView v, LoraAr
     return at;
   };
   for (int t = tid; t - lane < a.tokens; t += kEach * kGroupThreads) {
-    load(t);
+    int64_t index[kEach];
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      if (t - lane + j * kGroupThreads >= a.tokens) break;
-      if (t + j * kGroupThreads < a.tokens && index[j] >= v.adapters)
-        __hip_atomic_fetch_or(v.status, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      count(group_of(t + j * kGroupThreads, index[j]), s_count);
+      const int from = t + j * kGroupThreads;
+      index[j] = a.index[from < a.tokens ? from : a.tokens - 1];
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int at = t + j * kGroupThreads;
+      if (at - lane >= a.tokens) break;
+      const int64_t i = index[j];
+      const int group = at >= a.tokens ? kPast : i < 0 || i >= v.adapters ? v.adapters : (int)i;
+      if (group != kPast) {
+        if (i >= v.adapters) __hip_atomic_fetch_or(v.status, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        groups[at] = group;
+      }
+      count(group, s_count);
     }
   }
   __syncthreads();
@@ -150,15 +152,18 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(LoraView v, LoraAr
   for (int t = total + tid; t < tiles; t += kGroupThreads) a.tile_adapter[t] = kPast;
   __syncthreads();
   for (int t = tid; t - lane < a.tokens; t += kEach * kGroupThreads) {
-    load(t);
+    int group[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {  // (the thread's own)
+      const int at = t + j * kGroupThreads;
+      group[j] = at < a.tokens ? groups[at] : kPast;
+    }
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      if (t - lane + j * kGroupThreads >= a.tokens) break;
-      const int group = group_of(t + j * kGroupThreads, index[j]);
-      const int place = count(group, s_place);
-      // (an index that another stream changed since it was counted writes nothing outside)
-      if (group != kPast && (group < v.adapters || copies) && place < tiles * kTile)
-        a.order[place] = t + j * kGroupThreads;
+      const int at = t + j * kGroupThreads;
+      if (at - lane >= a.tokens) break;
+      const int place = count(group[j], s_place);
+      if (group[j] != kPast && (group[j] < v.adapters || copies)) a.order[place] = at;
     }
   }
 }

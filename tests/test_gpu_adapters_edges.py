@@ -1,0 +1,40 @@
+"""Adapters: calls that a serving program makes beside others, and inputs at the edge of what is allowed.  Tolerances
+as in test_gpu_adapters.py."""
+import pytest
+import torch
+
+from attn_cases import DEV, randn
+from test_gpu_adapters import Problem, announce
+
+pytestmark = pytest.mark.gpu
+
+
+def test_index_that_changes_during_calls(gpu_device):
+    """Another stream writes one of two index arrays while calls run: each token gets the adapter of one of the
+    two, whole and bit for bit, and nothing outside of the output is written."""
+    announce("adapters, index changes")
+    tokens, columns = 5000, 192
+    p = Problem(6, 256, (128, 64), 16, seed=21)
+    x, base = p.inputs(tokens)
+    choices = [torch.randint(-1, 6, (tokens,), generator=p.g, device=DEV) for _ in range(2)]
+    wants = [p.adapters.forward(x, base, index) for index in choices]
+    for index, want in zip(choices, wants):
+        p.check(x, base, index, want)
+    index = choices[0].clone()
+    outs = [torch.full((tokens + 200, columns), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(40)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        with torch.cuda.stream(side):
+            for j in range(4):
+                index.copy_(choices[j % 2])
+        p.adapters.forward(x, base, index, out=out[100:-100])
+    torch.cuda.synchronize()
+    for out in outs:
+        got = out[100:-100]
+        of = [(got == want).all(dim=1) for want in wants]
+        assert bool((of[0] | of[1]).all())
+        assert bool((out[:100] == 7.0).all() and (out[-100:] == 7.0).all())
+    p.adapters.check_status()
+    got = p.adapters.forward(x, base, index)
+    assert torch.equal(got, wants[1])
