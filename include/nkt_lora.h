@@ -25,7 +25,7 @@
  *           (so 64 lanes load the operand of a matrix instruction as 1 KB in one
  *           piece, and a lane's results are pairs of columns side by side);
  *   scales  fp32 [n, P];
- *   ranks   int32 [n, P];
+ *   ranks   int32 [n, P]: ranks past R count as R, negative ones as 0;
  *   status  one uint32, zeroed by the caller.
  */
 #ifndef NKT_LORA_H

@@ -175,9 +175,14 @@ __device__ __forceinline__ uint16_t* low_at(const LoraView& v, const LoraArgs& a
   return a.low + ((((int64_t)tile * v.parts + part) * (v.rank / 16) + s) * 2 + which) * 512;
 }
 
+// A part's rank of an adapter, within what its matrices hold (the caller's buffer may say anything).
+__device__ __forceinline__ int rank_of(const LoraView& v, int adapter, int part) {
+  const int rank = v.ranks[adapter * v.parts + part];
+  return rank < 0 ? 0 : rank < v.rank ? rank : v.rank;
+}
 // The adapter's ranks, one per part and lane.
 __device__ __forceinline__ int lane_ranks(const LoraView& v, int adapter, int lane) {
-  return lane < v.parts ? v.ranks[adapter * v.parts + lane] : 0;
+  return lane < v.parts ? rank_of(v, adapter, lane) : 0;
 }
 
 // A wave's share of 32 tokens of x times MB blocks of A: groups of 64 features kw, kw +
@@ -491,7 +496,7 @@ __global__ __launch_bounds__(512) void both_kernel(LoraView v, LoraArgs a, int s
     }
     return;
   }
-  const int rank = v.ranks[adapter * v.parts + part];
+  const int rank = rank_of(v, adapter, part);
   const float scale = v.scales[adapter * v.parts + part];
   const uint16_t* b = v.b + (int64_t)adapter * (v.columns / 64) * (KS * 1024) + lane * 8;
   constexpr int kAhead = KS < 2 ? KS : 2;  // steps of B asked for before low

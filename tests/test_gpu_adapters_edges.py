@@ -38,3 +38,18 @@ def test_index_that_changes_during_calls(gpu_device):
     p.adapters.check_status()
     got = p.adapters.forward(x, base, index)
     assert torch.equal(got, wants[1])
+
+
+@pytest.mark.parametrize("tokens", [5, 64, 200])
+@pytest.mark.parametrize("max_rank", [8, 32, 64, 100])
+def test_ranks_past_the_largest(gpu_device, tokens, max_rank):
+    """The ranks' buffer is an ordinary tensor: numbers that no adapter can have are those that it can."""
+    announce(f"adapters with ranks past {max_rank}, T={tokens}")
+    p = Problem(3, 128, (64, 128), max_rank, seed=22, ranks=[max_rank] * 3)
+    x, base = p.inputs(tokens)
+    index = torch.arange(tokens, device=DEV) % 4 - 1
+    largest = next(r for r in (16, 32, 64, 128) if max_rank <= r)  # (what was not loaded is zero)
+    p.adapters.ranks.copy_(torch.tensor([[largest, 1], [largest, largest], [0, largest]]))
+    want = p.adapters.forward(x, base, index)
+    p.adapters.ranks.copy_(torch.tensor([[129, 1], [2 ** 31 - 1, 5000], [-(2 ** 31), 1 << 20]]))
+    assert torch.equal(p.adapters.forward(x, base, index), want)
