@@ -25,6 +25,7 @@ per layer:
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -299,6 +300,8 @@ class NativeAttention:
         if axes is None:
             positions = self._ints(positions, torch.int64, (T,), "positions")
         else:
+            if not isinstance(axes, (list, tuple)):  # (the bytes of an array are not those of its numbers)
+                axes = [operator.index(i) for i in axes]
             if len(axes) != self.head_dim // 2 or min(axes) < 0 or max(axes) >= N.ATTN_MAX_AXES:
                 raise ValueError(f"axes must be {self.head_dim // 2} numbers in [0, {N.ATTN_MAX_AXES}), got {list(axes)}")
             if positions.dim() != 2 or not max(axes) < positions.shape[0] <= N.ATTN_MAX_AXES:
