@@ -129,4 +129,6 @@ class FusedDecoderLayer(nn.Module):
 
     def forward(self, hidden_states: torch.Tensor, batch: AttentionBatch,
                 weights: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return self.moe_block(self.attention_block(hidden_states, batch, weights))
+        # (an attention half that knows of no weights is called without them)
+        args = () if weights is None else (weights,)
+        return self.moe_block(self.attention_block(hidden_states, batch, *args))
