@@ -169,8 +169,9 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(LoraView v, LoraAr
 }
 
 // low, as the operands of the second product: two bf16 values whose sum is a rank's
-// fp32 value to 2^-16 of it (its upper 16 bits, and the rest rounded; an infinity has
-// no rest).  Per tile, part, 16 ranks and which of the two: 64 lanes x 8 ranks.
+// fp32 value to 2^-16 of it (its upper 16 bits, and the rest rounded).  The second is
+// zero only where the value is (an infinity's is one too), so that an infinity of B
+// stays one.  Per tile, part, 16 ranks and which of the two: 64 lanes x 8 ranks.
 __device__ __forceinline__ uint16_t* low_at(const LoraView& v, const LoraArgs& a, int tile, int part, int s, int which) {
   return a.low + ((((int64_t)tile * v.parts + part) * (v.rank / 16) + s) * 2 + which) * 512;
 }
@@ -253,7 +254,9 @@ __device__ __forceinline__ void split_ranks(const float* sums, int run, int toke
     const float y = first + i < rank ? sum * scale : 0.f;
     const uint32_t bits = __float_as_uint(y);
     high[i] = y != y ? 0x7fc00000u : bits & 0xffff0000u;
-    rest[i] = (bits & 0x7f800000u) == 0x7f800000u ? 0.f : y - __uint_as_float(high[i]);
+    // (0 times an infinity is NaN: in the place of no rest 2^-32 of y, which its fp32 sums lose)
+    rest[i] = y - __uint_as_float(high[i]);
+    rest[i] = rest[i] == 0.f || (bits & 0x7f800000u) == 0x7f800000u ? y * 0x1p-32f : rest[i];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from attn_cases import DEV, randn
+from nano_ktrans_amd import NativeAdapters
 from test_gpu_adapters import Problem, announce
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,22 @@ def test_ranks_past_the_largest(gpu_device, tokens, max_rank):
     want = p.adapters.forward(x, base, index)
     p.adapters.ranks.copy_(torch.tensor([[129, 1], [2 ** 31 - 1, 5000], [-(2 ** 31), 1 << 20]]))
     assert torch.equal(p.adapters.forward(x, base, index), want)
+
+
+@pytest.mark.parametrize("tokens", [3, 64, 90])
+def test_infinite_adapters(gpu_device, tokens):
+    """An infinity in B times what is exactly a bf16 number (or itself an infinity) is an infinity of the product's
+    sign; times zero it is NaN, as in the formula."""
+    announce(f"adapters with infinities T={tokens}")
+    adapters = NativeAdapters(num_adapters=1, in_features=64, out_features=64, max_rank=16)
+    a, b = torch.ones(1, 64, device=DEV), torch.full((64, 1), float("inf"), device=DEV)
+    b[32:] = float("-inf")
+    adapters.load(0, a, b)
+    x = torch.zeros(tokens, 64, dtype=torch.bfloat16, device=DEV)
+    x[0, 9], x[1, 9] = 3.0, float("-inf")
+    base = torch.zeros(tokens, 64, dtype=torch.bfloat16, device=DEV)
+    out = adapters.forward(x, base, torch.zeros(tokens, dtype=torch.int64, device=DEV))
+    want = torch.full((64,), float("inf"), dtype=torch.bfloat16, device=DEV)
+    want[32:] = float("-inf")
+    assert torch.equal(out[0], want) and torch.equal(out[1], -want)
+    assert bool(torch.isnan(out[2:]).all())
