@@ -193,7 +193,9 @@ __device__ __forceinline__ int chunk_key(int r) {
 // heads, int8 117 us, as 128 rows 151; bf16 137 and 153.
 //
 // STATS: each row's maximum and sum go out as well (keep_stats), the sum of the weights
-// before they are rounded to bf16.  The prompt above 550 - 580 us, the chunks 473.
+// before they are rounded to bf16; outputs are divided by that after the rounding, as without
+// STATS.  The prompt above, whole calls whose last 64 tokens count: 598 us, with the one sum
+// 580 (and outputs off by 0.0021 of their size instead of 0.0019), forward 553.
 template <int D, bool I8, bool TREE, int ROWS, bool STATS>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs a, Parts part) {
   constexpr int kQ = D / 16;       // Q fragments, and key products per half tile
@@ -263,10 +265,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   // Running maximum (log2), sum, and what a score less m must pass for m to move:
   // -infinity until the row has seen a token, then kSlack - above.
   float m = 0.f, l = 0.f, limit = -__builtin_huge_valf();
-  // (as in the row form; 128 rows of D = 128 have no registers left for it, and have more
+  // (bf16's 128 rows beside weights have no register for limit: it is 0 once the row has
+  // seen a token, and that shows in m, which is never 0 from there on)
+  constexpr bool kSeenByM = STATS && !I8 && !kPairs;
+  auto row_sees = [&] { return kSeenByM ? !(m == 0.f) : limit >= 0.f; };
+  // (as in the row form; bf16: l is the sum of the rounded weights, as without STATS, and
+  // exact that before; int8's 128 rows of D = 128 have no registers left for it, and have more
   // rows, so that less of the roundings is common to all)
-  constexpr bool kEvens = I8 && STATS && (D == 64 || kPairs);
-  float exact = 0.f, rounded = 0.f;
+  constexpr bool kEvens = STATS && (!I8 || D == 64 || kPairs);
+  float exact = 0.f, rounded = 0.f;  // (rounded: int8)
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
 
@@ -418,10 +425,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   float top = kUnseen;  // of the next half tile's scores, less m
   // (int8: p is the tile's position, scale the value scale of the lane's token of it)
   auto rescale = [&](int p, float scale) {
-    const bool moves = top > limit;
+    const bool moves = top > (kSeenByM ? row_sees() ? 0.f : -__builtin_huge_valf() : limit);
     if (__any(moves || (I8 && scale > kLargeScale))) {
-      const bool seen = limit >= 0.f;  // (nothing to rescale before)
-      float above = seen ? kSlack - limit : I8 ? 0.f : kSlack, up = 0.f;
+      const bool seen = row_sees();  // (nothing to rescale before)
+      float above = kSeenByM ? kSlack : seen ? kSlack - limit : I8 ? 0.f : kSlack, up = 0.f;
       if (I8) {
         const uint64_t large = __ballot(scale > kLargeScale);
         if (large) {
@@ -433,9 +440,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       const float by = moves ? top + above : seen ? up : 0.f;
       const float fix = seen ? __builtin_amdgcn_exp2f(-by) : 1.f;
       m += by;
-      limit = moves || seen ? kSlack - above : limit;
+      if (kSeenByM)
+        m = (moves || seen) && m == 0.f ? 0x1p-100f : m;
+      else
+        limit = moves || seen ? kSlack - above : limit;
       l *= fix;
-      if (kEvens) exact *= fix, rounded *= fix;
+      if (kEvens) exact *= fix;
+      if (kEvens && I8) rounded *= fix;
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[r] -= by;
 #pragma unroll
@@ -446,13 +457,14 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   };
   // scores -> pf (buf, sub: the half tile's value scales)
   auto weights = [&](const f32x16& x, int buf, int sub) {
+    float sum = 0.f;
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
       float w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         w[j] = __builtin_amdgcn_exp2f(x[q4 * 4 + j]);
-        if (I8 || STATS) l += w[j];
+        if (I8) l += w[j];
       }
       if (I8) {
         const f32x4 f = *(const f32x4*)(lds.vs[buf] + sub * 32 + (q4 >> 1) * 16 + half * 8 + (q4 & 1) * 4);
@@ -461,12 +473,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
       }
       pf[q4 >> 1][2 * (q4 & 1)] = pack_pair(w[0], w[1]);
       pf[q4 >> 1][2 * (q4 & 1) + 1] = pack_pair(w[2], w[3]);
-      if (kEvens) {
-        exact += (w[0] + w[1]) + (w[2] + w[3]);
+      if (kEvens) sum += (w[0] + w[1]) + (w[2] + w[3]);
+      if (kEvens && I8)
         rounded = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], rounded));
-      }
-      if (!I8 && !STATS) l = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], l));
+      if (!I8) l = add_pair(pf[q4 >> 1][2 * (q4 & 1)], add_pair(pf[q4 >> 1][2 * (q4 & 1) + 1], l));
     }
+    if (kEvens) exact += sum;
   };
   auto products = [&](int from, int to) {
 #pragma unroll
@@ -686,7 +698,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   }
   l = add_xor32(l);
   if (kEvens) {
-    const float by = even_by(add_xor32(exact), add_xor32(rounded));
+    exact = add_xor32(exact);
+    const float by = even_by(exact, I8 ? add_xor32(rounded) : l);
+    if (!I8) l = exact;
 #pragma unroll
     for (int i = 0; i < kO; ++i)
 #pragma unroll
@@ -731,7 +745,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
         *(f32x4*)(part.o + to * D + i * 32 + 8 * (r >> 2) + 4 * half) =
             f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
     if (half == 0) {
-      part.ml[2 * to] = limit >= 0.f ? m : kUnseen;
+      part.ml[2 * to] = row_sees() ? m : kUnseen;
       part.ml[2 * to + 1] = l;
     }
     return;
@@ -739,7 +753,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheView c, AttnArgs
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   const int out_token = out_row / G;
   if (STATS && half == 0)
-    keep_stats(a, s.first + out_token, h * G + out_row - out_token * G, limit >= 0.f ? m : kUnseen, l);
+    keep_stats(a, s.first + out_token, h * G + out_row - out_token * G, row_sees() ? m : kUnseen, l);
   uint16_t* out = a.out + ((int64_t)(s.first + out_token) * a.heads + h * G + (out_row - out_token * G)) * D;
 #pragma unroll
   for (int i = 0; i < kO; ++i)
