@@ -73,3 +73,32 @@ def test_infinite_adapters(gpu_device, tokens):
     want[32:] = float("-inf")
     assert torch.equal(out[0], want) and torch.equal(out[1], -want)
     assert bool(torch.isnan(out[2:]).all())
+
+
+@pytest.mark.parametrize("tokens", [60, 300, 3000])
+def test_two_streams_at_once(gpu_device, tokens):
+    """A captured call replayed on one stream beside eager calls on two others, with nothing between them."""
+    announce(f"adapters on three streams T={tokens}")
+    p = Problem(5, 512, (256, 128), 32, seed=23)
+    inputs = [p.inputs(tokens) + (torch.randint(-1, 5, (tokens,), generator=p.g, device=DEV),) for _ in range(3)]
+    alone = [p.adapters.forward(*x) for x in inputs]
+    for (x, base, index), want in zip(inputs, alone):
+        p.check(x, base, index, want)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        captured = p.adapters.forward(*inputs[0])
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(8):
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        for i in (1, 2):
+            with torch.cuda.stream(streams[i]):
+                outs[i - 1].append(p.adapters.forward(*inputs[i]))
+    torch.cuda.synchronize()
+    assert torch.equal(captured, alone[0])
+    for i in (1, 2):
+        assert all(torch.equal(out, alone[i]) for out in outs[i - 1])
+    p.adapters.check_status()

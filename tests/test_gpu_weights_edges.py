@@ -3,8 +3,9 @@ tests."""
 import pytest
 import torch
 
-from attn_cases import DEV, causal, dense, generator, make_problem, put, randn, reference, split_rows
-from test_gpu_weights import announce, check_weights, starts_of
+from attn_cases import DEV, check_rows, causal, dense, generator, make_problem, put, randn, reference, split_rows
+from nano_ktrans_amd import _native as N
+from test_gpu_weights import added_weights, announce, check_weights, start_weights, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,108 @@ def test_bf16_outputs_are_as_exact_as_forwards(gpu_device, heads, kv_heads, dim,
         size = y.double().abs().clamp(min=2.0 ** -6)
         assert bool(((x.double() - y.double()).abs() <= 2.0 ** -7 * size).all())
     assert squares[0] <= 1.01 ** 2 * squares[1], f"rms {squares[0] ** 0.5} where forward has {squares[1] ** 0.5}"
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 128), (14, 2, 64)])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 1, 2], [8, 5, 0], [150, 1, 300]])
+def test_lengths_that_are_cut(gpu_device, heads, kv_heads, dim, fmt, counts):
+    """Lengths past max_seq_len, past a sequence's pages, negative: reported; the rows keep their positions and see (and give
+    weight to) the tokens up to the cut.  Tolerances as in test_gpu_weights.py."""
+    announce(f"weights, cut lengths {heads}/{kv_heads}/{dim} {fmt} rows {counts}")
+    told, cut = [700, 450, -3], [600, 384, 0]
+    p = make_problem([700, 384, 40], heads=heads, kv_heads=kv_heads, dim=dim, fmt=fmt, page=64, seed=35)
+    p.table[1, 6:] = -1  # (the second sequence's pages end at 384: the rest is reported and not seen)
+    lens = torch.tensor(told, dtype=torch.int32, device=DEV)
+    g = generator(36)
+    q = randn(g, sum(counts), heads, dim)
+    before = start_weights(g, 3, kv_heads, 640)
+    after = before.clone()
+    got = p.attn.forward_weights(q, after, p.table, lens, starts_of(counts), max_queries=max(counts), max_seq_len=600)
+    seen = p.attn.status()
+    assert seen["bad_length"] and seen["bad_page"]
+    starts = split_rows(counts)
+    for b, n in enumerate(counts):
+        mine = slice(starts[b], starts[b + 1])
+        k, v = p.k[b][:cut[b]], p.v[b][:cut[b]]
+        sees = causal(n, max(told[b], 0))[:, :cut[b]]
+        want, A = reference(q[mine], k, v, sees, p.attn.scale)
+        check_rows(got[mine], want, A)
+        add = added_weights(q[mine], k, sees, p.attn.scale, n)
+        was, now = before[b].double(), after[b].double()
+        R = n * heads // kv_heads
+        bound = (2.0 ** -9.9 + (R + 8) * 2.0 ** -24) * add + 2.0 ** -24 * (was[:, :cut[b]] + add)
+        assert bool(((now[:, :cut[b]] - was[:, :cut[b]] - add).abs() <= bound).all())
+        assert torch.equal(after[b][:, cut[b]:], before[b][:, cut[b]:])
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("counts,most", [([5, 2], 2), ([40, 1], 16), ([300, 20], 70)])
+def test_more_rows_than_the_bound(gpu_device, fmt, counts, most):
+    """Rows past max_queries are reported, left as they were, and give nothing."""
+    announce(f"weights, rows {counts} past {most} {fmt}")
+    lengths = [400, 90]
+    p = make_problem(lengths, heads=8, kv_heads=2, dim=128, fmt=fmt, page=64, seed=37)
+    g = generator(38)
+    q = randn(g, sum(counts), 8, 128)
+    before = start_weights(g, 2, 2, 448)
+    after = before.clone()
+    out = torch.full((sum(counts), 8, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    p.attn.forward_weights(q, after, p.table, p.lens, starts_of(counts), max_queries=most, out=out)
+    with pytest.raises(N.NativeError, match="bad_length"):
+        p.attn.check_status()
+    starts = split_rows(counts)
+    for b, (n, length) in enumerate(zip(counts, lengths)):
+        done = min(n, most)
+        mine = slice(starts[b], starts[b] + done)
+        sees = causal(n, length)[:done]
+        want, A = reference(q[mine], p.k[b], p.v[b], sees, p.attn.scale)
+        check_rows(out[mine], want, A)
+        assert bool((out[starts[b] + done:starts[b + 1]] == 7.0).all())
+        add = added_weights(q[mine], p.k[b], sees, p.attn.scale, done)
+        was, now = before[b].double()[:, :length], after[b].double()[:, :length]
+        bound = (2.0 ** -9.9 + (done * 4 + 8) * 2.0 ** -24) * add + 2.0 ** -24 * (was + add)
+        assert bool(((now - was - add).abs() <= bound).all())
+        assert torch.equal(after[b][:, length:], before[b][:, length:])
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_two_streams_at_once(gpu_device, fmt):
+    """A captured decode step replayed on one stream, prompts on another and decode steps on a third, with nothing
+    between them: each gives what it gives alone, bit for bit."""
+    announce(f"weights on three streams {fmt}")
+    lengths = [3000, 33, 2400]
+    p = make_problem(lengths, heads=32, kv_heads=4, dim=128, fmt=fmt, page=64, seed=39)
+    g = generator(40)
+    q, rows, counts = randn(g, 3, 32, 128), randn(g, 730, 32, 128), [700, 20, 10]
+    starts, width = starts_of(counts), p.table.shape[1] * 64
+
+    def decode(w):
+        return p.attn.forward_weights(q, w, p.table, p.lens, max_seq_len=3000)
+
+    def prompt(w):
+        return p.attn.forward_weights(rows, w, p.table, p.lens, starts, max_queries=700, max_seq_len=3000)
+
+    alone = [torch.zeros(3, 4, width, device=DEV) for _ in range(2)]
+    steps = [decode(alone[0]) for _ in range(6)]
+    prompts = [prompt(alone[1]) for _ in range(6)]
+    together = [torch.zeros_like(alone[0]) for _ in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        captured = decode(together[0])
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(6):
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        with torch.cuda.stream(streams[1]):
+            outs[0].append(prompt(together[1]))
+        with torch.cuda.stream(streams[2]):
+            outs[1].append(decode(together[2]))
+    torch.cuda.synchronize()
+    assert torch.equal(captured, steps[-1]) and torch.equal(together[0], alone[0])
+    assert all(torch.equal(a, b) for a, b in zip(outs[0], prompts)) and torch.equal(together[1], alone[1])
+    assert all(torch.equal(a, b) for a, b in zip(outs[1], steps)) and torch.equal(together[2], alone[0])
+    p.attn.check_status()
