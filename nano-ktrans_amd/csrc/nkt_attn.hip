@@ -827,11 +827,11 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
 #pragma unroll
   for (int i = 0; i < kO; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = kUnseen, l = 0.f, above = I8 ? 0.f : kSlack;
-  // int8, beside the weights of cached tokens: weight x scale before and after it is rounded
-  // to bf16, whose sums' quotient takes what the roundings have in common out of the output
-  // (up to 300 tokens its error against 64 bits is up to 0.0027 without it)
-  constexpr bool kEvens = I8 && STATS;
-  float exact = 0.f, rounded = 0.f;
+  // Beside the weights of cached tokens: the sum of weights (int8: x scale) before they are
+  // rounded to bf16 for the product and after it; the quotient takes what the roundings have in
+  // common out of the output.
+  constexpr bool kEvens = STATS;
+  float exact = 0.f, rounded = 0.f;  // (exact: int8; else that is l)
   const float scale2 = a.scale * kLog2e;
   const int mask = (1 << c.page_shift) - 1;
   const int krow = (col >> 2) * (KS / 4) + (col & 3);
@@ -972,7 +972,8 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
       const float fix = to > kUnseen ? __builtin_amdgcn_exp2f(m - to) : 1.f;
       m = to;
       l *= fix;
-      if (kEvens) exact *= fix, rounded *= fix;
+      if (kEvens && I8) exact *= fix;
+      if (kEvens) rounded *= fix;
 #pragma unroll
       for (int i = 0; i < kO; ++i) o[i] *= fix;
     }
@@ -1012,10 +1013,8 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
     for (int t = 0; t < NT; ++t) {
       pf[t >> 1][2 * (t & 1)] = pack_pair(st[t][0], st[t][1]);
       pf[t >> 1][2 * (t & 1) + 1] = pack_pair(st[t][2], st[t][3]);
-      if (kEvens) {
-        exact += (st[t][0] + st[t][1]) + (st[t][2] + st[t][3]);
-        rounded = add_pair(pf[t >> 1][2 * (t & 1)], add_pair(pf[t >> 1][2 * (t & 1) + 1], rounded));
-      }
+      if (kEvens && I8) exact += (st[t][0] + st[t][1]) + (st[t][2] + st[t][3]);
+      if (kEvens) rounded = add_pair(pf[t >> 1][2 * (t & 1)], add_pair(pf[t >> 1][2 * (t & 1) + 1], rounded));
     }
 #pragma unroll
     for (int i = 0; i < kO; ++i) {
@@ -1055,7 +1054,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(CacheView c, AttnArgs 
   // the waves' results, added in order
   l = add_xor32(add_xor16(l));
   if (kEvens) {
-    const float by = even_by(add_xor32(add_xor16(exact)), add_xor32(add_xor16(rounded)));
+    const float by = even_by(I8 ? add_xor32(add_xor16(exact)) : l, add_xor32(add_xor16(rounded)));
 #pragma unroll
     for (int i = 0; i < kO; ++i) o[i] *= by;
   }

@@ -11,16 +11,19 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,counts", [
-    (8, 2, 128, [40]), (8, 2, 128, [16]), (14, 2, 64, [40]), (14, 2, 64, [8]), (4, 4, 128, [300]), (32, 4, 128, [5, 3])])
+    (8, 2, 128, [40]), (8, 2, 128, [16]), (14, 2, 64, [40]), (14, 2, 64, [8]), (4, 4, 128, [300]), (32, 4, 128, [5, 3]),
+    (32, 4, 128, [1]), (8, 2, 128, [4, 1]), (14, 2, 64, [2])])
 def test_later_token_that_outweighs_the_rest(gpu_device, heads, kv_heads, dim, counts):
-    """bf16, tiles.  A row's scores, in powers of two: 0 for token 0, 7 to 8 (by row) for token 70, far less for all
-    others; only token 70 has a value.  A row's largest weight so far may lie 2^8 below 1 when token 70 comes, so
-    that its weight w is no power of two and rounding it for the product changes it by up to 2^-8 of itself.  Divided
-    by a sum of the rounded weights that is gone: with r = 1 + e of each, the quotient is off by p0 |e0 - e1|, p0 <=
-    2^-7 the weight of token 0, under 2^-14 of it.  A score is a sum of two terms under 2^4 in size, off by 2^-20 at
-    most, which moves the quotient by p0 2^-20.  What is left is the output's rounding: (2^-8 + 2^-13) |want|."""
+    """bf16.  A row's scores, in powers of two: 0 for token 0, 7 to 8 (by row) for a later token of the same wave, far
+    less for all others; only the later token has a value.  A row's largest weight so far may lie 2^8 below 1 when
+    that comes, so that its weight w is no power of two and rounding it for the product changes it by up to 2^-8 of
+    itself.  Divided by a sum of the rounded weights that is gone: with r = 1 + e of each, the quotient is off by p0
+    |e0 - e1|, p0 <= 2^-7 the weight of token 0, under 2^-14 of it.  A score is a sum of two terms under 2^4 in size,
+    off by 2^-20 at most, which moves the quotient by p0 2^-20.  What is left is the output's rounding: (2^-8 + 2^-13)
+    |want|."""
     announce(f"weights, later token {heads}/{kv_heads}/{dim} rows {counts}")
-    lengths = [100 + n for n in counts]
+    late = 70 if max(counts) * heads // kv_heads > 16 else 130  # (few rows: a wave's steps are 128 tokens apart)
+    lengths = [late + 30 + n for n in counts]
     p = make_problem(lengths, heads=heads, kv_heads=kv_heads, dim=dim, fmt="bf16", page=64, seed=31)
     g = generator(32)
     rows = sum(counts)
@@ -33,9 +36,9 @@ def test_later_token_that_outweighs_the_rest(gpu_device, heads, kv_heads, dim, c
     for b, length in enumerate(lengths):
         k, v = torch.zeros(length, kv_heads, dim, device=DEV), torch.zeros(length, kv_heads, dim, device=DEV)
         k[:, :, 0] = -64.0 / unit
-        k[0, :, 0] = k[70, :, 0] = 0.0
-        k[70, :, 1] = 1.0 / unit
-        v[70] = 1 + torch.rand(kv_heads, dim, generator=g, device=DEV)
+        k[0, :, 0] = k[late, :, 0] = 0.0
+        k[late, :, 1] = 1.0 / unit
+        v[late] = 1 + torch.rand(kv_heads, dim, generator=g, device=DEV)
         at = torch.arange(length, device=DEV)
         slots = p.attn.slots(p.table, torch.full_like(at, b), at)
         put(p.attn, slots, k, v)
