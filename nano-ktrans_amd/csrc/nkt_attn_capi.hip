@@ -113,7 +113,8 @@ bool check_rows(const char* name, int64_t seq_stride, int64_t head_stride, int64
 }
 
 bool check_evict_sizes(const AttnHandle* h, int num_seqs, int max_seq_len, char* err, size_t len) {
-  // (fill_kernel has up to 2048 workgroups more than sequences x heads)
+  // (the selection has workgroups of 1024 threads, of which a launch takes under 2^32; fill_kernel up to 4095
+  // workgroups more than sequences x heads)
   if (num_seqs < 0 || (int64_t)num_seqs * h->cache.kv_heads > kMaxGroups / 4) {
     set_err(err, len, "num_seqs=%d: negative, or over 2^22 of %d heads", num_seqs, h->cache.kv_heads);
     return false;

@@ -442,9 +442,13 @@ __device__ __forceinline__ Moves moves_of(const CacheView& c, const EvictArgs& e
   return m;
 }
 
-// The whole of it by one workgroup per (sequence, head): for short sequences, where
-// launches cost more than the moves.  2112 tokens to 2048, 4 heads, bf16: 20 us; in three
-// launches 10.5 + 9.4 + 6.6 and what lies between them.
+// The whole of it by one workgroup per (sequence, head), for sequences of up to 4096 tokens.
+// Calls in us, in one launch and in three, 4 heads: one sequence of 2112 tokens to 2048 20
+// and 25, of 4096 to 4032 21 and 26, 64 of them (bf16) 27 and 78; but one of 1024 to 512 23
+// and 18, of 4096 to 1024 49 and 22, 16 of these 55 and 38, 64 of these 91 and 94 (int8 61
+// and 58), of 1024 to 512 31 and 37.  A program that evicts as it goes moves few tokens at a
+// time; where a whole prompt is cut at once, sixteen waves per head do what the three launches
+// give to the whole card, and lose until there are sequences enough.
 template <int D, bool I8, int N>
 __global__ __launch_bounds__(kSelectThreads) void evict_kernel(CacheView c, EvictArgs e) {
   __shared__ SelectLds lds;

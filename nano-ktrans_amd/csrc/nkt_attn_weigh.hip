@@ -216,11 +216,12 @@ __global__ __launch_bounds__(kThreads) void recount_kernel(CacheView c, WeighArg
 // held in registers: a lane's column is a row and its registers are tokens, so
 // that the sum over rows stays in the lane until the end, and the row's maximum
 // and sum are one value per lane.  The waves share the rows: 32 at a time go
-// straight into LDS, two steps ahead (chunk c of row r at c ^ key(r), so that the
-// rows' same chunk lies in 16 places of the 256 bytes that LDS reads at a time).
+// straight into LDS, three steps ahead (one where rows may not see all tokens; chunk
+// c of row r at c ^ key(r), so that the rows' same chunk lies in 16 places of the 256
+// bytes that LDS reads at a time).
 //
 // Bound by the matrix cores and an exponential per score beside them: a prompt of
-// 8192 tokens that all count, 32 / 4 heads, D = 128, bf16: 356 us, 0.77 PFLOP/s of the
+// 8192 tokens that all count, 32 / 4 heads, D = 128, bf16: 352 us, 0.78 PFLOP/s of the
 // repeated product alone (kept scores would be 4.3 GB each way); three chunks of up to
 // 1021 tokens on up to 9000, 32 / 8 heads, int8, of which the last 64 tokens count:
 // 31 us.

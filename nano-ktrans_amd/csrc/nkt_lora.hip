@@ -72,7 +72,7 @@ int tile_groups(int tiles) { return tiles < 64 ? tiles : (tiles + 7) / 8 * 8; }
 // ---------------------------------------------------------------------------
 // Tokens by adapter, in tiles of 32 that each have one adapter (kNone: without one,
 // where these have to be copied; kPast: no tile), for more tokens than one launch
-// takes.  By one workgroup: the counts stay in LDS, and 8192 tokens take 9 us (1000 about
+// takes.  By one workgroup: the counts stay in LDS, and 8418 tokens take 9 us (1000 about
 // 5, mostly the launch).  Which place of its adapter's tiles a token gets depends on
 // the order in which waves arrive; what is computed for it does not depend on its
 // place.
@@ -335,8 +335,16 @@ __global__ __launch_bounds__(KWAVES * 64) void shrink_kernel(LoraView v, LoraArg
 // columns.  A wave computes 32 tokens x 64 columns at a time: tokens in registers, a
 // pair of neighbouring columns in a lane, so that 32 lanes read and write 128 bytes of
 // a token's row.  The base of all its turns is asked for at once.  KS = R / 16.
-// Bound by the base and the output: 8192 tokens of 6144 columns, rank 64, take 56 us,
-// 3.6 TB/s.
+// Bound by the base and the output: 8418 tokens of 6144 columns, ranks 64 and 32, take 57
+// us, 3.6 TB/s; B, read anew by every tile of 32 tokens, is about 150 MB through the L2
+// beside them.
+//
+// Ranks that fill KS or half of it have copies of their own, whose loads are all asked for
+// at once.  Whole calls of 8192 tokens on 4096 -> 6144 columns, in us: R = 64, rank 64 103
+// (by the loop over ranks 113), 32 93 (94), by the loop 48 110 and 16 92 (105 and 90 in a
+// kernel that has nothing but the loop); R = 128, rank 128 151 (163), 64 112 (114), 96 160
+// (138), 32 107 (96); R = 32 on 2048 -> 5120, rank 32 58 (60), 24 58 (60).  300 tokens
+// differ by 1.5 at most.
 // ---------------------------------------------------------------------------
 constexpr int kTurns = 2;  // of a wave, at most
 
@@ -447,8 +455,9 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(LoraView v, LoraArgs a, 
 // computes the part's low for itself (R x in_features values of A from the L2, which
 // cost less than a second launch) and leaves it in LDS; its waves' base and B are on
 // their way meanwhile.  Bound by latency: a launch, x and A, B.  One token of 2048
-// features to 5120 columns, rank 16: 8.2 us; 64 tokens of 24 adapters of rank 32, 4096
-// features and columns: 16.7 us.
+// features to 5120 columns, rank 16: 8.9 us; 64 tokens of 24 adapters of rank 32, 4096
+// features and columns: 15.5 us, of which x is a part: all 32 rows of the tile, also those
+// of other adapters.
 // ---------------------------------------------------------------------------
 template <int KS>
 __global__ __launch_bounds__(512) void both_kernel(LoraView v, LoraArgs a, int slots, int per_wave) {
@@ -575,12 +584,25 @@ __global__ __launch_bounds__(512) void both_kernel(LoraView v, LoraArgs a, int s
   }
 }
 
-// One launch for up to 64 tokens.  One launch against grouped tokens (us; 8 adapters of
-// rank 16 on 2048 -> 5120, 24 of rank 32 on 4096 -> 4096, 8 of rank 64 on 4096 -> 6144):
-//     8 tokens   8.9 / 13.5    10.9 / 15.5    16.6 / 16.4
-//    32 tokens   9.4 / 13.7    15.7 / 16.2    17.7 / 16.6
-//    64 tokens   9.7 / 13.7    16.8 / 16.4    19.4 / 17.1, of one adapter 14.7 / 16.7
-// and one launch grows with each further tile and adapter of a tile.
+// One launch for up to 64 tokens: three launches cost the host about 8 us more in a call
+// outside of a graph, which then takes 19 to 20 at least.  One launch against grouped tokens,
+// us on the GPU, and of whole calls in brackets where the GPU is not all of them; adapters
+// dealt out in turn (of one adapter):
+//                                        1 token       8 tokens      32 tokens     64 tokens
+//   8 of rank 16, 2048 -> 5120            8.5 / 12.3    9.2 / 12.7    9.4 / 12.7    9.7 / 12.7  (9.3 / 13.1)
+//        whole calls                       12 / 20       12 / 20       12 / 20       12 / 19
+//   24 of rank 32, 4096 -> 4096          10.3 / 14.2   11.0 / 14.7   15.5 / 15.2   17.0 / 15.2  (12.4 / 15.2)
+//        whole calls                       12 / 20       12 / 20       15 / 19       17 / 20
+//   64 of rank 32, 4096 -> 4096          10.3 / 15.0   11.0 / 15.4   15.9 / 16.4   18.4 / 19.6  (15.5 / 16.4)
+//   8 of rank 64, 4096 -> 6144           13.9 / 14.6   16.8 / 15.7   17.8 / 15.7   19.4 / 16.0  (14.9 / 15.9)
+//        whole calls                       14 / 20       16 / 19       17 / 19       19 / 19
+//   8 of rank 128, 4096 -> 6144          23.8 / 15.5   28.4 / 18.4   30.6 / 18.5   33.6 / 19.2  (24.7 / 16.4)
+//   64 of rank 128, 4096 -> 4096         23.6 / 15.7   27.5 / 16.6   36.6 / 23.3   44.3 / 39.8  (32.5 / 18.9)
+//   8 of rank 16, 4096 -> 28672          10.5 / 13.8   12.6 / 15.6   14.0 / 15.9   17.3 / 16.2  (15.2 / 15.5)
+//   64 of rank 16, 4096 -> 28672         10.5 / 14.6   12.5 / 16.4   30.8 / 25.6   46.5 / 30.7  (47.1 / 22.8)
+// So the number of tokens alone chooses right up to rank 64 and a few thousand columns;
+// ranks over 64, and wide outputs beside many adapters (whose workgroups are given more
+// columns by the adapters that there could be), lose by it.
 constexpr int kBothTokens = 64;
 
 // Tiles of grouped tokens: each group may leave one tile open.
@@ -619,8 +641,9 @@ hipError_t launch_lora(const LoraView& v, LoraArgs a, void* workspace, hipStream
     const int tiles = (a.tokens + kTile - 1) / kTile;
     const int most = v.adapters < kTile ? v.adapters : kTile;
     const int slots = (a.tokens < most ? a.tokens : most) + (copies ? 1 : 0);
-    // more columns per workgroup once these are more than run at a time (64 tokens of 24
-    // adapters, 4096 columns: 16.8 us, with 512 columns each 27.2)
+    // more columns per workgroup once these are more than run at a time, had the tile all
+    // adapters that it could have (64 tokens of 24 adapters, 4096 columns: 16.8 us, with 512
+    // columns each 27.2)
     int chunks = 0, per_wave = 1;
     for (;; per_wave *= 2) {
       chunks = 0;
